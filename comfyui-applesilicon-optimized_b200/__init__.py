@@ -13,6 +13,7 @@ NODE_CLASS_MAPPINGS = {}
 NODE_DISPLAY_NAME_MAPPINGS = {}
 
 from ._patches import _native  # noqa: E402,F401  (registers torch.ops.b200q)
+from . import block_norm, kv8, w4  # noqa: E402,F401  (register theirs)
 
 
 def bootstrap():

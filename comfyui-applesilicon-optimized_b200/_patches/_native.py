@@ -35,6 +35,10 @@ _patches/fp8_ext/fp8_matmul2d.mm:355-360, _patches/fp8s_ext/w8a16_gemm.mm:316-32
   fp8_scaled_mm(a, w_nk, scale_a, scale_b, scale_result, bias, out_dtype, act)
   w8a16_linear(x, w_nk e4m3, w_scale, bias, act, out_dtype)
   fp8_decode(t, out_dtype)
+
+The low-bit decode operators are registered beside their bindings: ``w4.py``
+(4-bit weight linears), ``block_norm.py`` (norms before and after a block) and
+``kv8.py`` (paged 8-bit key/value cache and attention).
 """
 
 import ctypes
@@ -106,6 +110,21 @@ _SIGNATURES = {
                                            _i64, _i64, _i64, _vp], _int),
     "b200q_i8_mlp_bridge_prequant": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                                       _int, _i64, _vp, _vp, _i64, _vp, _vp], _int),
+    # low-bit decode operators (bindings: ../w4.py, ../block_norm.py, ../kv8.py)
+    "b200q_w4a16_workspace_size": ([_i64, _i64, _i64], _sz),
+    "b200q_w4a16_linear": ([_vp, _int, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp, _int, _int, _vp,
+                            _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp], _int),
+    "b200q_block_norm": ([_vp, _i64, _vp, _i64, _int, _int, _vp, _int, _vp, _i64, ctypes.c_float,
+                          _int, _vp, _int, _vp, _i64, _vp, _i64, _int, _i64, ctypes.c_float, _vp,
+                          _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp], _int),
+    "b200q_kv8_append": ([_vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                          _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp], _int),
+    "b200q_kv8_gather": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                          _vp, _vp, _int, _i64, _i64, _vp], _int),
+    "b200q_kv8_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64], _sz),
+    "b200q_kv8_attention": ([_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                             _i64, _i64, _vp, _i64, _i64, _vp, _i64, _int, ctypes.c_float, _vp,
+                             _vp, _vp, _vp, _sz, _vp], _int),
 }
 
 
@@ -158,6 +177,24 @@ def _stream(t):
 
 def _p(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+class _SameDevice:
+    """The tensors' device is current already."""
+
+    def __enter__(self):
+        pass
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME_DEVICE = _SameDevice()
+
+
+def device_of(dev):
+    """Context that makes ``dev`` current (nothing to do when it is)."""
+    return _SAME_DEVICE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
 
 
 def _require_cuda(*ts):

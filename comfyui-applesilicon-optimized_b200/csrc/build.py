@@ -13,41 +13,81 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PACK = os.path.dirname(HERE)
 ROOT = os.path.dirname(PACK)
 OUT = os.path.join(PACK, "_lib", "libb200q.so")
-SOURCES = ["capi.cu", "gemm8.cuh", "prologue.cuh", "qkv_rope.cuh", "quant.cuh", "w8a16.cuh", "w8a16_planes.cuh", "numerics.cuh", "ptx.cuh"]
 HEADER = os.path.join(ROOT, "include", "b200q.h")
+# translation unit -> the headers it includes (each is compiled on its own, in
+# parallel, and only when one of its sources is newer than its object)
+UNITS = {
+    "capi.cu": ["host.h", "gemm8.cuh", "prologue.cuh", "qkv_rope.cuh", "quant.cuh", "w8a16.cuh",
+                "w8a16_planes.cuh", "numerics.cuh", "ptx.cuh"],
+    "lowbit.cu": ["host.h", "w4a16.cuh", "block_norm.cuh", "kv8.cuh", "numerics.cuh", "ptx.cuh"],
+}
+SOURCES = sorted({f for unit, deps in UNITS.items() for f in (unit, *deps)})
+FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
+         "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
 
 
-def nvcc_cmd(out=OUT, extra=()):
+def nvcc_cmd(unit, out, extra=()):
     nvcc = os.environ.get("NVCC", "nvcc")
-    return [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
-            "-shared", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
-            "-o", out, os.path.join(HERE, "capi.cu"), *extra]
+    return [nvcc, *FLAGS, "-c", "-o", out, os.path.join(HERE, unit), *extra]
+
+
+def link_cmd(objects, out=OUT):
+    nvcc = os.environ.get("NVCC", "nvcc")
+    return [nvcc, *FLAGS, "-shared", "-o", out, *objects]
+
+
+def object_of(unit):
+    return os.path.join(PACK, "_lib", unit.replace(".cu", ".o"))
+
+
+def newer(target, sources):
+    """True when `target` exists and no source is newer."""
+    if not os.path.exists(target):
+        return False
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(s) <= t for s in sources if os.path.exists(s))
+
+
+def unit_sources(unit):
+    return [os.path.join(HERE, f) for f in (unit, *UNITS[unit])] + [HEADER]
 
 
 def up_to_date():
-    if not os.path.exists(OUT):
-        return False
-    t = os.path.getmtime(OUT)
-    deps = [os.path.join(HERE, s) for s in SOURCES] + [HEADER]
-    return all(os.path.getmtime(d) <= t for d in deps if os.path.exists(d))
+    return newer(OUT, [s for unit in UNITS for s in unit_sources(unit)])
 
 
 def build(force=False, verbose=False):
     if not force and up_to_date():
         return OUT
     os.makedirs(os.path.dirname(OUT), exist_ok=True)
-    cmd = nvcc_cmd()
-    if verbose:
-        print(" ".join(cmd))
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    msg = "\n".join(l for l in (r.stdout + r.stderr).splitlines()
-                    if "compute_" not in l or "Warning" not in l)
+    jobs = []
+    for unit in UNITS:
+        obj = object_of(unit)
+        if not force and newer(obj, unit_sources(unit)):
+            continue
+        cmd = nvcc_cmd(unit, obj, ["-Xptxas", "-v"] if verbose == "ptxas" else ())
+        if verbose:
+            print(" ".join(cmd))
+        jobs.append((obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT,
+                                           text=True)))
+    failed = []
+    for obj, job in jobs:
+        text = job.communicate()[0]
+        msg = "\n".join(l for l in text.splitlines() if "compute_" not in l or "Warning" not in l)
+        if job.returncode != 0:
+            failed.append(f"nvcc failed ({job.returncode}):\n{msg}")
+            if os.path.exists(obj):
+                os.remove(obj)
+        elif verbose and msg.strip():
+            print(msg)
+    if failed:
+        raise RuntimeError("\n".join(failed))
+    r = subprocess.run(link_cmd([object_of(u) for u in UNITS]), capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{msg}")
-    if verbose and msg.strip():
-        print(msg)
+        raise RuntimeError(f"link failed ({r.returncode}):\n{r.stdout}{r.stderr}")
     return OUT
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    v = "ptxas" if "--ptxas" in sys.argv else "--verbose" in sys.argv
+    print(build(force="--force" in sys.argv, verbose=v))

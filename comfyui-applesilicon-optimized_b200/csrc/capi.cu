@@ -14,6 +14,7 @@
 
 #include "../../include/b200q.h"
 #include "gemm8.cuh"
+#include "host.h"
 #include "qkv_rope.cuh"
 #include "quant.cuh"
 #include "w8a16.cuh"
@@ -943,6 +944,28 @@ int grid_for(int64_t work, int per_block, const DeviceInfo* d) {
 
 }  // namespace
 
+// ------------------------------------------------------------ shared with the other units
+namespace b200q {
+namespace host {
+
+int device_sms() {
+  const DeviceInfo* d = current_device();
+  return d ? d->num_sms : 0;
+}
+int finish_launch() { return ::finish_launch(); }
+bool pdl_on() { return pdl_launch_on(); }
+
+int gemm16_scaled(bool f16, const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M,
+                  int64_t N, int64_t K, const EpiArgs& ep, cudaStream_t st) {
+  const DeviceInfo* d = current_device();
+  if (!d) return B200Q_ERR_UNSUPPORTED;
+  if (f16) return gemm16<MmaKind::F16, kEpiScaled>(d, a, lda, w, ldw, M, N, K, ep, st);
+  return gemm16<MmaKind::BF16, kEpiScaled>(d, a, lda, w, ldw, M, N, K, ep, st);
+}
+
+}  // namespace host
+}  // namespace b200q
+
 // =====================================================================  C ABI
 extern "C" {
 
@@ -973,7 +996,11 @@ int b200q_get_device_status(unsigned int* status, int reset) {
     if (cudaMemcpyToSymbol(g_device_status, &zero, sizeof(unsigned int)) != cudaSuccess)
       return B200Q_ERR_CUDA;
   }
-  return B200Q_OK;
+  // each translation unit has its own status word
+  unsigned int other = 0;
+  const int st = host::lowbit_device_status(&other, reset != 0);
+  *status |= other;
+  return st;
 }
 
 int b200q_quant_rowwise_i8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ldx,

@@ -1,0 +1,558 @@
+// A paged 8-bit key/value cache: int8 codes [pages, heads, T, D] and one fp32
+// scale per (page, head), value = code * scale.  A page is a block of T tokens;
+// block_table[b][i] is the page of sequence b's tokens [i*T, (i+1)*T).
+//
+//   append     writes new tokens behind each sequence's length.  A block's scale
+//              is max(its scale so far if it holds tokens, max|new| / 127): it
+//              only grows, and codes already there are requantized when it does.
+//   gather     reads a range of tokens back as 16-bit / fp32 values.
+//   attention  softmax(q K^T) V over the cache.
+//
+// Page numbers come from device memory and are checked against the pool before
+// any access; a bad one sets the status word's bit 1 and its tokens are skipped.
+#pragma once
+
+#include "numerics.cuh"
+#include "ptx.cuh"
+
+namespace b200q {
+
+struct Kv8Cache {
+  int8_t *k, *v;           // [pages, heads, T, D]
+  float *ks, *vs;          // [pages, heads]
+  const int32_t* table;    // [B, max_blocks]
+  int64_t ld_table;
+  int max_blocks, pages, heads, T, D, log_t;
+};
+
+// Page of block `blk` of sequence b, or -1 (flagged) if the table holds no page there.
+__device__ __forceinline__ int kv8_page(const Kv8Cache& c, int b, int blk) {
+  if (blk < 0 || blk >= c.max_blocks) {
+    atomicOr(&g_device_status, kStatusBadArgument);
+    return -1;
+  }
+  const int p = __ldg(c.table + b * c.ld_table + blk);
+  if (p < 0 || p >= c.pages) {
+    atomicOr(&g_device_status, kStatusBadArgument);
+    return -1;
+  }
+  return p;
+}
+
+// ---------------------------------------------------------------- append
+struct Kv8AppendArgs {
+  Kv8Cache c;
+  const void *k, *v;  // [B, heads, S, D], unit inner stride, 16-byte aligned rows
+  int64_t kb, kh, kt, vb, vh, vt;  // strides in elements
+  const int32_t* start;   // [B] tokens already in the cache
+  const int32_t* counts;  // [B] new tokens (<= S), or null: S each
+  int B, S;
+};
+
+constexpr int kKvThreads = 256;
+
+// One CTA per (block, head, sequence, K or V).  NV: 8-value vectors a thread
+// holds (T * D <= 2048 * NV).
+template <typename T, int NV>
+__global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendArgs a) {
+  __shared__ uint32_t wmax[kKvThreads / 32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const Kv8Cache& c = a.c;
+  const bool is_v = blockIdx.z & 1;
+  const int b = blockIdx.z >> 1, h = blockIdx.y, tid = threadIdx.x;
+  const int start = a.start[b];
+  const int count = min(a.counts ? a.counts[b] : a.S, a.S);
+  if (start < 0 || count <= 0) return;
+  const int blk = (start >> c.log_t) + blockIdx.x;
+  const int64_t first = static_cast<int64_t>(blk) << c.log_t;  // the block's first position
+  const int64_t end = static_cast<int64_t>(start) + count;
+  if (first >= end) return;
+  const int page = kv8_page(c, b, blk);
+  if (page < 0) return;
+  const int old = static_cast<int>(first < start ? start - first : 0);  // tokens already there
+  const int upto = static_cast<int>(end - first < c.T ? end - first : c.T);
+  const int dv = c.D >> 3;  // vectors per token
+  const T* src = static_cast<const T*>(is_v ? a.v : a.k) + b * (is_v ? a.vb : a.kb) + h * (is_v ? a.vh : a.kh);
+  const int64_t st = is_v ? a.vt : a.kt;
+  int8_t* codes = (is_v ? c.v : c.k) + (static_cast<int64_t>(page) * c.heads + h) * (static_cast<int64_t>(c.T) * c.D);
+  float* scale = (is_v ? c.vs : c.ks) + static_cast<int64_t>(page) * c.heads + h;
+
+  uint4 raw[NV];
+  uint32_t top = 0;  // largest |x| as bits: NaN and infinities sort above
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = (old * dv) + tid + k * kKvThreads;
+    if (i < upto * dv) {
+      const int tok = i / dv;
+      raw[k] = __ldg(reinterpret_cast<const uint4*>(src + (first + tok - start) * st + (i - tok * dv) * 8));
+      const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((tid & 31) == 0) wmax[tid >> 5] = top;
+  const float before = old > 0 ? *scale : 0.0f;
+  __syncthreads();  // also: every thread has read the old scale
+#pragma unroll
+  for (int i = 0; i < kKvThreads / 32; ++i) top = max(top, wmax[i]);
+  const uint16_t tb = static_cast<uint16_t>(top);
+  const float amax = to_float<T>(*reinterpret_cast<const T*>(&tb));
+  const float grown = __fdiv_rn(amax, 127.0f);
+  // a NaN on either side must win, so that the block reads back as NaN
+  const float s = before > grown || before != before ? before : grown;
+  if (tid == 0) *scale = s;
+  const float div = s > 0.0f || s != s ? s : 1.0f;
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int i = (old * dv) + tid + k * kKvThreads;
+    if (i < upto * dv) {
+      const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
+      __align__(8) int8_t o[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint16_t e = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
+        const float f = rintf(__fdiv_rn(to_float<T>(*reinterpret_cast<const T*>(&e)), div));
+        o[j] = static_cast<int8_t>(fminf(fmaxf(f, -127.0f), 127.0f));
+      }
+      *reinterpret_cast<uint2*>(codes + i * 8) = *reinterpret_cast<const uint2*>(o);
+    }
+  }
+  if (old > 0 && s != before) {
+    const float ratio = __fdiv_rn(before, div);
+    for (int i = tid; i < old * dv; i += kKvThreads) {
+      __align__(8) int8_t o[8];
+      *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(codes + i * 8);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float f = rintf(__fmul_rn(static_cast<float>(o[j]), ratio));
+        o[j] = static_cast<int8_t>(fminf(fmaxf(f, -127.0f), 127.0f));
+      }
+      *reinterpret_cast<uint2*>(codes + i * 8) = *reinterpret_cast<const uint2*>(o);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- gather
+struct Kv8GatherArgs {
+  Kv8Cache c;
+  void *k, *v;            // [B, heads, S, D] contiguous
+  int out_dtype;          // kOutBF16 / kOutF16 / kOutF32
+  const int32_t* first;   // [B]
+  const int32_t* counts;  // [B] tokens to read (<= S); the rest of S is zeroed
+  int B, S;
+};
+
+// One thread per 8 codes; grid (vectors of a head, heads, 2 B).
+__global__ void __launch_bounds__(kKvThreads) kv8_gather_kernel(const Kv8GatherArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const Kv8Cache& c = a.c;
+  const bool is_v = blockIdx.z & 1;
+  const int b = blockIdx.z >> 1, h = blockIdx.y, dv = c.D >> 3;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x;
+  if (i >= static_cast<int64_t>(a.S) * dv) return;
+  const int tok = static_cast<int>(i / dv), d = static_cast<int>(i - static_cast<int64_t>(tok) * dv) * 8;
+  const int first = a.first[b];
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = 0.0f;
+  if (first >= 0 && tok < a.counts[b]) {
+    const int64_t pos = static_cast<int64_t>(first) + tok;
+    const int page = kv8_page(c, b, static_cast<int>(pos >> c.log_t));
+    if (page >= 0) {
+      const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+      const float s = __ldg((is_v ? c.vs : c.ks) + at);
+      const int8_t* p = (is_v ? c.v : c.k) + (at * c.T + (pos & (c.T - 1))) * c.D + d;
+      __align__(8) int8_t o[8];
+      *reinterpret_cast<uint2*>(o) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __fmul_rn(static_cast<float>(o[j]), s);
+    }
+  }
+  const int64_t dst = ((static_cast<int64_t>(b) * c.heads + h) * a.S + tok) * c.D + d;
+  void* out = is_v ? a.v : a.k;
+  if (a.out_dtype == kOutF32) {
+    float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + dst);
+    p[0] = make_float4(f[0], f[1], f[2], f[3]);
+    p[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      o[j] = a.out_dtype == kOutBF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ---------------------------------------------------------------- attention
+// Rows: the G query heads of a key/value head and their Tq tokens are packed as
+// rows r = token * G + head of one matrix, 16 rows per MMA (m16n8k16, fp16
+// operands, fp32 accumulation).  int8 codes are exact in fp16: with the sign bit
+// flipped a byte OR-ed into the mantissa of 1024 is 1152 + code, and subtracting
+// 1152 is exact.  q is scaled by the power of two of its row's largest |q| and
+// is then exact in fp16 (bf16: down to 2^-17 of the row's maximum, within 2^-25
+// of it below).
+//
+// Softmax, online, base 2.  With sigma = q.k_code * ks * scale * log2 e and vs the
+// block's V scale, the weights kept are P = 2^(sigma + log2 vs - m) <= 1, m the
+// running maximum of that exponent; then
+//   out = sum P * v_code / sum P / vs,
+// so V's scales cost one add per score instead of a pass over the accumulators,
+// and P fits fp16 whatever the scales are: P's fp16 rounding (2^-11 relative,
+// 2^-25 of the row's largest weight at least) is the only one before the
+// output's.  A block with vs = 0 adds its P to the sum only.
+//
+// Layout, D = 128: lane (g, t) loads 32 consecutive bytes (quarter t) of K token
+// g, and 16 bytes (eighth g) of V tokens 2t, 2t+1, 2t+8, 2t+9: every load of the
+// warp covers whole 128-byte rows.  The order of d inside the K product is free
+// (q is permuted alike), and V's columns come out as d = 16 g + i for tile i, so
+// a lane ends with 32 consecutive d of its rows.
+struct Kv8AttnArgs {
+  Kv8Cache c;
+  const void* q;  // [B, Hq, Tq, D] strides qb, qh, qt
+  int q_f16;
+  int64_t qb, qh, qt;
+  void* out;  // [B, Hq, Tq, D] strides ob, oh, ot
+  int64_t ob, oh, ot;
+  float* lse;     // [B, Hq, Tq] contiguous
+  float* part_o;  // [splits][B*Hq*Tq][D] fp32 (splits > 1)
+  float* part_ml; // [splits][B*Hq*Tq][2]: m (base 2), l
+  const int32_t* lens;
+  int B, Hq, G, Tq, causal, splits;
+  float scale_log2;  // softmax scale * log2 e
+};
+
+constexpr int kAttnWarps = 4;
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t hsub2_1152(uint32_t a) {
+  const uint32_t k = 0x64806480u;  // 1152, 1152
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&k));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Bytes 0,1 (lo) / 2,3 (hi) of a sign-flipped word as two exact fp16 values.
+__device__ __forceinline__ uint32_t i8_lo(uint32_t w) { return hsub2_1152(__byte_perm(w, 0x64646464u, 0x4140)); }
+__device__ __forceinline__ uint32_t i8_hi(uint32_t w) { return hsub2_1152(__byte_perm(w, 0x64646464u, 0x4342)); }
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Value of q as fp16 bits after scaling, from bf16 / fp16 bits.
+__device__ __forceinline__ uint32_t q_pair(uint32_t raw, int f16, float inv) {
+  float a, b;
+  if (f16) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&raw));
+    a = f.x;
+    b = f.y;
+  } else {
+    a = __uint_as_float(raw << 16);
+    b = __uint_as_float(raw & 0xFFFF0000u);
+  }
+  return pack_f16x2(a * inv, b * inv);
+}
+
+// log-sum-exp pieces of two halves of a row: (m, l) and the factors of each side.
+__device__ __forceinline__ float safe_ex2_diff(float m, float top) {
+  return m == -INFINITY ? 0.0f : ex2f(m - top);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8AttnArgs a) {
+  constexpr int KS = D / 16;   // k16 steps of the K product
+  constexpr int KW = D / 16;   // 32-bit words per lane and K token (D / 4 bytes)
+  constexpr int VW = D / 32;   // words per lane and V token (D / 8 bytes)
+  constexpr int NV = D / 8;    // n8 tiles of the output
+  __shared__ float sm_ml[kAttnWarps][16][2];
+  __shared__ float sm_o[16][D + 4];
+  griddep_wait();
+  griddep_launch_dependents();
+  const Kv8Cache& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int rows = a.G * a.Tq;
+  const int row_tiles = (rows + 15) >> 4;
+  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * 16;
+  const int cap = c.max_blocks << c.log_t;
+  const int len = min(max(a.lens[b], 0), cap);
+
+  // rows g and g + 8 of this lane: how many positions each sees
+  int lim[2];
+  int64_t q_at[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = min(r0 + g + 8 * i, rows - 1);
+    const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
+    lim[i] = a.causal ? min(max(len - a.Tq + ti + 1, 0), len) : len;
+    q_at[i] = b * a.qb + hi * a.qh + ti * a.qt;
+  }
+  // the tile's last row sees the most, its first the least
+  const int last = min(r0 + 15, rows - 1);
+  const int lim_max = a.causal ? min(max(len - a.Tq + last / a.G + 1, 0), len) : len;
+  const int lim_min = a.causal ? min(max(len - a.Tq + r0 / a.G + 1, 0), len) : len;
+  const int tiles = (lim_max + 15) >> 4;  // 16-token tiles to visit
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+
+  // ---- q fragments, scaled to fp16
+  uint32_t qf[KS][4];
+  float sc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + q_at[i] + t * (D / 4);
+    uint32_t raw[KS * 2];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      raw[4 * j] = v.x; raw[4 * j + 1] = v.y; raw[4 * j + 2] = v.z; raw[4 * j + 3] = v.w;
+    }
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < KS * 2; ++j) top = max(top, max(raw[j] & 0x7FFFu, (raw[j] >> 16) & 0x7FFFu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float inv = 1.0f, up = 1.0f;
+    if (!a.q_f16) {
+      int ex = static_cast<int>(top >> 7);
+      ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+      inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+      up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+    }
+    sc[i] = a.scale_log2 * up;
+#pragma unroll
+    for (int j = 0; j < KS; ++j) {
+      qf[j][i] = q_pair(raw[2 * j], a.q_f16, inv);
+      qf[j][i + 2] = q_pair(raw[2 * j + 1], a.q_f16, inv);
+    }
+  }
+
+  float o[NV][4];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+  const int64_t head_bytes = static_cast<int64_t>(c.T) * D;
+  for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
+    const int pos = tile << 4;
+    const int page = kv8_page(c, b, pos >> c.log_t);
+    if (page < 0) continue;
+    const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+    const int8_t* kp = c.k + at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
+    const int8_t* vp = c.v + at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
+    const float ks = __ldg(c.ks + at), vs = __ldg(c.vs + at);
+
+    uint32_t kw[2][KW], vw[4][VW];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4* p = reinterpret_cast<const uint4*>(kp + (8 * i + g) * D + t * (D / 4));
+#pragma unroll
+      for (int j = 0; j < KW / 4; ++j) {
+        const uint4 v = __ldg(p + j);
+        kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int8_t* p = vp + (2 * t + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8);
+      if constexpr (VW == 4) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
+      } else {
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        vw[i][0] = v.x; vw[i][1] = v.y;
+      }
+    }
+
+    // ---- scores of 16 tokens
+    float s[2][4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KS; ++j) {
+        const uint32_t w = kw[i][j] ^ 0x80808080u;
+        mma_f16(s[i], qf[j], i8_lo(w), i8_hi(w));
+      }
+    }
+    const bool zero_v = vs == 0.0f;
+    const float lv = zero_v ? 0.0f : log2f(vs);
+    const float iv = zero_v ? 1.0f : 1.0f / vs;
+    const bool mask = pos + 16 > lim_min;
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = j >> 1;
+        s[i][j] = fmaf(s[i][j], ks * sc[r], lv);
+        if (mask && pos + 8 * i + 2 * t + (j & 1) >= lim[r]) s[i][j] = -INFINITY;
+        top[r] = fmaxf(top[r], s[i][j]);
+      }
+    float corr[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+      const float mn = fmaxf(m[r], top[r]);
+      corr[r] = safe_ex2_diff(m[r], mn);
+      m[r] = mn;
+      l[r] *= corr[r];
+    }
+    uint32_t pf[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = j >> 1;
+        // a masked score is exactly -inf; a NaN one (NaN q or scales) stays NaN
+        p[j] = s[i][j] == -INFINITY ? 0.0f : ex2f(s[i][j] - m[r]);
+        l[r] = fmaf(p[j], iv, l[r]);
+      }
+      pf[2 * i] = zero_v ? 0u : pack_f16x2(p[0], p[1]);
+      pf[2 * i + 1] = zero_v ? 0u : pack_f16x2(p[2], p[3]);
+    }
+    if (__any_sync(0xffffffffu, corr[0] != 1.0f || corr[1] != 1.0f)) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        o[i][0] *= corr[0]; o[i][1] *= corr[0];
+        o[i][2] *= corr[1]; o[i][3] *= corr[1];
+      }
+    }
+    // ---- P V: tiles 4w .. 4w+3 come from word w of the four tokens
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint32_t ta = vw[0][w] ^ 0x80808080u, tb = vw[1][w] ^ 0x80808080u;
+      const uint32_t tc = vw[2][w] ^ 0x80808080u, td = vw[3][w] ^ 0x80808080u;
+      const uint32_t ab0 = __byte_perm(ta, tb, 0x5140), ab1 = __byte_perm(ta, tb, 0x7362);
+      const uint32_t cd0 = __byte_perm(tc, td, 0x5140), cd1 = __byte_perm(tc, td, 0x7362);
+      mma_f16(o[4 * w], pf, i8_lo(ab0), i8_lo(cd0));
+      mma_f16(o[4 * w + 1], pf, i8_hi(ab0), i8_hi(cd0));
+      mma_f16(o[4 * w + 2], pf, i8_lo(ab1), i8_lo(cd1));
+      mma_f16(o[4 * w + 3], pf, i8_hi(ab1), i8_hi(cd1));
+    }
+  }
+
+  // ---- join the warps (in order), then store or hand over the partial
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+    if (t == 0) {
+      sm_ml[warp][g + 8 * r][0] = m[r];
+      sm_ml[warp][g + 8 * r][1] = l[r];
+    }
+  }
+  __syncthreads();
+  float mt[2], lt[2], f[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    mt[r] = -INFINITY;
+    for (int w = 0; w < kAttnWarps; ++w) {
+      const float x = sm_ml[w][g + 8 * r][0];
+      mt[r] = fmaxf(mt[r], x);
+    }
+    lt[r] = 0.0f;
+    for (int w = 0; w < kAttnWarps; ++w)
+      lt[r] += sm_ml[w][g + 8 * r][1] * safe_ex2_diff(sm_ml[w][g + 8 * r][0], mt[r]);
+    f[r] = safe_ex2_diff(m[r], mt[r]);
+  }
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (warp == w) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // tile i, column g' holds d = (D / 8) g' + i; this lane's columns are 2t, 2t + 1
+          float* p = &sm_o[g + 8 * (j >> 1)][(2 * t + (j & 1)) * (D / 8) + i];
+          const float x = o[i][j] * f[j >> 1];
+          *p = w == 0 ? x : *p + x;
+        }
+    }
+    __syncthreads();
+  }
+  __shared__ float sm_fin[16][2];
+  if (warp == 0 && t == 0)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sm_fin[g + 8 * r][0] = mt[r];
+      sm_fin[g + 8 * r][1] = lt[r];
+    }
+  __syncthreads();
+  for (int e = tid; e < 16 * (D / 4); e += kAttnWarps * 32) {
+    const int row = e / (D / 4), d = (e - row * (D / 4)) * 4, r = r0 + row;
+    if (r >= rows) continue;
+    const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
+    const float4 x = *reinterpret_cast<const float4*>(&sm_o[row][d]);
+    const float mm = sm_fin[row][0], ll = sm_fin[row][1];
+    const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
+    if (a.splits > 1) {
+      const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
+      *reinterpret_cast<float4*>(a.part_o + at * D + d) = x;
+      if (d == 0) {
+        a.part_ml[at * 2] = mm;
+        a.part_ml[at * 2 + 1] = ll;
+      }
+      continue;
+    }
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + d;
+    *reinterpret_cast<uint2*>(dst) =
+        a.q_f16 ? make_uint2(pack_f16x2(x.x * inv, x.y * inv), pack_f16x2(x.z * inv, x.w * inv))
+                : make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+    if (d == 0) a.lse[flat] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+  }
+}
+
+// Joins the splits of each row in split order: one warp per row.
+template <int D>
+__global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnArgs a) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t flat = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Tq;
+  if (flat >= rows) return;
+  const int lane = threadIdx.x & 31;
+  constexpr int PL = D / 32;  // values per lane
+  float mt = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) {
+    const float x = a.part_ml[(s * rows + flat) * 2];
+    mt = fmaxf(mt, x);
+  }
+  float lt = 0.0f, acc[PL];
+#pragma unroll
+  for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = safe_ex2_diff(a.part_ml[(s * rows + flat) * 2], mt);
+    lt += a.part_ml[(s * rows + flat) * 2 + 1] * f;
+    const float* p = a.part_o + (s * rows + flat) * D + lane * PL;
+#pragma unroll
+    for (int i = 0; i < PL; ++i) acc[i] = fmaf(p[i], f, acc[i]);
+  }
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  const int ti = static_cast<int>(flat % a.Tq);
+  const int64_t bh = flat / a.Tq;
+  const int64_t b = bh / a.Hq, hi = bh - b * a.Hq;
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + lane * PL;
+#pragma unroll
+  for (int i = 0; i < PL; i += 2)
+    *reinterpret_cast<uint32_t*>(dst + i) = a.q_f16 ? pack_f16x2(acc[i] * inv, acc[i + 1] * inv)
+                                                    : pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+  if (lane == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
+}
+
+}  // namespace b200q

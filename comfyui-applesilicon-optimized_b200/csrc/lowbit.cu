@@ -1,0 +1,422 @@
+// C ABI launch layer of the low-bit decode operators (declarations:
+// include/b200q.h): 4-bit weight linears, the norms before and after a block,
+// and the paged 8-bit key/value cache.  As in capi.cu: arguments are checked on
+// the host before any launch, nothing is allocated, nothing synchronises, and
+// kernels go to the caller's stream as programmatic dependents.
+#include "../../include/b200q.h"
+#include "block_norm.cuh"
+#include "host.h"
+#include "kv8.cuh"
+#include "w4a16.cuh"
+
+using namespace b200q;
+
+namespace b200q {
+namespace host {
+int lowbit_device_status(unsigned int* status, bool reset) {
+  if (cudaMemcpyFromSymbol(status, g_device_status, sizeof(unsigned int)) != cudaSuccess)
+    return B200Q_ERR_CUDA;
+  const unsigned int zero = 0;
+  if (reset && cudaMemcpyToSymbol(g_device_status, &zero, sizeof(unsigned int)) != cudaSuccess)
+    return B200Q_ERR_CUDA;
+  return B200Q_OK;
+}
+}  // namespace host
+}  // namespace b200q
+
+namespace {
+
+constexpr int64_t kIntMax = (int64_t(1) << 31) - 1;
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// A launch with optional dynamic shared memory and cluster size, as a
+// programmatic dependent of the kernel before it (B200Q_PDL=0: plainly).
+template <typename... KArgs, typename... Args>
+int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, cudaStream_t st,
+           Args... args) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return B200Q_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(block));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (host::pdl_on()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = static_cast<unsigned>(cluster);
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = 1;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  cudaLaunchKernelEx(&cfg, kern, args...);  // errors surface in finish_launch
+  return host::finish_launch();
+}
+
+// ------------------------------------------------------------ 4-bit linear
+// Largest M of the warp-MMA kernel; above it the weight is decoded once per call
+// for the tile GEMM.
+constexpr int64_t kW4MaxSmallM = 32;
+
+struct W4Plan {
+  int wr, splits, smem;
+};
+
+// Rows per CTA (16 * wr) and cluster size.  With few tokens a CTA takes one
+// 16-row tile and its 8 warps split K; more tokens make staging x per CTA cost
+// more than it gives, so a CTA takes 64 rows and a cluster splits K.
+W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int G, int cols) {
+  W4Plan p{};
+  const int64_t KG = K / G;
+  p.wr = M <= 4 ? 1 : 4;
+  p.splits = 1;
+  const int64_t want = M <= 4 ? 296 : 592;  // CTAs of 8 warps
+  while (p.splits < 8 && cdiv(N, 16 * p.wr) * p.splits < want && 2 * p.splits * (kW4Warps / p.wr) <= KG)
+    p.splits *= 2;
+  auto bytes = [&](int s) { return w4_smem_bytes(int(M), int(cdiv(KG, s)) * G, cols, p.wr); };
+  while (p.splits < 8 && bytes(p.splits) > 100 * 1024) p.splits *= 2;
+  p.smem = bytes(p.splits);
+  return p;
+}
+
+template <typename T, int LW>
+int launch_w4_cols(const W4Args& a, const EpiArgs& ep, const W4Plan& p, int nt, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(cdiv(a.N, 16 * p.wr) * p.splits));
+  switch (nt) {
+    case 1: return launch(w4a16_kernel<T, LW, 1>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
+    case 2: return launch(w4a16_kernel<T, LW, 2>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
+    default: return launch(w4a16_kernel<T, LW, 4>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
+  }
+}
+template <typename T>
+int launch_w4(const W4Args& a, const EpiArgs& ep, const W4Plan& p, int nt, cudaStream_t st) {
+  switch (a.G) {
+    case 32: return launch_w4_cols<T, 1>(a, ep, p, nt, st);
+    case 64: return launch_w4_cols<T, 2>(a, ep, p, nt, st);
+    default: return launch_w4_cols<T, 4>(a, ep, p, nt, st);
+  }
+}
+
+struct W4Work {
+  size_t w, x, row, col, total;  // byte offsets
+};
+W4Work w4_work(int64_t M, int64_t N, int64_t K) {
+  auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
+  W4Work o{};
+  o.x = up(size_t(N) * K * 2);
+  o.row = o.x + up(size_t(M) * K * 2);
+  o.col = o.row + up(size_t(M) * 4);
+  o.total = o.col + up(size_t(N) * 4);
+  return o;
+}
+
+int norm_threads(int64_t D, int vec, int npt) {
+  const int64_t t = cdiv(cdiv(D, vec), npt);
+  return static_cast<int>(cdiv(t, 32) * 32);
+}
+template <int DTYPE>
+int launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(a.rows));
+  if (vec) {
+    if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 8, 1>, grid, norm_threads(a.D, 8, 1), 0, 1, st, a);
+    if (a.D <= 8 * 1024) return launch(block_norm_kernel<DTYPE, 8, 2>, grid, norm_threads(a.D, 8, 2), 0, 1, st, a);
+    return launch(block_norm_kernel<DTYPE, 8, 4>, grid, norm_threads(a.D, 8, 4), 0, 1, st, a);
+  }
+  if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 1, 8>, grid, norm_threads(a.D, 1, 8), 0, 1, st, a);
+  return launch(block_norm_kernel<DTYPE, 1, 32>, grid, norm_threads(a.D, 1, 32), 0, 1, st, a);
+}
+
+// ------------------------------------------------------------ 8-bit cache
+// Checks a cache and fills its kernel view.
+bool make_cache(Kv8Cache* c, int8_t* k, int8_t* v, float* ks, float* vs, int64_t pages,
+                int64_t heads, int64_t block, int64_t D, const int32_t* table, int64_t ld_table,
+                int64_t max_blocks) {
+  if (!k || !v || !ks || !vs || !table || pages < 1 || pages > kIntMax || heads < 1 ||
+      heads > 65535 || (D != 64 && D != 128) || max_blocks < 1 || ld_table < max_blocks ||
+      (block != 16 && block != 32 && block != 64 && block != 128) || max_blocks * block > kIntMax ||
+      !aligned(k, 16) || !aligned(v, 16))
+    return false;
+  c->k = k;
+  c->v = v;
+  c->ks = ks;
+  c->vs = vs;
+  c->table = table;
+  c->ld_table = ld_table;
+  c->max_blocks = static_cast<int>(max_blocks);
+  c->pages = static_cast<int>(pages);
+  c->heads = static_cast<int>(heads);
+  c->T = static_cast<int>(block);
+  c->D = static_cast<int>(D);
+  c->log_t = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : 7;
+  return true;
+}
+
+template <typename T>
+int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
+  // a sequence may start inside a block: one more block than S fills
+  const dim3 grid(static_cast<unsigned>(cdiv(a.S + a.c.T - 1, a.c.T)), static_cast<unsigned>(a.c.heads),
+                  static_cast<unsigned>(2 * a.B));
+  const int vecs = a.c.T * a.c.D / 8;
+  if (vecs <= kKvThreads) return launch(kv8_append_kernel<T, 1>, grid, kKvThreads, 0, 1, st, a);
+  if (vecs <= 2 * kKvThreads) return launch(kv8_append_kernel<T, 2>, grid, kKvThreads, 0, 1, st, a);
+  if (vecs <= 4 * kKvThreads) return launch(kv8_append_kernel<T, 4>, grid, kKvThreads, 0, 1, st, a);
+  return launch(kv8_append_kernel<T, 8>, grid, kKvThreads, 0, 1, st, a);
+}
+
+// How many CTAs share a sequence's length: enough to fill the GPU, at least 128
+// tokens each.
+int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
+  const int64_t base = B * heads * cdiv(Hq / heads * Tq, 16);
+  int64_t s = cdiv(int64_t(sms) * 6, base);
+  const int64_t most = cdiv(max_len, 128);
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+size_t attn_work_bytes(int splits, int64_t rows, int64_t D) {
+  return splits > 1 ? size_t(splits) * rows * (D + 2) * 4 : 0;
+}
+bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
+  return B >= 0 && B <= 65535 && heads >= 1 && Hq >= heads && Hq % heads == 0 && Tq >= 0 &&
+         Hq / heads * Tq <= kIntMax && heads * cdiv(Hq / heads * Tq, 16) <= 65535;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K) {
+  if (M <= kW4MaxSmallM || N <= 0 || K <= 0) return 0;
+  return w4_work(M, N, K).total;
+}
+
+int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw,
+                       const void* scales, int scale_dtype, const uint8_t* zeros, int64_t group,
+                       const void* bias, int bias_dtype, int act, void* out, int out_dtype,
+                       int64_t ldo, int64_t M, int64_t N, int64_t K, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  if (M < 0 || N < 0 || K <= 0 || M > kIntMax || N > kIntMax || K > kIntMax ||
+      (group != 32 && group != 64 && group != 128) || K % group != 0 ||
+      (x_dtype != B200Q_BF16 && x_dtype != B200Q_F16) || scale_dtype < B200Q_BIAS_BF16 ||
+      scale_dtype > B200Q_BIAS_F32 || bias_dtype < B200Q_BIAS_NONE || bias_dtype > B200Q_BIAS_F32 ||
+      act < B200Q_ACT_NONE || act > B200Q_ACT_GELU_ERF || out_dtype < B200Q_BF16 ||
+      out_dtype > B200Q_F32 || ldx < K || ldw < K / 2 || ldo < N || ldw % 16 != 0)
+    return B200Q_ERR_INVALID;
+  if (M == 0 || N == 0) return B200Q_OK;
+  if (!x || !w || !scales || !out || !aligned(w, 16) || (bias_dtype != B200Q_BIAS_NONE && !bias))
+    return B200Q_ERR_INVALID;
+  const int sms = host::device_sms();
+  if (!sms) return B200Q_ERR_UNSUPPORTED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  EpiArgs ep{};
+  ep.out = out;
+  ep.ldo = ldo;
+  ep.out_dtype = out_dtype;
+  ep.bias = bias;
+  ep.bias_dtype = bias_dtype;
+  ep.act = act;
+  ep.M = static_cast<int>(M);
+  ep.N = static_cast<int>(N);
+  const bool x_vec = aligned(x, 16) && ldx % 8 == 0;
+  if (M <= kW4MaxSmallM) {
+    W4Args a{};
+    a.x = x;
+    a.ldx = ldx;
+    a.w = w;
+    a.ldw = ldw;
+    a.scales = scales;
+    a.scale_dtype = scale_dtype;
+    a.zeros = zeros;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.K = static_cast<int>(K);
+    a.G = static_cast<int>(group);
+    a.x_vec = x_vec;
+    const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
+    const W4Plan p = w4_plan(M, N, K, a.G, 8 * nt);
+    if (p.smem > 227 * 1024) return B200Q_ERR_UNSUPPORTED;  // K beyond about 50,000 at 32 tokens
+    a.wr = p.wr;
+    a.splits = p.splits;
+    return x_dtype == B200Q_F16 ? launch_w4<__half>(a, ep, p, nt, st)
+                                : launch_w4<__nv_bfloat16>(a, ep, p, nt, st);
+  }
+  const W4Work o = w4_work(M, N, K);
+  if (!workspace || workspace_bytes < o.total || !aligned(workspace, 256)) return B200Q_ERR_WORKSPACE;
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  __half* w16 = reinterpret_cast<__half*>(base);
+  float* col = reinterpret_cast<float*>(base + o.col);
+  int s = launch(w4_decode_rows_kernel, dim3(static_cast<unsigned>(N)), 256, 0, 1, st, w, ldw, scales,
+                 scale_dtype, zeros, int(N), int(K), int(group), w16, col);
+  if (s != B200Q_OK) return s;
+  ep.col_scale = col;
+  ep.col_scale_vec = 1;
+  if (x_dtype == B200Q_BF16 || !x_vec) {
+    if (x_dtype != B200Q_BF16) return B200Q_ERR_INVALID;  // fp16 rows must be 16-byte aligned here
+    __half* x16 = reinterpret_cast<__half*>(base + o.x);
+    float* row = reinterpret_cast<float*>(base + o.row);
+    s = launch(w4_x_f16_kernel, dim3(static_cast<unsigned>(M)), 256, 0, 1, st,
+               static_cast<const __nv_bfloat16*>(x), ldx, int(K), int(x_vec), x16, row);
+    if (s != B200Q_OK) return s;
+    ep.row_scale = row;
+    ep.row_scale_vec = 1;
+    x = x16;
+    ldx = K;
+  }
+  return host::gemm16_scaled(true, x, ldx, w16, K, M, N, K, ep, st);
+}
+
+int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype,
+                     int post_kind, const void* post_w, int post_w_dtype, const void* gate,
+                     int64_t ld_gate, float res_scale, int pre_kind, const void* w, int w_dtype,
+                     const void* scale, int64_t ld_scale, const void* shift, int64_t ld_shift,
+                     int mod_dtype, int64_t rows_per_mod, float eps, void* h, int64_t ldh,
+                     void* out, int64_t ldo, int8_t* q, int64_t ldq, float* q_scale, int64_t rows,
+                     int64_t D, void* stream) {
+  if (rows < 0 || rows > kIntMax || D < 1 || D > B200Q_NORM_MAX_D || rows_per_mod < 1 ||
+      (dtype != B200Q_BF16 && dtype != B200Q_F16) || post_kind < B200Q_NORM_NONE ||
+      post_kind > B200Q_NORM_LAYER || pre_kind < B200Q_NORM_NONE || pre_kind > B200Q_NORM_LAYER ||
+      ldx < D || (y && ldy < D) || (h && ldh < D) || (out && ldo < D) || (q && ldq < D) ||
+      (q && !q_scale) || (out && q) || (!y && (h || gate || post_w)))
+    return B200Q_ERR_INVALID;
+  auto bad_dtype = [](const void* p, int t) { return p && (t < B200Q_BIAS_BF16 || t > B200Q_BIAS_F32); };
+  if (bad_dtype(post_w, post_w_dtype) || bad_dtype(w, w_dtype) || bad_dtype(gate, mod_dtype) ||
+      bad_dtype(scale, mod_dtype) || bad_dtype(shift, mod_dtype) || (gate && ld_gate < D) ||
+      (scale && ld_scale < D) || (shift && ld_shift < D))
+    return B200Q_ERR_INVALID;
+  if (rows == 0) return B200Q_OK;
+  if (!x || (!out && !q && !h)) return B200Q_ERR_INVALID;
+  if (!host::device_sms()) return B200Q_ERR_UNSUPPORTED;
+  NormArgs a{};
+  a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy;
+  a.post_w = post_w; a.post_w_dtype = post_w_dtype;
+  a.w = w; a.w_dtype = w_dtype;
+  a.gate = gate; a.scale = scale; a.shift = shift;
+  a.ld_gate = ld_gate; a.ld_scale = ld_scale; a.ld_shift = ld_shift;
+  a.mod_dtype = mod_dtype;
+  a.res_scale = res_scale; a.eps = eps;
+  a.post_kind = post_kind; a.pre_kind = pre_kind;
+  a.h = h; a.ldh = ldh; a.out = out; a.ldo = ldo; a.q = q; a.ldq = ldq; a.q_scale = q_scale;
+  a.rows = static_cast<int>(rows); a.D = static_cast<int>(D);
+  a.rows_per_mod = static_cast<int>(rows_per_mod < kIntMax ? rows_per_mod : kIntMax);
+  // 16-byte vectors need every row of every operand on a 16-byte boundary
+  auto ok = [](const void* p, int64_t ld) { return !p || (aligned(p, 16) && ld % 8 == 0); };
+  const bool vec = D % 8 == 0 && ok(x, ldx) && ok(y, ldy) && ok(h, ldh) && ok(out, ldo) &&
+                   ok(gate, ld_gate) && ok(scale, ld_scale) && ok(shift, ld_shift) &&
+                   ok(post_w, 0) && ok(w, 0) && (!q || (aligned(q, 8) && ldq % 8 == 0));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == B200Q_F16 ? launch_norm<kBiasF16>(a, vec, st) : launch_norm<kBiasBF16>(a, vec, st);
+}
+
+int b200q_kv8_append(const void* k, const void* v, int dtype, int64_t B, int64_t S,
+                     const int64_t* k_strides, const int64_t* v_strides, int8_t* k_codes,
+                     int8_t* v_codes, float* k_scale, float* v_scale, int64_t pages, int64_t heads,
+                     int64_t block, int64_t D, const int32_t* table, int64_t ld_table,
+                     int64_t max_blocks, const int32_t* start, const int32_t* counts,
+                     void* stream) {
+  Kv8AppendArgs a{};
+  if (B < 0 || B > 32767 || S < 0 || S > kIntMax / 2 || (dtype != B200Q_BF16 && dtype != B200Q_F16) ||
+      !k_strides || !v_strides ||
+      !make_cache(&a.c, k_codes, v_codes, k_scale, v_scale, pages, heads, block, D, table, ld_table,
+                  max_blocks))
+    return B200Q_ERR_INVALID;
+  if (B == 0 || S == 0) return B200Q_OK;
+  if (!k || !v || !start || !aligned(k, 16) || !aligned(v, 16)) return B200Q_ERR_INVALID;
+  for (int i = 0; i < 3; ++i)
+    if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0) return B200Q_ERR_INVALID;
+  if (!host::device_sms()) return B200Q_ERR_UNSUPPORTED;
+  a.k = k; a.v = v;
+  a.kb = k_strides[0]; a.kh = k_strides[1]; a.kt = k_strides[2];
+  a.vb = v_strides[0]; a.vh = v_strides[1]; a.vt = v_strides[2];
+  a.start = start; a.counts = counts;
+  a.B = static_cast<int>(B); a.S = static_cast<int>(S);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == B200Q_F16 ? launch_append<__half>(a, st) : launch_append<__nv_bfloat16>(a, st);
+}
+
+int b200q_kv8_gather(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                     const float* v_scale, int64_t pages, int64_t heads, int64_t block, int64_t D,
+                     const int32_t* table, int64_t ld_table, int64_t max_blocks,
+                     const int32_t* first, const int32_t* counts, void* k, void* v, int out_dtype,
+                     int64_t B, int64_t S, void* stream) {
+  Kv8GatherArgs a{};
+  if (B < 0 || B > 32767 || S < 0 || S > kIntMax / 2 || out_dtype < B200Q_BF16 || out_dtype > B200Q_F32 ||
+      !make_cache(&a.c, const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes),
+                  const_cast<float*>(k_scale), const_cast<float*>(v_scale), pages, heads, block, D,
+                  table, ld_table, max_blocks))
+    return B200Q_ERR_INVALID;
+  if (B == 0 || S == 0) return B200Q_OK;
+  if (!k || !v || !first || !counts || !aligned(k, 16) || !aligned(v, 16)) return B200Q_ERR_INVALID;
+  if (!host::device_sms()) return B200Q_ERR_UNSUPPORTED;
+  a.k = k; a.v = v; a.out_dtype = out_dtype;
+  a.first = first; a.counts = counts;
+  a.B = static_cast<int>(B); a.S = static_cast<int>(S);
+  const dim3 grid(static_cast<unsigned>(cdiv(S * (D / 8), kKvThreads)), static_cast<unsigned>(heads),
+                  static_cast<unsigned>(2 * B));
+  return launch(kv8_gather_kernel, grid, kKvThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
+}
+
+size_t b200q_kv8_attention_workspace_size(int64_t B, int64_t Hq, int64_t heads, int64_t Tq,
+                                          int64_t D, int64_t max_len) {
+  const int sms = host::device_sms();
+  if (!sms || !attn_dims(B, Hq, heads, Tq) || B * Tq == 0) return 0;
+  return attn_work_bytes(attn_splits(sms, B, Hq, heads, Tq, max_len), B * Hq * Tq, D);
+}
+
+int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Tq,
+                        const int64_t* q_strides, const int8_t* k_codes, const int8_t* v_codes,
+                        const float* k_scale, const float* v_scale, int64_t pages, int64_t heads,
+                        int64_t block, int64_t D, const int32_t* table, int64_t ld_table,
+                        int64_t max_blocks, const int32_t* lens, int64_t max_len, int causal,
+                        float softmax_scale, void* out, const int64_t* out_strides, float* lse,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  Kv8AttnArgs a{};
+  if ((dtype != B200Q_BF16 && dtype != B200Q_F16) || !attn_dims(B, Hq, heads, Tq) || !q_strides ||
+      !out_strides || max_len < 0 ||
+      !make_cache(&a.c, const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes),
+                  const_cast<float*>(k_scale), const_cast<float*>(v_scale), pages, heads, block, D,
+                  table, ld_table, max_blocks))
+    return B200Q_ERR_INVALID;
+  if (B == 0 || Tq == 0) return B200Q_OK;
+  if (!q || !lens || !out || !lse || !aligned(q, 16) || !aligned(out, 16)) return B200Q_ERR_INVALID;
+  for (int i = 0; i < 3; ++i)
+    if (q_strides[i] % 8 != 0 || out_strides[i] % 8 != 0) return B200Q_ERR_INVALID;
+  const int sms = host::device_sms();
+  if (!sms) return B200Q_ERR_UNSUPPORTED;
+  const int64_t rows = B * Hq * Tq;
+  const int splits = attn_splits(sms, B, Hq, heads, Tq, max_len);
+  if (splits > 1 && (!workspace || workspace_bytes < attn_work_bytes(splits, rows, D) || !aligned(workspace, 16)))
+    return B200Q_ERR_WORKSPACE;
+  a.q = q; a.q_f16 = dtype == B200Q_F16;
+  a.qb = q_strides[0]; a.qh = q_strides[1]; a.qt = q_strides[2];
+  a.out = out;
+  a.ob = out_strides[0]; a.oh = out_strides[1]; a.ot = out_strides[2];
+  a.lse = lse;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + (splits > 1 ? size_t(splits) * rows * D : 0);
+  a.lens = lens;
+  a.B = static_cast<int>(B); a.Hq = static_cast<int>(Hq); a.G = static_cast<int>(Hq / heads);
+  a.Tq = static_cast<int>(Tq); a.causal = causal != 0; a.splits = splits;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
+                  static_cast<unsigned>(B));
+  int s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, 0, 1, st, a)
+                   : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, 0, 1, st, a);
+  if (s != B200Q_OK || splits == 1) return s;
+  const dim3 jgrid(static_cast<unsigned>(cdiv(rows, 4)));
+  return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, 128, 0, 1, st, a)
+                  : launch(kv8_attn_join_kernel<64>, jgrid, 128, 0, 1, st, a);
+}
+
+}  // extern "C"

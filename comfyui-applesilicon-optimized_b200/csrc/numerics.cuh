@@ -119,7 +119,7 @@ __device__ __forceinline__ float silu_f32_exact_inl(float a) {
   const float e = __double2float_rn(exp(-static_cast<double>(a)));
   return __fdiv_rn(a, __fadd_rn(1.0f, e));
 }
-__device__ __noinline__ float silu_f32_exact(float a) { return silu_f32_exact_inl(a); }
+static __device__ __noinline__ float silu_f32_exact(float a) { return silu_f32_exact_inl(a); }
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

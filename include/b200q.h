@@ -367,6 +367,101 @@ B200Q_API int b200q_w8a16_linear_noalloc(const void* x, int x_dtype, int64_t ldx
 B200Q_API int b200q_fp8_decode(const uint8_t* src, int64_t n, int fp8_kind, void* dst, int out_dtype,
                      void* stream);
 
+/* ---- Low-bit decode operators (no reference counterpart: the reference has no
+ * 4-bit weights, no fused block norms and no key/value cache). */
+
+/* 4-bit weight-only linear: out = act(X . W^T + bias) with
+ *   W[n,k] = scales[n, k/group] * (code[n,k] - zeros[n, k/group]),
+ * code 0..15, two per byte along K (even k in the low nibble), w [N, K/2] bytes
+ * with row stride ldw (a multiple of 16, base 16-byte aligned); scales
+ * [N, K/group] contiguous, scale_dtype a B200Q_BIAS_* code; zeros [N, K/group]
+ * bytes 0..15 or NULL (8).  group 32, 64 or 128, K % group == 0.  X [M, K]
+ * bf16/f16, bias bf16/f16/f32 or NULL, out bf16/f16/f32.  fp32 accumulation.
+ * M <= 32 rounds once, at the output; larger M decodes W to fp16 in the
+ * workspace (one rounding to 11 bits per weight) for the tile GEMM, and needs
+ * b200q_w4a16_workspace_size bytes, 256-byte aligned (and, for f16 X, rows on
+ * 16-byte boundaries). */
+B200Q_API size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K);
+B200Q_API int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w,
+                                 int64_t ldw, const void* scales, int scale_dtype,
+                                 const uint8_t* zeros, int64_t group, const void* bias,
+                                 int bias_dtype, int act, void* out, int out_dtype, int64_t ldo,
+                                 int64_t M, int64_t N, int64_t K, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* norm kinds */
+#define B200Q_NORM_NONE 0
+#define B200Q_NORM_RMS 1
+#define B200Q_NORM_LAYER 2
+#define B200Q_NORM_MAX_D 32768
+
+/* The norms before and after a block, in one pass over rows of D values:
+ *   with y:    h = res_scale * x + gate[b] * (norm_post(y) * post_w),  else h = x
+ *   out (or q, q_scale) = norm_pre(h) * w * (1 + scale[b]) + shift[b]
+ * b = row / rows_per_mod.  x, y, h, out are bf16/f16 (dtype); post_w, w [D] and
+ * gate, scale, shift [mods, D] (row strides ld_*) are bf16/f16/f32 by their
+ * B200Q_BIAS_* codes, each may be NULL (factor 1 / term 0).  h may be NULL; out
+ * and q may not both be given; q [rows, D] int8 with q_scale [rows] fp32 =
+ * max|out| / 127 (a row with a non-finite value gets a NaN scale).  The second
+ * norm and the quantization take the unrounded h and out.  out and q NULL: h
+ * only. */
+B200Q_API int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype,
+                               int post_kind, const void* post_w, int post_w_dtype,
+                               const void* gate, int64_t ld_gate, float res_scale, int pre_kind,
+                               const void* w, int w_dtype, const void* scale, int64_t ld_scale,
+                               const void* shift, int64_t ld_shift, int mod_dtype,
+                               int64_t rows_per_mod, float eps, void* h, int64_t ldh, void* out,
+                               int64_t ldo, int8_t* q, int64_t ldq, float* q_scale, int64_t rows,
+                               int64_t D, void* stream);
+
+/* Paged 8-bit key/value cache: k_codes, v_codes [pages, heads, block, D] int8 and
+ * k_scale, v_scale [pages, heads] fp32 >= 0 (value = code * scale; all contiguous,
+ * codes 16-byte aligned); table [B, max_blocks] int32, row stride ld_table: the
+ * page of each block of `block` tokens of a sequence.  block 16, 32, 64 or 128;
+ * D 64 or 128.  Page numbers are checked on the device: a bad one sets bit 1 of
+ * b200q_get_device_status and its tokens are skipped.
+ *
+ * append: k, v [B, heads, S, D] bf16/f16 (strides of the first three axes, in
+ * elements, multiples of 8; 16-byte aligned): sequence b's first counts[b]
+ * tokens (NULL: S) go to positions start[b], start[b] + 1, ...  A block's scale
+ * becomes max(its scale if it already holds tokens, max|new| / 127); codes it
+ * holds are requantized when the scale grew.  Sequences must not share a page
+ * that is written. */
+B200Q_API int b200q_kv8_append(const void* k, const void* v, int dtype, int64_t B, int64_t S,
+                               const int64_t* k_strides, const int64_t* v_strides,
+                               int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,
+                               int64_t pages, int64_t heads, int64_t block, int64_t D,
+                               const int32_t* table, int64_t ld_table, int64_t max_blocks,
+                               const int32_t* start, const int32_t* counts, void* stream);
+
+/* gather: k, v [B, heads, S, D] contiguous (bf16/f16/f32) = the values of tokens
+ * first[b] .. first[b] + counts[b] - 1; zeros behind them. */
+B200Q_API int b200q_kv8_gather(const int8_t* k_codes, const int8_t* v_codes, const float* k_scale,
+                               const float* v_scale, int64_t pages, int64_t heads, int64_t block,
+                               int64_t D, const int32_t* table, int64_t ld_table,
+                               int64_t max_blocks, const int32_t* first, const int32_t* counts,
+                               void* k, void* v, int out_dtype, int64_t B, int64_t S,
+                               void* stream);
+
+/* attention: q [B, Hq, Tq, D] bf16/f16 (Hq a multiple of heads; query head i uses
+ * cache head i / (Hq / heads)) over the first lens[b] tokens of sequence b.
+ * causal: query i of Tq sees positions <= lens[b] - Tq + i; otherwise all.  out
+ * [B, Hq, Tq, D] like q, lse [B, Hq, Tq] fp32 contiguous (natural log of the
+ * softmax's sum); a row that sees nothing gives 0 and -inf.  max_len: an upper
+ * bound of lens used for planning only.  workspace:
+ * b200q_kv8_attention_workspace_size bytes (same max_len). */
+B200Q_API size_t b200q_kv8_attention_workspace_size(int64_t B, int64_t Hq, int64_t heads,
+                                                    int64_t Tq, int64_t D, int64_t max_len);
+B200Q_API int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Tq,
+                                  const int64_t* q_strides, const int8_t* k_codes,
+                                  const int8_t* v_codes, const float* k_scale,
+                                  const float* v_scale, int64_t pages, int64_t heads,
+                                  int64_t block, int64_t D, const int32_t* table,
+                                  int64_t ld_table, int64_t max_blocks, const int32_t* lens,
+                                  int64_t max_len, int causal, float softmax_scale, void* out,
+                                  const int64_t* out_strides, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
