@@ -110,21 +110,9 @@ _SIGNATURES = {
                                            _i64, _i64, _i64, _vp], _int),
     "b200q_i8_mlp_bridge_prequant": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                                       _int, _i64, _vp, _vp, _i64, _vp, _vp], _int),
-    # low-bit decode operators (bindings: ../w4.py, ../block_norm.py, ../kv8.py)
     "b200q_w4a16_workspace_size": ([_i64, _i64, _i64], _sz),
     "b200q_w4a16_linear": ([_vp, _int, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp, _int, _int, _vp,
                             _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp], _int),
-    "b200q_block_norm": ([_vp, _i64, _vp, _i64, _int, _int, _vp, _int, _vp, _i64, ctypes.c_float,
-                          _int, _vp, _int, _vp, _i64, _vp, _i64, _int, _i64, ctypes.c_float, _vp,
-                          _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _vp], _int),
-    "b200q_kv8_append": ([_vp, _vp, _int, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
-                          _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp], _int),
-    "b200q_kv8_gather": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
-                          _vp, _vp, _int, _i64, _i64, _vp], _int),
-    "b200q_kv8_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64], _sz),
-    "b200q_kv8_attention": ([_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
-                             _i64, _i64, _vp, _i64, _i64, _vp, _i64, _int, ctypes.c_float, _vp,
-                             _vp, _vp, _vp, _sz, _vp], _int),
 }
 
 
@@ -179,22 +167,27 @@ def _p(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
 
-class _SameDevice:
-    """The tensors' device is current already."""
-
-    def __enter__(self):
-        pass
-
-    def __exit__(self, *exc):
-        return False
+_bindings = None
 
 
-_SAME_DEVICE = _SameDevice()
-
-
-def device_of(dev):
-    """Context that makes ``dev`` current (nothing to do when it is)."""
-    return _SAME_DEVICE if torch._C._cuda_getDevice() == dev.index else torch.cuda.device(dev)
+def bindings():
+    """The compiled Python bindings of the low-bit decode operators (csrc/bindings.cpp,
+    on top of the library; raises if they were not built)."""
+    global _bindings
+    if _bindings is None:
+        import importlib.machinery
+        import importlib.util
+        lib()
+        path = os.path.join(os.path.dirname(_LIB_PATH), "b200q_bindings.so")
+        if not os.path.exists(path):
+            raise RuntimeError(f"{TAG} bindings missing at {path}; run the build "
+                               f"(__graft_entry__.build() or csrc/build.py)")
+        loader = importlib.machinery.ExtensionFileLoader("b200q_bindings", path)
+        spec = importlib.util.spec_from_file_location("b200q_bindings", path, loader=loader)
+        mod = importlib.util.module_from_spec(spec)
+        loader.exec_module(mod)
+        _bindings = mod
+    return _bindings
 
 
 def _require_cuda(*ts):

@@ -1,8 +1,10 @@
-"""Build the b200q C-ABI library in-tree: ``_lib/libb200q.so`` (sm_100a).
+"""Build in-tree: the b200q C-ABI library ``_lib/libb200q.so`` (sm_100a) and, on
+top of it, ``_lib/b200q_bindings.so``, the CPython bindings of the low-bit decode
+operators (``bindings.cpp``, against torch's headers).
 
 Usage: ``python csrc/build.py [--verbose]``.  Rebuilds only when a source is
 newer than the library.  nvcc cross-compiles, so no GPU is needed.  The
-translation unit is compiled without --use_fast_math: the INT8 epilogue and the
+translation units are compiled without --use_fast_math: the INT8 epilogue and the
 quantizers rely on IEEE round-to-nearest fp32 arithmetic.
 """
 import os
@@ -33,7 +35,37 @@ def nvcc_cmd(unit, out, extra=()):
 
 def link_cmd(objects, out=OUT):
     nvcc = os.environ.get("NVCC", "nvcc")
-    return [nvcc, *FLAGS, "-shared", "-o", out, *objects]
+    return [nvcc, *FLAGS, "-shared", "-Xlinker", "-soname=libb200q.so", "-o", out, *objects]
+
+
+BINDINGS = os.path.join(PACK, "_lib", "b200q_bindings.so")
+BINDINGS_SOURCES = [os.path.join(HERE, "bindings.cpp"), HEADER]
+
+
+def cxx_runtime():
+    """The libstdc++.so.6 that torch has loaded into this process.  The bindings share
+    exceptions with torch, so they must not bring a runtime of their own, and a
+    compiler may have only the static one beside it."""
+    with open("/proc/self/maps") as f:
+        for line in f:
+            path = line.split(maxsplit=5)[-1].strip()
+            if os.path.basename(path).startswith("libstdc++.so.6"):
+                return path
+    return "-lstdc++"
+
+
+def bindings_cmd(out=BINDINGS):
+    import sysconfig
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    inc = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *[a for d in inc for a in ("-isystem", d)], "-o", out, os.path.join(HERE, "bindings.cpp"),
+            OUT, "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+            "-lc10_cuda", "-nostdlib++", cxx_runtime(), "-Wl,-rpath,$ORIGIN"]
 
 
 def object_of(unit):
@@ -53,7 +85,8 @@ def unit_sources(unit):
 
 
 def up_to_date():
-    return newer(OUT, [s for unit in UNITS for s in unit_sources(unit)])
+    return (newer(OUT, [s for unit in UNITS for s in unit_sources(unit)])
+            and newer(BINDINGS, BINDINGS_SOURCES))
 
 
 def build(force=False, verbose=False):
@@ -82,9 +115,15 @@ def build(force=False, verbose=False):
             print(msg)
     if failed:
         raise RuntimeError("\n".join(failed))
-    r = subprocess.run(link_cmd([object_of(u) for u in UNITS]), capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed ({r.returncode}):\n{r.stdout}{r.stderr}")
+    steps = [link_cmd([object_of(u) for u in UNITS])]
+    if force or not newer(BINDINGS, BINDINGS_SOURCES):
+        steps.append(bindings_cmd())
+    for cmd in steps:
+        if verbose:
+            print(" ".join(cmd))
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({r.returncode}):\n{r.stdout}{r.stderr}")
     return OUT
 
 
