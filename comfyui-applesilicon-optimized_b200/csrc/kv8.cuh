@@ -226,6 +226,39 @@ struct Kv8AttnArgs {
 };
 
 constexpr int kAttnWarps = 4;
+constexpr int kAttnStages = 4;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One stage of a warp's ring: 16 tokens of K and V, the block's scales, and
+// whether its page number was good.
+template <int D>
+struct AttnStage {
+  uint8_t k[16 * D], v[16 * D];
+  float ks, vs;
+  int ok, pad;
+};
+template <int D>
+constexpr int attn_smem_bytes() {
+  return kAttnWarps * kAttnStages * static_cast<int>(sizeof(AttnStage<D>));
+}
+// Byte offset of 16-byte chunk `ch` of token row `row`, XOR-swizzled so that the
+// K reads (rows g, chunks of quarter t) and the V reads (rows 2t, chunk g) of a
+// warp are both free of bank conflicts (D = 64: V's 8-byte reads 2-way).
+template <int D>
+__device__ __forceinline__ int attn_at(int row, int ch) {
+  return D == 128 ? row * 128 + ((ch ^ (row & 7)) << 4) : row * 64 + ((ch ^ ((row >> 1) & 3)) << 4);
+}
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -344,34 +377,64 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
     for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
+  // This warp's tiles t0 + warp, + kAttnWarps, ... go through a ring of its own:
+  // asynchronous copies run kAttnStages - 1 tiles ahead, no barrier between warps.
+  extern __shared__ __align__(128) uint8_t attn_smem[];
+  AttnStage<D>* ring = reinterpret_cast<AttnStage<D>*>(attn_smem) + warp * kAttnStages;
   const int64_t head_bytes = static_cast<int64_t>(c.T) * D;
+  auto issue = [&](int tile, int slot) {
+    if (tile < t1) {
+      const int pos = tile << 4;
+      const int page = kv8_page(c, b, pos >> c.log_t);
+      AttnStage<D>* st = ring + slot;
+      if (lane == 0) st->ok = page >= 0;
+      if (page >= 0) {
+        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+        const int64_t from = at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
+        const uint32_t kd = smem_u32(st->k), vd = smem_u32(st->v);
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const int i = lane + 32 * j, row = i / (D / 16), ch = i % (D / 16);
+          cp_async16(kd + attn_at<D>(row, ch), c.k + from + i * 16);
+          cp_async16(vd + attn_at<D>(row, ch), c.v + from + i * 16);
+        }
+        if (lane == 0) cp_async4(smem_u32(&st->ks), c.ks + at);
+        if (lane == 1) cp_async4(smem_u32(&st->vs), c.vs + at);
+      }
+    }
+    cp_async_commit();  // one group per tile, empty past the end
+  };
+#pragma unroll
+  for (int i = 0; i < kAttnStages - 1; ++i) issue(t0 + warp + kAttnWarps * i, i);
+
+  int slot = 0;
   for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
+    cp_async_wait<kAttnStages - 2>();
+    __syncwarp();  // the tile has landed for every lane, and the slot read last is free
+    issue(tile + kAttnWarps * (kAttnStages - 1), (slot + kAttnStages - 1) % kAttnStages);
+    const AttnStage<D>* st = ring + slot;
+    slot = (slot + 1) % kAttnStages;
+    if (!st->ok) continue;
     const int pos = tile << 4;
-    const int page = kv8_page(c, b, pos >> c.log_t);
-    if (page < 0) continue;
-    const int64_t at = static_cast<int64_t>(page) * c.heads + h;
-    const int8_t* kp = c.k + at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
-    const int8_t* vp = c.v + at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
-    const float ks = __ldg(c.ks + at), vs = __ldg(c.vs + at);
+    const float ks = st->ks, vs = st->vs;
 
     uint32_t kw[2][KW], vw[4][VW];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const uint4* p = reinterpret_cast<const uint4*>(kp + (8 * i + g) * D + t * (D / 4));
 #pragma unroll
       for (int j = 0; j < KW / 4; ++j) {
-        const uint4 v = __ldg(p + j);
+        const uint4 v = *reinterpret_cast<const uint4*>(st->k + attn_at<D>(8 * i + g, t * (KW / 4) + j));
         kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
       }
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int8_t* p = vp + (2 * t + (i & 1) + 8 * (i >> 1)) * D + g * (D / 8);
+      const int row = 2 * t + (i & 1) + 8 * (i >> 1);
       if constexpr (VW == 4) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint4 v = *reinterpret_cast<const uint4*>(st->v + attn_at<D>(row, g));
         vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
       } else {
-        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+        const uint2 v = *reinterpret_cast<const uint2*>(st->v + attn_at<D>(row, g >> 1) + (g & 1) * 8);
         vw[i][0] = v.x; vw[i][1] = v.y;
       }
     }
@@ -518,41 +581,38 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
   }
 }
 
-// Joins the splits of each row in split order: one warp per row.
+// Joins the splits of each row in split order: one CTA of D threads per row, a
+// thread per value; the splits' loads are independent of one another.
+constexpr int kAttnMaxSplits = 64;
 template <int D>
-__global__ void __launch_bounds__(128) kv8_attn_join_kernel(const Kv8AttnArgs a) {
+__global__ void __launch_bounds__(D) kv8_attn_join_kernel(const Kv8AttnArgs a) {
+  __shared__ float ml[kAttnMaxSplits][2];
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t flat = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Tq;
-  if (flat >= rows) return;
-  const int lane = threadIdx.x & 31;
-  constexpr int PL = D / 32;  // values per lane
+  const int64_t flat = blockIdx.x, rows = gridDim.x;
+  for (int i = threadIdx.x; i < a.splits; i += D) {
+    const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (i * rows + flat) * 2);
+    ml[i][0] = v.x;
+    ml[i][1] = v.y;
+  }
+  __syncthreads();
   float mt = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ml[s][0]);
+  const float* p = a.part_o + flat * D + threadIdx.x;
+  float lt = 0.0f, acc = 0.0f;
+#pragma unroll 8
   for (int s = 0; s < a.splits; ++s) {
-    const float x = a.part_ml[(s * rows + flat) * 2];
-    mt = fmaxf(mt, x);
+    const float f = safe_ex2_diff(ml[s][0], mt);
+    lt = fmaf(ml[s][1], f, lt);
+    acc = fmaf(p[s * rows * D], f, acc);
   }
-  float lt = 0.0f, acc[PL];
-#pragma unroll
-  for (int i = 0; i < PL; ++i) acc[i] = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = safe_ex2_diff(a.part_ml[(s * rows + flat) * 2], mt);
-    lt += a.part_ml[(s * rows + flat) * 2 + 1] * f;
-    const float* p = a.part_o + (s * rows + flat) * D + lane * PL;
-#pragma unroll
-    for (int i = 0; i < PL; ++i) acc[i] = fmaf(p[i], f, acc[i]);
-  }
-  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  acc = lt == 0.0f ? 0.0f : acc / lt;
   const int ti = static_cast<int>(flat % a.Tq);
-  const int64_t bh = flat / a.Tq;
-  const int64_t b = bh / a.Hq, hi = bh - b * a.Hq;
-  uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + lane * PL;
-#pragma unroll
-  for (int i = 0; i < PL; i += 2)
-    *reinterpret_cast<uint32_t*>(dst + i) = a.q_f16 ? pack_f16x2(acc[i] * inv, acc[i + 1] * inv)
-                                                    : pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
-  if (lane == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
+  const int64_t bh = flat / a.Tq, b = bh / a.Hq, hi = bh - b * a.Hq;
+  const int64_t at = b * a.ob + hi * a.oh + ti * a.ot + threadIdx.x;
+  if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(acc);
+  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(acc);
+  if (threadIdx.x == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
 }
 
 }  // namespace b200q

@@ -174,14 +174,15 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
   return launch(kv8_append_kernel<T, 8>, grid, kKvThreads, 0, 1, st, a);
 }
 
-// How many CTAs share a sequence's length: enough to fill the GPU, at least 128
-// tokens each.
+// How many CTAs share a sequence's length: enough to give every SM two, and at
+// most 4096 tokens each so that ragged batches balance; at least 128 tokens each.
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t base = B * heads * cdiv(Hq / heads * Tq, 16);
-  int64_t s = cdiv(int64_t(sms) * 6, base);
+  int64_t s = cdiv(int64_t(sms) * 2, base);
+  if (s < cdiv(max_len, 4096)) s = cdiv(max_len, 4096);
   const int64_t most = cdiv(max_len, 128);
   if (s > most) s = most;
-  if (s > 64) s = 64;
+  if (s > kAttnMaxSplits) s = kAttnMaxSplits;
   return s < 1 ? 1 : static_cast<int>(s);
 }
 size_t attn_work_bytes(int splits, int64_t rows, int64_t D) {
@@ -189,7 +190,7 @@ size_t attn_work_bytes(int splits, int64_t rows, int64_t D) {
 }
 bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
   return B >= 0 && B <= 65535 && heads >= 1 && Hq >= heads && Hq % heads == 0 && Tq >= 0 &&
-         Hq / heads * Tq <= kIntMax && heads * cdiv(Hq / heads * Tq, 16) <= 65535;
+         Hq / heads * Tq <= kIntMax && B * Hq * Tq <= kIntMax && heads * cdiv(Hq / heads * Tq, 16) <= 65535;
 }
 
 }  // namespace
@@ -411,12 +412,12 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
                   static_cast<unsigned>(B));
-  int s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, 0, 1, st, a)
-                   : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, 0, 1, st, a);
+  int s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
+                   : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
   if (s != B200Q_OK || splits == 1) return s;
-  const dim3 jgrid(static_cast<unsigned>(cdiv(rows, 4)));
+  const dim3 jgrid(static_cast<unsigned>(rows));
   return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, 128, 0, 1, st, a)
-                  : launch(kv8_attn_join_kernel<64>, jgrid, 128, 0, 1, st, a);
+                  : launch(kv8_attn_join_kernel<64>, jgrid, 64, 0, 1, st, a);
 }
 
 }  // extern "C"
