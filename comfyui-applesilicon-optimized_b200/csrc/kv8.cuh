@@ -301,6 +301,83 @@ __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
   return m == -INFINITY ? 0.0f : ex2f(m - top);
 }
 
+// Starts the copies of 16-token tile `tile` of (sequence b, head h) into `st`, one
+// group per call (an empty one past the end).
+template <int D>
+__device__ __forceinline__ void attn_issue(const Kv8Cache& c, int b, int h, int tile, int end,
+                                           AttnStage<D>* st, int lane) {
+  if (tile < end) {
+    const int pos = tile << 4;
+    const int page = kv8_page(c, b, pos >> c.log_t);
+    if (lane == 0) st->ok = page >= 0;
+    if (page >= 0) {
+      const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+      const int64_t from = at * (static_cast<int64_t>(c.T) * D) + static_cast<int64_t>(pos & (c.T - 1)) * D;
+      const uint32_t kd = smem_u32(st->k), vd = smem_u32(st->v);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+        const int i = lane + 32 * j, row = i / (D / 16), ch = i % (D / 16);
+        cp_async16(kd + attn_at<D>(row, ch), c.k + from + i * 16);
+        cp_async16(vd + attn_at<D>(row, ch), c.v + from + i * 16);
+      }
+      if (lane == 0) cp_async4(smem_u32(&st->ks), c.ks + at);
+      if (lane == 1) cp_async4(smem_u32(&st->vs), c.vs + at);
+    }
+  }
+  cp_async_commit();
+}
+// This lane's K and V words of a stage: K tokens g and g + 8, quarter t; V tokens 2t,
+// 2t+1, 2t+8, 2t+9, eighth g.
+template <int D>
+__device__ __forceinline__ void attn_read(const AttnStage<D>* st, int g, int t, uint32_t (&kw)[2][D / 16],
+                                          uint32_t (&vw)[4][D / 32]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(st->k + attn_at<D>(8 * i + g, t * (D / 64) + j));
+      kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+    if constexpr (D == 128) {
+      const uint4 v = *reinterpret_cast<const uint4*>(st->v + attn_at<D>(row, g));
+      vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(st->v + attn_at<D>(row, g >> 1) + (g & 1) * 8);
+      vw[i][0] = v.x; vw[i][1] = v.y;
+    }
+  }
+}
+// Stores 4 values (d .. d+3) of packed row r, or hands them over to the join.
+template <int D>
+__device__ __forceinline__ void attn_finish(const Kv8AttnArgs& a, int b, int h, int split, int r, int d,
+                                            float4 x, float m, float l) {
+  const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
+  const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
+  if (a.splits > 1) {
+    const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
+    *reinterpret_cast<float4*>(a.part_o + at * D + d) = x;
+    if (d == 0) {
+      a.part_ml[at * 2] = m;
+      a.part_ml[at * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + d;
+  *reinterpret_cast<uint2*>(dst) =
+      a.q_f16 ? make_uint2(pack_f16x2(x.x * inv, x.y * inv), pack_f16x2(x.z * inv, x.w * inv))
+              : make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  if (d == 0) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+// Positions that token ti of Tq sees.
+__device__ __forceinline__ int attn_limit(const Kv8AttnArgs& a, int len, int ti) {
+  return a.causal ? min(max(len - a.Tq + ti + 1, 0), len) : len;
+}
+
 template <int D>
 __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8AttnArgs a) {
   constexpr int KS = D / 16;   // k16 steps of the K product
@@ -381,29 +458,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
   // asynchronous copies run kAttnStages - 1 tiles ahead, no barrier between warps.
   extern __shared__ __align__(128) uint8_t attn_smem[];
   AttnStage<D>* ring = reinterpret_cast<AttnStage<D>*>(attn_smem) + warp * kAttnStages;
-  const int64_t head_bytes = static_cast<int64_t>(c.T) * D;
-  auto issue = [&](int tile, int slot) {
-    if (tile < t1) {
-      const int pos = tile << 4;
-      const int page = kv8_page(c, b, pos >> c.log_t);
-      AttnStage<D>* st = ring + slot;
-      if (lane == 0) st->ok = page >= 0;
-      if (page >= 0) {
-        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
-        const int64_t from = at * head_bytes + static_cast<int64_t>(pos & (c.T - 1)) * D;
-        const uint32_t kd = smem_u32(st->k), vd = smem_u32(st->v);
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          const int i = lane + 32 * j, row = i / (D / 16), ch = i % (D / 16);
-          cp_async16(kd + attn_at<D>(row, ch), c.k + from + i * 16);
-          cp_async16(vd + attn_at<D>(row, ch), c.v + from + i * 16);
-        }
-        if (lane == 0) cp_async4(smem_u32(&st->ks), c.ks + at);
-        if (lane == 1) cp_async4(smem_u32(&st->vs), c.vs + at);
-      }
-    }
-    cp_async_commit();  // one group per tile, empty past the end
-  };
+  auto issue = [&](int tile, int slot) { attn_issue<D>(c, b, h, tile, t1, ring + slot, lane); };
 #pragma unroll
   for (int i = 0; i < kAttnStages - 1; ++i) issue(t0 + warp + kAttnWarps * i, i);
 
@@ -419,25 +474,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
     const float ks = st->ks, vs = st->vs;
 
     uint32_t kw[2][KW], vw[4][VW];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < KW / 4; ++j) {
-        const uint4 v = *reinterpret_cast<const uint4*>(st->k + attn_at<D>(8 * i + g, t * (KW / 4) + j));
-        kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-      if constexpr (VW == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(st->v + attn_at<D>(row, g));
-        vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
-      } else {
-        const uint2 v = *reinterpret_cast<const uint2*>(st->v + attn_at<D>(row, g >> 1) + (g & 1) * 8);
-        vw[i][0] = v.x; vw[i][1] = v.y;
-      }
-    }
+    attn_read<D>(st, g, t, kw, vw);
 
     // ---- scores of 16 tokens
     float s[2][4];
@@ -559,25 +596,246 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
   for (int e = tid; e < 16 * (D / 4); e += kAttnWarps * 32) {
     const int row = e / (D / 4), d = (e - row * (D / 4)) * 4, r = r0 + row;
     if (r >= rows) continue;
-    const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
-    const float4 x = *reinterpret_cast<const float4*>(&sm_o[row][d]);
-    const float mm = sm_fin[row][0], ll = sm_fin[row][1];
-    const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
-    if (a.splits > 1) {
-      const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
-      *reinterpret_cast<float4*>(a.part_o + at * D + d) = x;
-      if (d == 0) {
-        a.part_ml[at * 2] = mm;
-        a.part_ml[at * 2 + 1] = ll;
-      }
-      continue;
+    attn_finish<D>(a, b, h, split, r, d, *reinterpret_cast<const float4*>(&sm_o[row][d]), sm_fin[row][0],
+                   sm_fin[row][1]);
+  }
+}
+
+// ---- up to 8 rows per key/value head (one token of up to 8 grouped heads)
+//
+// q.K on the integer tensor path: q's row, scaled by a power of two 2^-E to
+// |v| < 128, is three int8 digits v = p0 + p1 / 128 + p2 / 128^2 (within 2^-22 of
+// 2^E), and K's codes are the other operand as they are stored: no instruction
+// converts them.  Rows 0-7 of an m16n8k32 MMA hold p0 and rows 8-15 p1 of the 8
+// rows, a second MMA p2.  The int32 accumulators start at the bits of 1.5 * 2^23,
+// so a subtraction turns each sum (|sum| <= 128 * 127 * 128 < 2^22) into its fp32
+// value exactly.
+//
+// P V is computed transposed, V^T (16 d x 16 tokens) as the MMA's rows and P as its
+// 8 columns: half the MMAs and accumulators of the 16-row form.
+__device__ __forceinline__ void mma_s8_start(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const int z = 0x4B400000;
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(z));
+}
+__device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Three int8 digits of v, |v| < 128.
+__device__ __forceinline__ void digits3(float v, int& p0, int& p1, int& p2) {
+  const float a = fminf(fmaxf(rintf(v), -127.0f), 127.0f);
+  const float r = (v - a) * 128.0f;
+  const float c = fminf(fmaxf(rintf(r), -127.0f), 127.0f);
+  const float e = fminf(fmaxf(rintf((r - c) * 128.0f), -127.0f), 127.0f);
+  p0 = static_cast<int>(a);
+  p1 = static_cast<int>(c);
+  p2 = static_cast<int>(e);
+}
+// 2^E above the largest |value| of 16-bit bits `top`, as (2^-E * 128, 2^E / 128);
+// NaN for a row holding inf or NaN.
+__device__ __forceinline__ void digit_scale(uint32_t top, int f16, float* down, float* up) {
+  const uint16_t tb = static_cast<uint16_t>(top);
+  const float m = f16 ? __half2float(*reinterpret_cast<const __half*>(&tb))
+                      : __uint_as_float(top << 16);
+  int ex = static_cast<int>(__float_as_uint(m) >> 23);  // biased: m < 2^(ex - 126)
+  const bool bad = ex == 255;
+  ex = min(max(ex, 8), 254);
+  *down = __uint_as_float(static_cast<uint32_t>(126 - ex + 127 + 7) << 23);
+  *up = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(ex - 126 + 127 - 7) << 23);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8AttnArgs a) {
+  constexpr int KS = D / 32;   // k32 steps of the K product
+  constexpr int VW = D / 32;   // words per lane and V token
+  constexpr int NM = D / 16;   // m16 tiles of the output
+  __shared__ float sm_ml[kAttnWarps][8][2];
+  __shared__ float sm_o[8][D + 4];
+  extern __shared__ __align__(128) uint8_t attn_smem[];
+  griddep_wait();
+  griddep_launch_dependents();
+  const Kv8Cache& c = a.c;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int split = blockIdx.x, b = blockIdx.z, rows = a.G * a.Tq, h = blockIdx.y;
+  const int len = min(max(a.lens[b], 0), c.max_blocks << c.log_t);
+  const int lim = attn_limit(a, len, min(g, rows - 1) / a.G);
+  const int lim_max = attn_limit(a, len, (rows - 1) / a.G), lim_min = attn_limit(a, len, 0);
+  const int tiles = (lim_max + 15) >> 4;
+  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+
+  AttnStage<D>* ring = reinterpret_cast<AttnStage<D>*>(attn_smem) + warp * kAttnStages;
+#pragma unroll
+  for (int i = 0; i < kAttnStages - 1; ++i)
+    attn_issue<D>(c, b, h, t0 + warp + kAttnWarps * i, t1, ring + i, lane);
+
+  // ---- q digits of row g, quarter t
+  uint32_t q01[KS][4], q2[KS][4];
+  float sc;
+  {
+    const int r = min(g, rows - 1), ti = r / a.G, hi = h * a.G + (r - ti * a.G);
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qb + hi * a.qh + ti * a.qt + t * (D / 4);
+    uint32_t raw[D / 8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      raw[4 * j] = v.x; raw[4 * j + 1] = v.y; raw[4 * j + 2] = v.z; raw[4 * j + 3] = v.w;
     }
-    const float inv = ll == 0.0f ? 0.0f : 1.0f / ll;
-    uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + d;
-    *reinterpret_cast<uint2*>(dst) =
-        a.q_f16 ? make_uint2(pack_f16x2(x.x * inv, x.y * inv), pack_f16x2(x.z * inv, x.w * inv))
-                : make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-    if (d == 0) a.lse[flat] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * 0.6931471805599453f;
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) top = max(top, max(raw[j] & 0x7FFFu, (raw[j] >> 16) & 0x7FFFu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    float down, up;
+    digit_scale(top, a.q_f16, &down, &up);
+    sc = a.scale_log2 * up;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {  // 4 values: word j of the lane's K bytes
+      uint32_t w[3] = {0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t e = static_cast<uint16_t>(raw[2 * j + (i >> 1)] >> (16 * (i & 1)));
+        const float v = a.q_f16 ? __half2float(*reinterpret_cast<const __half*>(&e))
+                                : __uint_as_float(static_cast<uint32_t>(e) << 16);
+        int p0, p1, p2;
+        digits3(v * down, p0, p1, p2);
+        w[0] |= static_cast<uint32_t>(p0 & 255) << (8 * i);
+        w[1] |= static_cast<uint32_t>(p1 & 255) << (8 * i);
+        w[2] |= static_cast<uint32_t>(p2 & 255) << (8 * i);
+      }
+      q01[j >> 1][2 * (j & 1)] = w[0];
+      q01[j >> 1][2 * (j & 1) + 1] = w[1];
+      q2[j >> 1][2 * (j & 1)] = w[2];
+      q2[j >> 1][2 * (j & 1) + 1] = 0;
+    }
+  }
+
+  float o[NM][4];
+#pragma unroll
+  for (int i = 0; i < NM; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  int slot = 0;
+  for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
+    cp_async_wait<kAttnStages - 2>();
+    __syncwarp();  // the tile has landed for every lane, and the slot read last is free
+    attn_issue<D>(c, b, h, tile + kAttnWarps * (kAttnStages - 1), t1,
+                  ring + (slot + kAttnStages - 1) % kAttnStages, lane);
+    const AttnStage<D>* st = ring + slot;
+    slot = (slot + 1) % kAttnStages;
+    if (!st->ok) continue;
+    const float ks = st->ks, vs = st->vs;
+    uint32_t kw[2][D / 16], vw[4][VW];
+    attn_read<D>(st, g, t, kw, vw);
+
+    const bool zero_v = vs == 0.0f;
+    const float lv = zero_v ? 0.0f : log2f(vs), iv = zero_v ? 1.0f : __fdividef(1.0f, vs);
+    const float ksc = ks * sc;
+    float s[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int d01[4], d2[4];
+      mma_s8_start(d01, q01[0], kw[i][0], kw[i][1]);
+      mma_s8_start(d2, q2[0], kw[i][0], kw[i][1]);
+#pragma unroll
+      for (int j = 1; j < KS; ++j) {
+        mma_s8(d01, q01[j], kw[i][2 * j], kw[i][2 * j + 1]);
+        mma_s8(d2, q2[j], kw[i][2 * j], kw[i][2 * j + 1]);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float f0 = __int_as_float(d01[j]) - 12582912.0f, f1 = __int_as_float(d01[j + 2]) - 12582912.0f,
+                    f2 = __int_as_float(d2[j]) - 12582912.0f;
+        s[2 * i + j] = fmaf(fmaf(fmaf(f2, 0.0078125f, f1), 0.0078125f, f0), ksc, lv);
+      }
+    }
+    const int pos = tile << 4;
+    if (pos + 16 > lim_min) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (pos + 8 * (i >> 1) + 2 * t + (i & 1) >= lim) s[i] = -INFINITY;
+    }
+    float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (__any_sync(0xffffffffu, top > m)) {
+      const float mn = fmaxf(m, top);
+      const float corr = safe_ex2_diff(m, mn);
+      m = mn;
+      l *= corr;
+      // the accumulators' columns are rows 2t and 2t + 1
+      const float c0 = __shfl_sync(0xffffffffu, corr, 8 * t), c1 = __shfl_sync(0xffffffffu, corr, 8 * t + 4);
+#pragma unroll
+      for (int i = 0; i < NM; ++i) {
+        o[i][0] *= c0; o[i][1] *= c1;
+        o[i][2] *= c0; o[i][3] *= c1;
+      }
+    }
+    float p[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)  // a masked score is exactly -inf; a NaN one stays NaN
+      p[i] = s[i] == -INFINITY ? 0.0f : ex2f(s[i] - m);
+    l = fmaf((p[0] + p[1]) + (p[2] + p[3]), iv, l);
+    const uint32_t pb0 = zero_v ? 0u : pack_f16x2(p[0], p[1]), pb1 = zero_v ? 0u : pack_f16x2(p[2], p[3]);
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      const uint32_t ta = vw[0][w] ^ 0x80808080u, tb = vw[1][w] ^ 0x80808080u;
+      const uint32_t tc = vw[2][w] ^ 0x80808080u, td = vw[3][w] ^ 0x80808080u;
+      const uint32_t ab0 = __byte_perm(ta, tb, 0x5140), ab1 = __byte_perm(ta, tb, 0x7362);
+      const uint32_t cd0 = __byte_perm(tc, td, 0x5140), cd1 = __byte_perm(tc, td, 0x7362);
+      const uint32_t a0[4] = {i8_lo(ab0), i8_hi(ab0), i8_lo(cd0), i8_hi(cd0)};
+      const uint32_t a1[4] = {i8_lo(ab1), i8_hi(ab1), i8_lo(cd1), i8_hi(cd1)};
+      mma_f16(o[2 * w], a0, pb0, pb1);
+      mma_f16(o[2 * w + 1], a1, pb0, pb1);
+    }
+  }
+
+  // ---- join the warps (in order), then store or hand over the partial
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  if (t == 0) {
+    sm_ml[warp][g][0] = m;
+    sm_ml[warp][g][1] = l;
+  }
+  __syncthreads();
+  auto top_of = [&](int r) {
+    float x = sm_ml[0][r][0];
+#pragma unroll
+    for (int w = 1; w < kAttnWarps; ++w) x = fmaxf(x, sm_ml[w][r][0]);
+    return x;
+  };
+  const float f0 = safe_ex2_diff(sm_ml[warp][2 * t][0], top_of(2 * t));
+  const float f1 = safe_ex2_diff(sm_ml[warp][2 * t + 1][0], top_of(2 * t + 1));
+  for (int w = 0; w < kAttnWarps; ++w) {
+    if (warp == w) {
+#pragma unroll
+      for (int i = 0; i < NM; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // tile i: this lane's rows g and g + 8 are d = (D / 8) g + 2 i and + 1
+          float* q = &sm_o[2 * t + (j & 1)][g * (D / 8) + 2 * i + (j >> 1)];
+          const float x = o[i][j] * ((j & 1) ? f1 : f0);
+          *q = w == 0 ? x : *q + x;
+        }
+    }
+    __syncthreads();
+  }
+  for (int e = tid; e < rows * (D / 4); e += kAttnWarps * 32) {
+    const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
+    const float mt = top_of(r);
+    float lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) lt += sm_ml[w][r][1] * safe_ex2_diff(sm_ml[w][r][0], mt);
+    attn_finish<D>(a, b, h, split, r, d, *reinterpret_cast<const float4*>(&sm_o[r][d]), mt, lt);
   }
 }
 

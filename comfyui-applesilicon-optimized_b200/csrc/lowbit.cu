@@ -412,8 +412,15 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
                   static_cast<unsigned>(B));
-  int s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
-                   : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
+  int s;
+  // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel)
+  if (a.G * Tq <= 8) {
+    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
+                 : launch(kv8_attn8_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
+  } else {
+    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
+                 : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
+  }
   if (s != B200Q_OK || splits == 1) return s;
   const dim3 jgrid(static_cast<unsigned>(rows));
   return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, 128, 0, 1, st, a)
