@@ -954,6 +954,10 @@ int device_sms() {
 }
 int finish_launch() { return ::finish_launch(); }
 bool pdl_on() { return pdl_launch_on(); }
+bool tmap_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t ld_bytes,
+             uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  return make_tmap(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, cols, rows, ld_bytes, box_cols, box_rows, swizzle);
+}
 
 int gemm16_scaled(bool f16, const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M,
                   int64_t N, int64_t K, const EpiArgs& ep, cudaStream_t st) {

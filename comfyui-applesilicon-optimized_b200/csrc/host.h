@@ -3,6 +3,7 @@
 // and the 16-bit tile GEMM.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -18,6 +19,9 @@ int device_sms();
 int finish_launch();
 // B200Q_PDL (read per call): launch kernels as programmatic dependents.
 bool pdl_on();
+// Tensor map of a row-major [rows, cols] byte matrix with box box_cols x box_rows.
+bool tmap_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t ld_bytes,
+             uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 // The status word of lowbit.cu's kernels on the current device (read, and
 // cleared when `reset`); b200q_get_device_status merges it with capi.cu's.
 int lowbit_device_status(unsigned int* status, bool reset);

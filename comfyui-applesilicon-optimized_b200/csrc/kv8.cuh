@@ -227,30 +227,40 @@ struct Kv8AttnArgs {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnStages = 4;
+constexpr int kAttnThreads = (kAttnWarps + 1) * 32;  // and a producer warp
+constexpr int kAttnChunk = 64;                       // tokens per stage
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-// One stage of a warp's ring: 16 tokens of K and V, the block's scales, and
-// whether its page number was good.
+// The CTA's ring: stages of 64 tokens of K and V, brought by TMA with the row
+// swizzle; 16-token tile w of a stage belongs to consumer warp w.  meta: per tile
+// {ks, log2 vs, 1 / vs, state}, state 0 = skip (bad page), 1 = ok, 2 = vs is 0.
 template <int D>
-struct AttnStage {
-  uint8_t k[16 * D], v[16 * D];
-  float ks, vs;
-  int ok, pad;
+struct AttnRing {
+  uint8_t k[kAttnStages][kAttnChunk * D];
+  uint8_t v[kAttnStages][kAttnChunk * D];
+  float4 meta[kAttnStages][kAttnWarps];
+  uint64_t full[kAttnStages], empty[kAttnStages];
+  int abort;
 };
 template <int D>
 constexpr int attn_smem_bytes() {
-  return kAttnWarps * kAttnStages * static_cast<int>(sizeof(AttnStage<D>));
+  return static_cast<int>(sizeof(AttnRing<D>)) + 1024;
+}
+template <int D>
+__device__ __forceinline__ AttnRing<D>* attn_ring() {
+  extern __shared__ uint8_t attn_smem[];  // the swizzle pattern is anchored at 1024 bytes
+  return reinterpret_cast<AttnRing<D>*>((reinterpret_cast<uintptr_t>(attn_smem) + 1023) & ~uintptr_t(1023));
+}
+template <int D>
+__device__ __forceinline__ void attn_ring_init(AttnRing<D>* ring) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kAttnStages; ++i) {
+      mbar_init(&ring->full[i], 1);
+      mbar_init(&ring->empty[i], kAttnWarps);
+    }
+    ring->abort = 0;
+    fence_mbarrier_init();
+  }
+  __syncthreads();
 }
 // Byte offset of 16-byte chunk `ch` of token row `row`, XOR-swizzled so that the
 // K reads (rows g, chunks of quarter t) and the V reads (rows 2t, chunk g) of a
@@ -301,41 +311,70 @@ __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
   return m == -INFINITY ? 0.0f : ex2f(m - top);
 }
 
-// Starts the copies of 16-token tile `tile` of (sequence b, head h) into `st`, one
-// group per call (an empty one past the end).
+// The producer warp: chunks c0 .. c1 - 1 (64 tokens each) of (sequence b, head h).
+// Lane i looks up tile i % 4 of chunk i / 4 of the next eight chunks at once (page,
+// scales, their logarithm and inverse), then the chunks go out one by one: a box of
+// min(T, 64) rows per page.  Tiles at or past `tiles` are not fetched.
 template <int D>
-__device__ __forceinline__ void attn_issue(const Kv8Cache& c, int b, int h, int tile, int end,
-                                           AttnStage<D>* st, int lane) {
-  if (tile < end) {
-    const int pos = tile << 4;
-    const int page = kv8_page(c, b, pos >> c.log_t);
-    if (lane == 0) st->ok = page >= 0;
-    if (page >= 0) {
-      const int64_t at = static_cast<int64_t>(page) * c.heads + h;
-      const int64_t from = at * (static_cast<int64_t>(c.T) * D) + static_cast<int64_t>(pos & (c.T - 1)) * D;
-      const uint32_t kd = smem_u32(st->k), vd = smem_u32(st->v);
-#pragma unroll
-      for (int j = 0; j < D / 32; ++j) {
-        const int i = lane + 32 * j, row = i / (D / 16), ch = i % (D / 16);
-        cp_async16(kd + attn_at<D>(row, ch), c.k + from + i * 16);
-        cp_async16(vd + attn_at<D>(row, ch), c.v + from + i * 16);
+__device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtensorMap* tk, const CUtensorMap* tv,
+                                             AttnRing<D>* ring, int b, int h, int c0, int c1, int tiles) {
+  const Kv8Cache& c = a.c;
+  const int lane = threadIdx.x & 31;
+  const int box = c.T < kAttnChunk ? c.T : kAttnChunk;
+  const int per_box = box >> 4;  // tiles
+  int n = 0;                     // chunks issued
+  bool live = true;
+  for (int base = c0; base < c1 && live; base += 8) {
+    const int tile = base * 4 + lane, pos = tile << 4;
+    int page = -1;
+    float4 meta = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (tile < tiles && (base + (lane >> 2)) < c1) {
+      page = kv8_page(c, b, pos >> c.log_t);
+      if (page >= 0) {
+        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+        const float vs = __ldg(c.vs + at);
+        meta.x = __ldg(c.ks + at);
+        meta.y = vs == 0.0f ? 0.0f : log2f(vs);
+        meta.z = vs == 0.0f ? 1.0f : 1.0f / vs;
+        meta.w = vs == 0.0f ? 2.0f : 1.0f;
       }
-      if (lane == 0) cp_async4(smem_u32(&st->ks), c.ks + at);
-      if (lane == 1) cp_async4(smem_u32(&st->vs), c.vs + at);
+    }
+    const bool lead = page >= 0 && (lane & (per_box - 1)) == 0;
+    const unsigned leads = __ballot_sync(0xffffffffu, lead);
+    const int y = static_cast<int>((static_cast<int64_t>(page) * c.heads + h) * c.T + (pos & (c.T - 1)));
+    for (int i = 0; i < 8 && base + i < c1; ++i, ++n) {
+      const int s = n % kAttnStages;
+      if (n >= kAttnStages && !mbar_wait_warp(&ring->empty[s], ((n / kAttnStages) - 1) & 1, &ring->abort)) {
+        live = false;
+        break;
+      }
+      const bool mine = (lane >> 2) == i;
+      if (mine) ring->meta[s][lane & 3] = meta;
+      __syncwarp();
+      if (lane == 0)
+        mbar_arrive_expect_tx(&ring->full[s], 2 * D * box * __popc((leads >> (4 * i)) & 15u));
+      __syncwarp();
+      if (mine && lead) {
+        tma_load_2d(tk, &ring->full[s], ring->k[s] + (lane & 3) * 16 * D, 0, y);
+        tma_load_2d(tv, &ring->full[s], ring->v[s] + (lane & 3) * 16 * D, 0, y);
+      }
     }
   }
-  cp_async_commit();
+  if (!live && lane == 0) {  // gave up: let the copies in flight land before the CTA ends
+    for (int i = n > kAttnStages ? n - kAttnStages : 0; i < n; ++i)
+      mbar_wait_drain(&ring->full[i % kAttnStages], (i / kAttnStages) & 1);
+  }
 }
-// This lane's K and V words of a stage: K tokens g and g + 8, quarter t; V tokens 2t,
-// 2t+1, 2t+8, 2t+9, eighth g.
+// This lane's K and V words of a 16-token tile: K tokens g and g + 8, quarter t; V
+// tokens 2t, 2t+1, 2t+8, 2t+9, eighth g.
 template <int D>
-__device__ __forceinline__ void attn_read(const AttnStage<D>* st, int g, int t, uint32_t (&kw)[2][D / 16],
-                                          uint32_t (&vw)[4][D / 32]) {
+__device__ __forceinline__ void attn_read(const uint8_t* k, const uint8_t* v_, int g, int t,
+                                          uint32_t (&kw)[2][D / 16], uint32_t (&vw)[4][D / 32]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
     for (int j = 0; j < D / 64; ++j) {
-      const uint4 v = *reinterpret_cast<const uint4*>(st->k + attn_at<D>(8 * i + g, t * (D / 64) + j));
+      const uint4 v = *reinterpret_cast<const uint4*>(k + attn_at<D>(8 * i + g, t * (D / 64) + j));
       kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
     }
   }
@@ -343,10 +382,10 @@ __device__ __forceinline__ void attn_read(const AttnStage<D>* st, int g, int t, 
   for (int i = 0; i < 4; ++i) {
     const int row = 2 * t + (i & 1) + 8 * (i >> 1);
     if constexpr (D == 128) {
-      const uint4 v = *reinterpret_cast<const uint4*>(st->v + attn_at<D>(row, g));
+      const uint4 v = *reinterpret_cast<const uint4*>(v_ + attn_at<D>(row, g));
       vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
     } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(st->v + attn_at<D>(row, g >> 1) + (g & 1) * 8);
+      const uint2 v = *reinterpret_cast<const uint2*>(v_ + attn_at<D>(row, g >> 1) + (g & 1) * 8);
       vw[i][0] = v.x; vw[i][1] = v.y;
     }
   }
@@ -379,13 +418,17 @@ __device__ __forceinline__ int attn_limit(const Kv8AttnArgs& a, int len, int ti)
 }
 
 template <int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads)
+    kv8_attn_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                    const Kv8AttnArgs a) {
   constexpr int KS = D / 16;   // k16 steps of the K product
   constexpr int KW = D / 16;   // 32-bit words per lane and K token (D / 4 bytes)
   constexpr int VW = D / 32;   // words per lane and V token (D / 8 bytes)
   constexpr int NV = D / 8;    // n8 tiles of the output
   __shared__ float sm_ml[kAttnWarps][16][2];
   __shared__ float sm_o[16][D + 4];
+  AttnRing<D>* ring = attn_ring<D>();
+  attn_ring_init<D>(ring);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -412,8 +455,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
   const int lim_max = a.causal ? min(max(len - a.Tq + last / a.G + 1, 0), len) : len;
   const int lim_min = a.causal ? min(max(len - a.Tq + r0 / a.G + 1, 0), len) : len;
   const int tiles = (lim_max + 15) >> 4;  // 16-token tiles to visit
-  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+  const int chunks = (tiles + 3) >> 2;
+  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
+  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
 
   // ---- q fragments, scaled to fp16
   uint32_t qf[KS][4];
@@ -454,27 +498,20 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
     for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-  // This warp's tiles t0 + warp, + kAttnWarps, ... go through a ring of its own:
-  // asynchronous copies run kAttnStages - 1 tiles ahead, no barrier between warps.
-  extern __shared__ __align__(128) uint8_t attn_smem[];
-  AttnStage<D>* ring = reinterpret_cast<AttnStage<D>*>(attn_smem) + warp * kAttnStages;
-  auto issue = [&](int tile, int slot) { attn_issue<D>(c, b, h, tile, t1, ring + slot, lane); };
-#pragma unroll
-  for (int i = 0; i < kAttnStages - 1; ++i) issue(t0 + warp + kAttnWarps * i, i);
-
-  int slot = 0;
-  for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
-    cp_async_wait<kAttnStages - 2>();
-    __syncwarp();  // the tile has landed for every lane, and the slot read last is free
-    issue(tile + kAttnWarps * (kAttnStages - 1), (slot + kAttnStages - 1) % kAttnStages);
-    const AttnStage<D>* st = ring + slot;
-    slot = (slot + 1) % kAttnStages;
-    if (!st->ok) continue;
-    const int pos = tile << 4;
-    const float ks = st->ks, vs = st->vs;
-
+  if (warp == kAttnWarps) attn_produce<D>(a, &tk, &tv, ring, b, h, c0, c1, tiles);
+  for (int n = 0; warp < kAttnWarps && n < c1 - c0; ++n) {
+    const int s_ = n % kAttnStages;
+    if (!mbar_wait_warp(&ring->full[s_], (n / kAttnStages) & 1, &ring->abort)) break;
+    const float4 meta = ring->meta[s_][warp];
     uint32_t kw[2][KW], vw[4][VW];
-    attn_read<D>(st, g, t, kw, vw);
+    attn_read<D>(ring->k[s_] + warp * 16 * D, ring->v[s_] + warp * 16 * D, g, t, kw, vw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ring->empty[s_]);
+    if (meta.w == 0.0f) continue;
+    const int pos = ((c0 + n) * 4 + warp) << 4;
+    const bool zero_v = meta.w == 2.0f;
+    const float lv = meta.y, iv = meta.z;
+    const float ksc[2] = {meta.x * sc[0], meta.x * sc[1]};
 
     // ---- scores of 16 tokens
     float s[2][4];
@@ -488,9 +525,6 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
         mma_f16(s[i], qf[j], i8_lo(w), i8_hi(w));
       }
     }
-    const bool zero_v = vs == 0.0f;
-    const float lv = zero_v ? 0.0f : log2f(vs);
-    const float iv = zero_v ? 1.0f : 1.0f / vs;
     const bool mask = pos + 16 > lim_min;
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -498,7 +532,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int r = j >> 1;
-        s[i][j] = fmaf(s[i][j], ks * sc[r], lv);
+        s[i][j] = fmaf(s[i][j], ksc[r], lv);
         if (mask && pos + 8 * i + 2 * t + (j & 1) >= lim[r]) s[i][j] = -INFINITY;
         top[r] = fmaxf(top[r], s[i][j]);
       }
@@ -552,7 +586,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
   for (int r = 0; r < 2; ++r) {
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
     l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    if (t == 0) {
+    if (t == 0 && warp < kAttnWarps) {
       sm_ml[warp][g + 8 * r][0] = m[r];
       sm_ml[warp][g + 8 * r][1] = l[r];
     }
@@ -593,7 +627,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn_kernel(const Kv8Attn
       sm_fin[g + 8 * r][1] = lt[r];
     }
   __syncthreads();
-  for (int e = tid; e < 16 * (D / 4); e += kAttnWarps * 32) {
+  for (int e = tid; e < 16 * (D / 4); e += kAttnThreads) {
     const int row = e / (D / 4), d = (e - row * (D / 4)) * 4, r = r0 + row;
     if (r >= rows) continue;
     attn_finish<D>(a, b, h, split, r, d, *reinterpret_cast<const float4*>(&sm_o[row][d]), sm_fin[row][0],
@@ -652,13 +686,16 @@ __device__ __forceinline__ void digit_scale(uint32_t top, int f16, float* down, 
 }
 
 template <int D>
-__global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 3)
+    kv8_attn8_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const Kv8AttnArgs a) {
   constexpr int KS = D / 32;   // k32 steps of the K product
   constexpr int VW = D / 32;   // words per lane and V token
   constexpr int NM = D / 16;   // m16 tiles of the output
   __shared__ float sm_ml[kAttnWarps][8][2];
   __shared__ float sm_o[8][D + 4];
-  extern __shared__ __align__(128) uint8_t attn_smem[];
+  AttnRing<D>* ring = attn_ring<D>();
+  attn_ring_init<D>(ring);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -668,18 +705,15 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
   const int lim = attn_limit(a, len, min(g, rows - 1) / a.G);
   const int lim_max = attn_limit(a, len, (rows - 1) / a.G), lim_min = attn_limit(a, len, 0);
   const int tiles = (lim_max + 15) >> 4;
-  const int t0 = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-  const int t1 = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
-
-  AttnStage<D>* ring = reinterpret_cast<AttnStage<D>*>(attn_smem) + warp * kAttnStages;
-#pragma unroll
-  for (int i = 0; i < kAttnStages - 1; ++i)
-    attn_issue<D>(c, b, h, t0 + warp + kAttnWarps * i, t1, ring + i, lane);
+  const int chunks = (tiles + 3) >> 2;
+  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
+  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
+  if (warp == kAttnWarps) attn_produce<D>(a, &tk, &tv, ring, b, h, c0, c1, tiles);
 
   // ---- q digits of row g, quarter t
-  uint32_t q01[KS][4], q2[KS][4];
-  float sc;
-  {
+  uint32_t q01[KS][4], q2[KS][2];
+  float sc = 0.0f;
+  if (warp < kAttnWarps) {
     const int r = min(g, rows - 1), ti = r / a.G, hi = h * a.G + (r - ti * a.G);
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qb + hi * a.qh + ti * a.qt + t * (D / 4);
     uint32_t raw[D / 8];
@@ -712,8 +746,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
       }
       q01[j >> 1][2 * (j & 1)] = w[0];
       q01[j >> 1][2 * (j & 1) + 1] = w[1];
-      q2[j >> 1][2 * (j & 1)] = w[2];
-      q2[j >> 1][2 * (j & 1) + 1] = 0;
+      q2[j >> 1][j & 1] = w[2];
     }
   }
 
@@ -724,32 +757,29 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
     for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  int slot = 0;
-  for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
-    cp_async_wait<kAttnStages - 2>();
-    __syncwarp();  // the tile has landed for every lane, and the slot read last is free
-    attn_issue<D>(c, b, h, tile + kAttnWarps * (kAttnStages - 1), t1,
-                  ring + (slot + kAttnStages - 1) % kAttnStages, lane);
-    const AttnStage<D>* st = ring + slot;
-    slot = (slot + 1) % kAttnStages;
-    if (!st->ok) continue;
-    const float ks = st->ks, vs = st->vs;
+  for (int n = 0; warp < kAttnWarps && n < c1 - c0; ++n) {
+    const int s_ = n % kAttnStages;
+    if (!mbar_wait_warp(&ring->full[s_], (n / kAttnStages) & 1, &ring->abort)) break;
+    const float4 meta = ring->meta[s_][warp];
     uint32_t kw[2][D / 16], vw[4][VW];
-    attn_read<D>(st, g, t, kw, vw);
-
-    const bool zero_v = vs == 0.0f;
-    const float lv = zero_v ? 0.0f : log2f(vs), iv = zero_v ? 1.0f : __fdividef(1.0f, vs);
-    const float ksc = ks * sc;
+    attn_read<D>(ring->k[s_] + warp * 16 * D, ring->v[s_] + warp * 16 * D, g, t, kw, vw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ring->empty[s_]);
+    if (meta.w == 0.0f) continue;
+    const bool zero_v = meta.w == 2.0f;
+    const float lv = meta.y, iv = meta.z, ksc = meta.x * sc;
     float s[4];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       int d01[4], d2[4];
       mma_s8_start(d01, q01[0], kw[i][0], kw[i][1]);
-      mma_s8_start(d2, q2[0], kw[i][0], kw[i][1]);
+      const uint32_t z0[4] = {q2[0][0], 0u, q2[0][1], 0u};
+      mma_s8_start(d2, z0, kw[i][0], kw[i][1]);
 #pragma unroll
       for (int j = 1; j < KS; ++j) {
         mma_s8(d01, q01[j], kw[i][2 * j], kw[i][2 * j + 1]);
-        mma_s8(d2, q2[j], kw[i][2 * j], kw[i][2 * j + 1]);
+        const uint32_t zj[4] = {q2[j][0], 0u, q2[j][1], 0u};
+        mma_s8(d2, zj, kw[i][2 * j], kw[i][2 * j + 1]);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -758,7 +788,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
         s[2 * i + j] = fmaf(fmaf(fmaf(f2, 0.0078125f, f1), 0.0078125f, f0), ksc, lv);
       }
     }
-    const int pos = tile << 4;
+    const int pos = ((c0 + n) * 4 + warp) << 4;
     if (pos + 16 > lim_min) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -802,7 +832,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
   // ---- join the warps (in order), then store or hand over the partial
   l += __shfl_xor_sync(0xffffffffu, l, 1);
   l += __shfl_xor_sync(0xffffffffu, l, 2);
-  if (t == 0) {
+  if (t == 0 && warp < kAttnWarps) {
     sm_ml[warp][g][0] = m;
     sm_ml[warp][g][1] = l;
   }
@@ -813,8 +843,9 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
     for (int w = 1; w < kAttnWarps; ++w) x = fmaxf(x, sm_ml[w][r][0]);
     return x;
   };
-  const float f0 = safe_ex2_diff(sm_ml[warp][2 * t][0], top_of(2 * t));
-  const float f1 = safe_ex2_diff(sm_ml[warp][2 * t + 1][0], top_of(2 * t + 1));
+  const int wi = min(warp, kAttnWarps - 1);
+  const float f0 = safe_ex2_diff(sm_ml[wi][2 * t][0], top_of(2 * t));
+  const float f1 = safe_ex2_diff(sm_ml[wi][2 * t + 1][0], top_of(2 * t + 1));
   for (int w = 0; w < kAttnWarps; ++w) {
     if (warp == w) {
 #pragma unroll
@@ -829,7 +860,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) kv8_attn8_kernel(const Kv8Att
     }
     __syncthreads();
   }
-  for (int e = tid; e < rows * (D / 4); e += kAttnWarps * 32) {
+  for (int e = tid; e < rows * (D / 4); e += kAttnThreads) {
     const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
     const float mt = top_of(r);
     float lt = 0.0f;

@@ -145,7 +145,7 @@ bool make_cache(Kv8Cache* c, int8_t* k, int8_t* v, float* ks, float* vs, int64_t
   if (!k || !v || !ks || !vs || !table || pages < 1 || pages > kIntMax || heads < 1 ||
       heads > 65535 || (D != 64 && D != 128) || max_blocks < 1 || ld_table < max_blocks ||
       (block != 16 && block != 32 && block != 64 && block != 128) || max_blocks * block > kIntMax ||
-      !aligned(k, 16) || !aligned(v, 16))
+      pages * heads * block > kIntMax || !aligned(k, 16) || !aligned(v, 16))
     return false;
   c->k = k;
   c->v = v;
@@ -412,14 +412,22 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
                   static_cast<unsigned>(B));
+  // the pool as rows of D bytes; a page's rows of one head are contiguous
+  const int64_t pool_rows = pages * heads * block;
+  const uint32_t box = static_cast<uint32_t>(block < kAttnChunk ? block : kAttnChunk);
+  const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  CUtensorMap tk, tv;
+  if (!host::tmap_u8(&tk, k_codes, D, pool_rows, D, static_cast<uint32_t>(D), box, sw) ||
+      !host::tmap_u8(&tv, v_codes, D, pool_rows, D, static_cast<uint32_t>(D), box, sw))
+    return B200Q_ERR_CUDA;
   int s;
   // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel)
   if (a.G * Tq <= 8) {
-    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
-                 : launch(kv8_attn8_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
+    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
+                 : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   } else {
-    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnWarps * 32, attn_smem_bytes<128>(), 1, st, a)
-                 : launch(kv8_attn_kernel<64>, grid, kAttnWarps * 32, attn_smem_bytes<64>(), 1, st, a);
+    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
+                 : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   }
   if (s != B200Q_OK || splits == 1) return s;
   const dim3 jgrid(static_cast<unsigned>(rows));
