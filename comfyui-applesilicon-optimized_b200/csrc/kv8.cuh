@@ -222,10 +222,13 @@ struct Kv8AttnArgs {
   float* part_ml; // [splits][B*Hq*Tq][2]: m (base 2), l
   const int32_t* lens;
   int B, Hq, G, Tq, causal, splits;
+  int cluster;  // the splits are one cluster (no partials in memory)
   float scale_log2;  // softmax scale * log2 e
 };
 
 constexpr int kAttnWarps = 4;
+constexpr int kAttnMaxSplits = 64;    // joined by the join kernel
+constexpr int kAttnMaxCluster = 16;
 constexpr int kAttnStages = 4;
 constexpr int kAttnThreads = (kAttnWarps + 1) * 32;  // and a producer warp
 constexpr int kAttnChunk = 64;                       // tokens per stage
@@ -254,7 +257,7 @@ template <int D>
 __device__ __forceinline__ void attn_ring_init(AttnRing<D>* ring) {
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAttnStages; ++i) {
-      mbar_init(&ring->full[i], 1);
+      mbar_init(&ring->full[i], 2);  // the copies and the meta words
       mbar_init(&ring->empty[i], kAttnWarps);
     }
     ring->abort = 0;
@@ -314,7 +317,9 @@ __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
 // The producer warp: chunks c0 .. c1 - 1 (64 tokens each) of (sequence b, head h).
 // Lane i looks up tile i % 4 of chunk i / 4 of the next eight chunks at once (page,
 // scales, their logarithm and inverse), then the chunks go out one by one: a box of
-// min(T, 64) rows per page.  Tiles at or past `tiles` are not fetched.
+// min(T, 64) rows per page.  Tiles at or past `tiles` are not fetched.  The first
+// stages' copies start before the scales are waited for: a stage is full after two
+// arrivals, the copies' and the one behind its meta words.
 template <int D>
 __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtensorMap* tk, const CUtensorMap* tv,
                                              AttnRing<D>* ring, int b, int h, int c0, int c1, int tiles) {
@@ -327,37 +332,39 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
   for (int base = c0; base < c1 && live; base += 8) {
     const int tile = base * 4 + lane, pos = tile << 4;
     int page = -1;
-    float4 meta = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (tile < tiles && (base + (lane >> 2)) < c1) {
-      page = kv8_page(c, b, pos >> c.log_t);
-      if (page >= 0) {
-        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
-        const float vs = __ldg(c.vs + at);
-        meta.x = __ldg(c.ks + at);
-        meta.y = vs == 0.0f ? 0.0f : log2f(vs);
-        meta.z = vs == 0.0f ? 1.0f : 1.0f / vs;
-        meta.w = vs == 0.0f ? 2.0f : 1.0f;
-      }
-    }
+    if (tile < tiles && (base + (lane >> 2)) < c1) page = kv8_page(c, b, pos >> c.log_t);
+    const int64_t at = static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h;
+    const float ks = __ldg(c.ks + at), vs = __ldg(c.vs + at);
     const bool lead = page >= 0 && (lane & (per_box - 1)) == 0;
     const unsigned leads = __ballot_sync(0xffffffffu, lead);
-    const int y = static_cast<int>((static_cast<int64_t>(page) * c.heads + h) * c.T + (pos & (c.T - 1)));
-    for (int i = 0; i < 8 && base + i < c1; ++i, ++n) {
-      const int s = n % kAttnStages;
-      if (n >= kAttnStages && !mbar_wait_warp(&ring->empty[s], ((n / kAttnStages) - 1) & 1, &ring->abort)) {
-        live = false;
-        break;
-      }
-      const bool mine = (lane >> 2) == i;
-      if (mine) ring->meta[s][lane & 3] = meta;
-      __syncwarp();
+    const int y = static_cast<int>(at * c.T) + (pos & (c.T - 1));
+    auto copy = [&](int i, int s) {
       if (lane == 0)
         mbar_arrive_expect_tx(&ring->full[s], 2 * D * box * __popc((leads >> (4 * i)) & 15u));
       __syncwarp();
-      if (mine && lead) {
+      if ((lane >> 2) == i && lead) {
         tma_load_2d(tk, &ring->full[s], ring->k[s] + (lane & 3) * 16 * D, 0, y);
         tma_load_2d(tv, &ring->full[s], ring->v[s] + (lane & 3) * 16 * D, 0, y);
       }
+    };
+    const int many = min(8, c1 - base);
+    if (n == 0)
+      for (int i = 0; i < min(many, kAttnStages); ++i) copy(i, i);
+    float4 meta = make_float4(ks, 0.0f, 1.0f, 2.0f);
+    if (vs != 0.0f) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
+    if (page < 0) meta.w = 0.0f;
+    for (int i = 0; i < many; ++i, ++n) {
+      const int s = n % kAttnStages;
+      if (n >= kAttnStages) {
+        if (!mbar_wait_warp(&ring->empty[s], ((n / kAttnStages) - 1) & 1, &ring->abort)) {
+          live = false;
+          break;
+        }
+        copy(i, s);
+      }
+      if ((lane >> 2) == i) ring->meta[s][lane & 3] = meta;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->full[s]);
     }
   }
   if (!live && lane == 0) {  // gave up: let the copies in flight land before the CTA ends
@@ -365,11 +372,9 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
       mbar_wait_drain(&ring->full[i % kAttnStages], (i / kAttnStages) & 1);
   }
 }
-// This lane's K and V words of a 16-token tile: K tokens g and g + 8, quarter t; V
-// tokens 2t, 2t+1, 2t+8, 2t+9, eighth g.
+// This lane's K words of a 16-token tile: tokens g and g + 8, quarter t.
 template <int D>
-__device__ __forceinline__ void attn_read(const uint8_t* k, const uint8_t* v_, int g, int t,
-                                          uint32_t (&kw)[2][D / 16], uint32_t (&vw)[4][D / 32]) {
+__device__ __forceinline__ void attn_read_k(const uint8_t* k, int g, int t, uint32_t (&kw)[2][D / 16]) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -378,39 +383,102 @@ __device__ __forceinline__ void attn_read(const uint8_t* k, const uint8_t* v_, i
       kw[i][4 * j] = v.x; kw[i][4 * j + 1] = v.y; kw[i][4 * j + 2] = v.z; kw[i][4 * j + 3] = v.w;
     }
   }
+}
+// Its V words: tokens 2t, 2t+1, 2t+8, 2t+9, eighth g.
+template <int D>
+__device__ __forceinline__ void attn_read_v(const uint8_t* vp, int g, int t, uint32_t (&vw)[4][D / 32]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 2 * t + (i & 1) + 8 * (i >> 1);
     if constexpr (D == 128) {
-      const uint4 v = *reinterpret_cast<const uint4*>(v_ + attn_at<D>(row, g));
+      const uint4 v = *reinterpret_cast<const uint4*>(vp + attn_at<D>(row, g));
       vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
     } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(v_ + attn_at<D>(row, g >> 1) + (g & 1) * 8);
+      const uint2 v = *reinterpret_cast<const uint2*>(vp + attn_at<D>(row, g >> 1) + (g & 1) * 8);
       vw[i][0] = v.x; vw[i][1] = v.y;
     }
   }
 }
-// Stores 4 values (d .. d+3) of packed row r, or hands them over to the join.
-template <int D>
-__device__ __forceinline__ void attn_finish(const Kv8AttnArgs& a, int b, int h, int split, int r, int d,
-                                            float4 x, float m, float l) {
-  const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
-  const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
-  if (a.splits > 1) {
-    const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
-    *reinterpret_cast<float4*>(a.part_o + at * D + d) = x;
-    if (d == 0) {
-      a.part_ml[at * 2] = m;
-      a.part_ml[at * 2 + 1] = l;
-    }
-    return;
+
+// Where the warps leave their rows: R rows of D values per warp in the ring's
+// memory (its last stage has been read).  Row stride and the skew by d / 16 (D =
+// 64: d / 8) spread a warp's writes, rows 2t x d = (D / 8) g, over the banks.
+template <int D, int R>
+struct AttnOut {
+  static constexpr int kStride = D + 20;
+  float o[kAttnWarps][R][kStride];
+  static __device__ __forceinline__ int at(int d) { return d + d / (D / 8); }
+};
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+  float f;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return f;
+}
+// Joins the warps, then the cluster's CTAs, in order; stores the rows or hands the
+// CTA's partial to the join kernel.  ml: (m, l) of each warp and row; each warp's o
+// is already scaled to the CTA's maximum.  Called by all threads, rows r0 .. of the
+// `live` ones present.
+template <int D, int R>
+__device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, AttnOut<D, R>* buf,
+                                              const float (&ml)[kAttnWarps][R][2], float (&fin)[R][2], int b,
+                                              int h, int split, int r0, int live) {
+  __syncthreads();
+  if (threadIdx.x < R) {
+    const int r = threadIdx.x;
+    float m = ml[0][r][0], l = 0.0f;
+#pragma unroll
+    for (int w = 1; w < kAttnWarps; ++w) m = fmaxf(m, ml[w][r][0]);
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) l += ml[w][r][1] * safe_ex2_diff(ml[w][r][0], m);
+    fin[r][0] = m;
+    fin[r][1] = l;
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + d;
-  *reinterpret_cast<uint2*>(dst) =
-      a.q_f16 ? make_uint2(pack_f16x2(x.x * inv, x.y * inv), pack_f16x2(x.z * inv, x.w * inv))
-              : make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
-  if (d == 0) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  const int ranks = a.cluster ? a.splits : 1;
+  const int rank = a.cluster ? split : 0;
+  if (a.cluster) {
+    for (int e = threadIdx.x; e < live * D; e += kAttnThreads) {
+      const int r = e / D, d = AttnOut<D, R>::at(e - r * D);
+      buf->o[0][r][d] += (buf->o[1][r][d] + buf->o[2][r][d]) + buf->o[3][r][d];
+    }
+    __syncwarp();
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  for (int e = threadIdx.x + kAttnThreads * rank; e < live * D; e += kAttnThreads * ranks) {
+    const int r = e / D, d = e - r * D, ds = AttnOut<D, R>::at(d);
+    const int row = r0 + r, ti = row / a.G, hi = h * a.G + (row - ti * a.G);
+    const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
+    float m, l, x;
+    if (a.cluster) {
+      m = -INFINITY;
+      for (int k = 0; k < ranks; ++k) m = fmaxf(m, ld_cluster(&fin[r][0], k));
+      l = x = 0.0f;
+#pragma unroll 4
+      for (int k = 0; k < ranks; ++k) {
+        const float f = safe_ex2_diff(ld_cluster(&fin[r][0], k), m);
+        l = fmaf(ld_cluster(&fin[r][1], k), f, l);
+        x = fmaf(ld_cluster(&buf->o[0][r][ds], k), f, x);
+      }
+    } else {
+      m = fin[r][0];
+      l = fin[r][1];
+      x = (buf->o[0][r][ds] + buf->o[1][r][ds]) + (buf->o[2][r][ds] + buf->o[3][r][ds]);
+      if (a.splits > 1) {
+        const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
+        a.part_o[at * D + d] = x;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+        continue;
+      }
+    }
+    x = l == 0.0f ? 0.0f : x / l;
+    const int64_t at = b * a.ob + hi * a.oh + ti * a.ot + d;
+    if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(x);
+    if (d == 0) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+  __syncwarp();
+  if (a.cluster) cluster_sync();  // the other CTAs may still be reading this one's rows
 }
 // Positions that token ti of Tq sees.
 __device__ __forceinline__ int attn_limit(const Kv8AttnArgs& a, int len, int ti) {
@@ -426,7 +494,7 @@ __global__ void __launch_bounds__(kAttnThreads)
   constexpr int VW = D / 32;   // words per lane and V token (D / 8 bytes)
   constexpr int NV = D / 8;    // n8 tiles of the output
   __shared__ float sm_ml[kAttnWarps][16][2];
-  __shared__ float sm_o[16][D + 4];
+  __shared__ float sm_fin[16][2];
   AttnRing<D>* ring = attn_ring<D>();
   attn_ring_init<D>(ring);
   griddep_wait();
@@ -503,11 +571,13 @@ __global__ void __launch_bounds__(kAttnThreads)
     const int s_ = n % kAttnStages;
     if (!mbar_wait_warp(&ring->full[s_], (n / kAttnStages) & 1, &ring->abort)) break;
     const float4 meta = ring->meta[s_][warp];
+    if (meta.w == 0.0f) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->empty[s_]);
+      continue;
+    }
     uint32_t kw[2][KW], vw[4][VW];
-    attn_read<D>(ring->k[s_] + warp * 16 * D, ring->v[s_] + warp * 16 * D, g, t, kw, vw);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ring->empty[s_]);
-    if (meta.w == 0.0f) continue;
+    attn_read_k<D>(ring->k[s_] + warp * 16 * D, g, t, kw);
     const int pos = ((c0 + n) * 4 + warp) << 4;
     const bool zero_v = meta.w == 2.0f;
     const float lv = meta.y, iv = meta.z;
@@ -567,6 +637,9 @@ __global__ void __launch_bounds__(kAttnThreads)
         o[i][2] *= corr[1]; o[i][3] *= corr[1];
       }
     }
+    attn_read_v<D>(ring->v[s_] + warp * 16 * D, g, t, vw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ring->empty[s_]);
     // ---- P V: tiles 4w .. 4w+3 come from word w of the four tokens
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
@@ -592,47 +665,23 @@ __global__ void __launch_bounds__(kAttnThreads)
     }
   }
   __syncthreads();
-  float mt[2], lt[2], f[2];
+  AttnOut<D, 16>* buf = reinterpret_cast<AttnOut<D, 16>*>(ring->k);
+  static_assert(sizeof(AttnOut<D, 16>) <= sizeof(ring->k) + sizeof(ring->v), "");
+  if (warp < kAttnWarps) {
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    mt[r] = -INFINITY;
-    for (int w = 0; w < kAttnWarps; ++w) {
-      const float x = sm_ml[w][g + 8 * r][0];
-      mt[r] = fmaxf(mt[r], x);
-    }
-    lt[r] = 0.0f;
-    for (int w = 0; w < kAttnWarps; ++w)
-      lt[r] += sm_ml[w][g + 8 * r][1] * safe_ex2_diff(sm_ml[w][g + 8 * r][0], mt[r]);
-    f[r] = safe_ex2_diff(m[r], mt[r]);
-  }
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (warp == w) {
+    for (int r = 0; r < 2; ++r) {
+      float mt = sm_ml[0][g + 8 * r][0];
+#pragma unroll
+      for (int w = 1; w < kAttnWarps; ++w) mt = fmaxf(mt, sm_ml[w][g + 8 * r][0]);
+      const float f = safe_ex2_diff(m[r], mt);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // tile i, column g' holds d = (D / 8) g' + i; this lane's columns are 2t, 2t + 1
-          float* p = &sm_o[g + 8 * (j >> 1)][(2 * t + (j & 1)) * (D / 8) + i];
-          const float x = o[i][j] * f[j >> 1];
-          *p = w == 0 ? x : *p + x;
-        }
+        for (int j = 0; j < 2; ++j)  // tile i, column 2t + j is d = (D / 8) (2t + j) + i
+          buf->o[warp][g + 8 * r][AttnOut<D, 16>::at((2 * t + j) * (D / 8) + i)] = o[i][2 * r + j] * f;
     }
-    __syncthreads();
   }
-  __shared__ float sm_fin[16][2];
-  if (warp == 0 && t == 0)
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      sm_fin[g + 8 * r][0] = mt[r];
-      sm_fin[g + 8 * r][1] = lt[r];
-    }
-  __syncthreads();
-  for (int e = tid; e < 16 * (D / 4); e += kAttnThreads) {
-    const int row = e / (D / 4), d = (e - row * (D / 4)) * 4, r = r0 + row;
-    if (r >= rows) continue;
-    attn_finish<D>(a, b, h, split, r, d, *reinterpret_cast<const float4*>(&sm_o[row][d]), sm_fin[row][0],
-                   sm_fin[row][1]);
-  }
+  attn_epilogue<D, 16>(a, buf, sm_ml, sm_fin, b, h, split, r0, min(16, rows - r0));
 }
 
 // ---- up to 8 rows per key/value head (one token of up to 8 grouped heads)
@@ -693,7 +742,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   constexpr int VW = D / 32;   // words per lane and V token
   constexpr int NM = D / 16;   // m16 tiles of the output
   __shared__ float sm_ml[kAttnWarps][8][2];
-  __shared__ float sm_o[8][D + 4];
+  __shared__ float sm_fin[8][2];
   AttnRing<D>* ring = attn_ring<D>();
   attn_ring_init<D>(ring);
   griddep_wait();
@@ -761,11 +810,13 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
     const int s_ = n % kAttnStages;
     if (!mbar_wait_warp(&ring->full[s_], (n / kAttnStages) & 1, &ring->abort)) break;
     const float4 meta = ring->meta[s_][warp];
+    if (meta.w == 0.0f) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->empty[s_]);
+      continue;
+    }
     uint32_t kw[2][D / 16], vw[4][VW];
-    attn_read<D>(ring->k[s_] + warp * 16 * D, ring->v[s_] + warp * 16 * D, g, t, kw, vw);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&ring->empty[s_]);
-    if (meta.w == 0.0f) continue;
+    attn_read_k<D>(ring->k[s_] + warp * 16 * D, g, t, kw);
     const bool zero_v = meta.w == 2.0f;
     const float lv = meta.y, iv = meta.z, ksc = meta.x * sc;
     float s[4];
@@ -816,6 +867,9 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
       p[i] = s[i] == -INFINITY ? 0.0f : ex2f(s[i] - m);
     l = fmaf((p[0] + p[1]) + (p[2] + p[3]), iv, l);
     const uint32_t pb0 = zero_v ? 0u : pack_f16x2(p[0], p[1]), pb1 = zero_v ? 0u : pack_f16x2(p[2], p[3]);
+    attn_read_v<D>(ring->v[s_] + warp * 16 * D, g, t, vw);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ring->empty[s_]);
 #pragma unroll
     for (int w = 0; w < VW; ++w) {
       const uint32_t ta = vw[0][w] ^ 0x80808080u, tb = vw[1][w] ^ 0x80808080u;
@@ -837,42 +891,26 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
     sm_ml[warp][g][1] = l;
   }
   __syncthreads();
-  auto top_of = [&](int r) {
-    float x = sm_ml[0][r][0];
+  AttnOut<D, 8>* buf = reinterpret_cast<AttnOut<D, 8>*>(ring->k);
+  if (warp < kAttnWarps) {
 #pragma unroll
-    for (int w = 1; w < kAttnWarps; ++w) x = fmaxf(x, sm_ml[w][r][0]);
-    return x;
-  };
-  const int wi = min(warp, kAttnWarps - 1);
-  const float f0 = safe_ex2_diff(sm_ml[wi][2 * t][0], top_of(2 * t));
-  const float f1 = safe_ex2_diff(sm_ml[wi][2 * t + 1][0], top_of(2 * t + 1));
-  for (int w = 0; w < kAttnWarps; ++w) {
-    if (warp == w) {
+    for (int j = 0; j < 2; ++j) {
+      float mt = sm_ml[0][2 * t + j][0];
+#pragma unroll
+      for (int w = 1; w < kAttnWarps; ++w) mt = fmaxf(mt, sm_ml[w][2 * t + j][0]);
+      const float f = safe_ex2_diff(sm_ml[warp][2 * t + j][0], mt);
 #pragma unroll
       for (int i = 0; i < NM; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // tile i: this lane's rows g and g + 8 are d = (D / 8) g + 2 i and + 1
-          float* q = &sm_o[2 * t + (j & 1)][g * (D / 8) + 2 * i + (j >> 1)];
-          const float x = o[i][j] * ((j & 1) ? f1 : f0);
-          *q = w == 0 ? x : *q + x;
-        }
+        for (int r = 0; r < 2; ++r)  // tile i: this lane's rows g and g + 8 are d = (D / 8) g + 2 i and + 1
+          buf->o[warp][2 * t + j][AttnOut<D, 8>::at(g * (D / 8) + 2 * i + r)] = o[i][2 * r + j] * f;
     }
-    __syncthreads();
   }
-  for (int e = tid; e < rows * (D / 4); e += kAttnThreads) {
-    const int r = e / (D / 4), d = (e - r * (D / 4)) * 4;
-    const float mt = top_of(r);
-    float lt = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kAttnWarps; ++w) lt += sm_ml[w][r][1] * safe_ex2_diff(sm_ml[w][r][0], mt);
-    attn_finish<D>(a, b, h, split, r, d, *reinterpret_cast<const float4*>(&sm_o[r][d]), mt, lt);
-  }
+  attn_epilogue<D, 8>(a, buf, sm_ml, sm_fin, b, h, split, 0, rows);
 }
 
 // Joins the splits of each row in split order: one CTA of D threads per row, a
 // thread per value; the splits' loads are independent of one another.
-constexpr int kAttnMaxSplits = 64;
 template <int D>
 __global__ void __launch_bounds__(D) kv8_attn_join_kernel(const Kv8AttnArgs a) {
   __shared__ float ml[kAttnMaxSplits][2];
