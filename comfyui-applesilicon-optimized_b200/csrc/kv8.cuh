@@ -222,24 +222,23 @@ struct Kv8AttnArgs {
   float* part_ml; // [splits][B*Hq*Tq][2]: m (base 2), l
   const int32_t* lens;
   int B, Hq, G, Tq, causal, splits;
-  int cluster;  // the splits are one cluster (no partials in memory)
   float scale_log2;  // softmax scale * log2 e
 };
 
-constexpr int kAttnWarps = 4;
+constexpr int kAttnBox = 64;          // rows of a TMA box at most
 constexpr int kAttnMaxSplits = 64;    // joined by the join kernel
-constexpr int kAttnMaxCluster = 16;
 constexpr int kAttnStages = 4;
+
+constexpr int kAttnWarps = 4;                        // consumer warps
 constexpr int kAttnThreads = (kAttnWarps + 1) * 32;  // and a producer warp
-constexpr int kAttnChunk = 64;                       // tokens per stage
 
 // The CTA's ring: stages of 64 tokens of K and V, brought by TMA with the row
 // swizzle; 16-token tile w of a stage belongs to consumer warp w.  meta: per tile
 // {ks, log2 vs, 1 / vs, state}, state 0 = skip (bad page), 1 = ok, 2 = vs is 0.
 template <int D>
 struct AttnRing {
-  uint8_t k[kAttnStages][kAttnChunk * D];
-  uint8_t v[kAttnStages][kAttnChunk * D];
+  uint8_t k[kAttnStages][16 * kAttnWarps * D];
+  uint8_t v[kAttnStages][16 * kAttnWarps * D];
   float4 meta[kAttnStages][kAttnWarps];
   uint64_t full[kAttnStages], empty[kAttnStages];
   int abort;
@@ -254,8 +253,10 @@ __device__ __forceinline__ AttnRing<D>* attn_ring() {
   return reinterpret_cast<AttnRing<D>*>((reinterpret_cast<uintptr_t>(attn_smem) + 1023) & ~uintptr_t(1023));
 }
 template <int D>
-__device__ __forceinline__ void attn_ring_init(AttnRing<D>* ring) {
+__device__ __forceinline__ void attn_ring_init(AttnRing<D>* ring, const CUtensorMap* tk, const CUtensorMap* tv) {
   if (threadIdx.x == 0) {
+    tma_prefetch_desc(tk);
+    tma_prefetch_desc(tv);
     for (int i = 0; i < kAttnStages; ++i) {
       mbar_init(&ring->full[i], 2);  // the copies and the meta words
       mbar_init(&ring->empty[i], kAttnWarps);
@@ -274,7 +275,7 @@ __device__ __forceinline__ int attn_at(int row, int ch) {
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -325,14 +326,14 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
                                              AttnRing<D>* ring, int b, int h, int c0, int c1, int tiles) {
   const Kv8Cache& c = a.c;
   const int lane = threadIdx.x & 31;
-  const int box = c.T < kAttnChunk ? c.T : kAttnChunk;
+  const int box = c.T < kAttnBox ? c.T : kAttnBox;
   const int per_box = box >> 4;  // tiles
   int n = 0;                     // chunks issued
   bool live = true;
-  for (int base = c0; base < c1 && live; base += 8) {
-    const int tile = base * 4 + lane, pos = tile << 4;
+  for (int base = c0; base < c1 && live; base += 32 / kAttnWarps) {
+    const int tile = base * kAttnWarps + lane, pos = tile << 4;
     int page = -1;
-    if (tile < tiles && (base + (lane >> 2)) < c1) page = kv8_page(c, b, pos >> c.log_t);
+    if (tile < tiles && (base + (lane / kAttnWarps)) < c1) page = kv8_page(c, b, pos >> c.log_t);
     const int64_t at = static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h;
     const float ks = __ldg(c.ks + at), vs = __ldg(c.vs + at);
     const bool lead = page >= 0 && (lane & (per_box - 1)) == 0;
@@ -340,14 +341,14 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     const int y = static_cast<int>(at * c.T) + (pos & (c.T - 1));
     auto copy = [&](int i, int s) {
       if (lane == 0)
-        mbar_arrive_expect_tx(&ring->full[s], 2 * D * box * __popc((leads >> (4 * i)) & 15u));
+        mbar_arrive_expect_tx(&ring->full[s], 2 * D * box * __popc((leads >> (kAttnWarps * i)) & ((1u << kAttnWarps) - 1u)));
       __syncwarp();
-      if ((lane >> 2) == i && lead) {
-        tma_load_2d(tk, &ring->full[s], ring->k[s] + (lane & 3) * 16 * D, 0, y);
-        tma_load_2d(tv, &ring->full[s], ring->v[s] + (lane & 3) * 16 * D, 0, y);
+      if ((lane / kAttnWarps) == i && lead) {
+        tma_load_2d(tk, &ring->full[s], ring->k[s] + (lane % kAttnWarps) * 16 * D, 0, y);
+        tma_load_2d(tv, &ring->full[s], ring->v[s] + (lane % kAttnWarps) * 16 * D, 0, y);
       }
     };
-    const int many = min(8, c1 - base);
+    const int many = min(32 / kAttnWarps, c1 - base);
     if (n == 0)
       for (int i = 0; i < min(many, kAttnStages); ++i) copy(i, i);
     float4 meta = make_float4(ks, 0.0f, 1.0f, 2.0f);
@@ -362,7 +363,7 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
         }
         copy(i, s);
       }
-      if ((lane >> 2) == i) ring->meta[s][lane & 3] = meta;
+      if ((lane / kAttnWarps) == i) ring->meta[s][lane % kAttnWarps] = meta;
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->full[s]);
     }
@@ -409,17 +410,11 @@ struct AttnOut {
   float o[kAttnWarps][R][kStride];
   static __device__ __forceinline__ int at(int d) { return d + d / (D / 8); }
 };
-__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
-  float f;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
-  return f;
-}
-// Joins the warps, then the cluster's CTAs, in order; stores the rows or hands the
-// CTA's partial to the join kernel.  ml: (m, l) of each warp and row; each warp's o
-// is already scaled to the CTA's maximum.  Called by all threads, rows r0 .. of the
-// `live` ones present.
+// Joins the warps in order and stores the rows, or hands the CTA's partial to the
+// join kernel.  ml: (m, l) of each warp and row; each warp's o is already scaled to
+// the CTA's maximum.  Called by all threads, for rows r0 .. r0 + live - 1.
 template <int D, int R>
-__device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, AttnOut<D, R>* buf,
+__device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, const AttnOut<D, R>* buf,
                                               const float (&ml)[kAttnWarps][R][2], float (&fin)[R][2], int b,
                                               int h, int split, int r0, int live) {
   __syncthreads();
@@ -433,43 +428,20 @@ __device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, AttnOut<D, R
     fin[r][0] = m;
     fin[r][1] = l;
   }
-  const int ranks = a.cluster ? a.splits : 1;
-  const int rank = a.cluster ? split : 0;
-  if (a.cluster) {
-    for (int e = threadIdx.x; e < live * D; e += kAttnThreads) {
-      const int r = e / D, d = AttnOut<D, R>::at(e - r * D);
-      buf->o[0][r][d] += (buf->o[1][r][d] + buf->o[2][r][d]) + buf->o[3][r][d];
-    }
-    __syncwarp();
-    cluster_sync();
-  } else {
-    __syncthreads();
-  }
-  for (int e = threadIdx.x + kAttnThreads * rank; e < live * D; e += kAttnThreads * ranks) {
+  __syncthreads();
+  for (int e = threadIdx.x; e < live * D; e += kAttnThreads) {
     const int r = e / D, d = e - r * D, ds = AttnOut<D, R>::at(d);
     const int row = r0 + r, ti = row / a.G, hi = h * a.G + (row - ti * a.G);
     const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
-    float m, l, x;
-    if (a.cluster) {
-      m = -INFINITY;
-      for (int k = 0; k < ranks; ++k) m = fmaxf(m, ld_cluster(&fin[r][0], k));
-      l = x = 0.0f;
-#pragma unroll 4
-      for (int k = 0; k < ranks; ++k) {
-        const float f = safe_ex2_diff(ld_cluster(&fin[r][0], k), m);
-        l = fmaf(ld_cluster(&fin[r][1], k), f, l);
-        x = fmaf(ld_cluster(&buf->o[0][r][ds], k), f, x);
-      }
-    } else {
-      m = fin[r][0];
-      l = fin[r][1];
-      x = (buf->o[0][r][ds] + buf->o[1][r][ds]) + (buf->o[2][r][ds] + buf->o[3][r][ds]);
-      if (a.splits > 1) {
-        const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
-        a.part_o[at * D + d] = x;
-        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
-        continue;
-      }
+    const float m = fin[r][0], l = fin[r][1];
+    float x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAttnWarps; ++w) x += buf->o[w][r][ds];
+    if (a.splits > 1) {
+      const int64_t at = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
+      a.part_o[at * D + d] = x;
+      if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m, l);
+      continue;
     }
     x = l == 0.0f ? 0.0f : x / l;
     const int64_t at = b * a.ob + hi * a.oh + ti * a.ot + d;
@@ -477,8 +449,6 @@ __device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, AttnOut<D, R
     else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(x);
     if (d == 0) a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
-  __syncwarp();
-  if (a.cluster) cluster_sync();  // the other CTAs may still be reading this one's rows
 }
 // Positions that token ti of Tq sees.
 __device__ __forceinline__ int attn_limit(const Kv8AttnArgs& a, int len, int ti) {
@@ -496,7 +466,7 @@ __global__ void __launch_bounds__(kAttnThreads)
   __shared__ float sm_ml[kAttnWarps][16][2];
   __shared__ float sm_fin[16][2];
   AttnRing<D>* ring = attn_ring<D>();
-  attn_ring_init<D>(ring);
+  attn_ring_init<D>(ring, &tk, &tv);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -523,7 +493,7 @@ __global__ void __launch_bounds__(kAttnThreads)
   const int lim_max = a.causal ? min(max(len - a.Tq + last / a.G + 1, 0), len) : len;
   const int lim_min = a.causal ? min(max(len - a.Tq + r0 / a.G + 1, 0), len) : len;
   const int tiles = (lim_max + 15) >> 4;  // 16-token tiles to visit
-  const int chunks = (tiles + 3) >> 2;
+  const int chunks = (tiles + kAttnWarps - 1) / kAttnWarps;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
   const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
 
@@ -578,7 +548,7 @@ __global__ void __launch_bounds__(kAttnThreads)
     }
     uint32_t kw[2][KW], vw[4][VW];
     attn_read_k<D>(ring->k[s_] + warp * 16 * D, g, t, kw);
-    const int pos = ((c0 + n) * 4 + warp) << 4;
+    const int pos = ((c0 + n) * kAttnWarps + warp) << 4;
     const bool zero_v = meta.w == 2.0f;
     const float lv = meta.y, iv = meta.z;
     const float ksc[2] = {meta.x * sc[0], meta.x * sc[1]};
@@ -687,41 +657,43 @@ __global__ void __launch_bounds__(kAttnThreads)
 // ---- up to 8 rows per key/value head (one token of up to 8 grouped heads)
 //
 // q.K on the integer tensor path: q's row, scaled by a power of two 2^-E to
-// |v| < 128, is three int8 digits v = p0 + p1 / 128 + p2 / 128^2 (within 2^-22 of
+// |v| < 64, is three int8 digits v = p0 + p1 / 128 + p2 / 128^2 (within 2^-21 of
 // 2^E), and K's codes are the other operand as they are stored: no instruction
 // converts them.  Rows 0-7 of an m16n8k32 MMA hold p0 and rows 8-15 p1 of the 8
 // rows, a second MMA p2.  The int32 accumulators start at the bits of 1.5 * 2^23,
-// so a subtraction turns each sum (|sum| <= 128 * 127 * 128 < 2^22) into its fp32
+// so a subtraction turns each sum (|sum| <= 64 * 127 * 128 < 2^20) into its fp32
 // value exactly.
 //
 // P V is computed transposed, V^T (16 d x 16 tokens) as the MMA's rows and P as its
 // 8 columns: half the MMAs and accumulators of the 16-row form.
 __device__ __forceinline__ void mma_s8_start(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   const int z = 0x4B400000;
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(z));
 }
 __device__ __forceinline__ void mma_s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Three int8 digits of v, |v| < 128.
-__device__ __forceinline__ void digits3(float v, int& p0, int& p1, int& p2) {
-  const float a = fminf(fmaxf(rintf(v), -127.0f), 127.0f);
-  const float r = (v - a) * 128.0f;
-  const float c = fminf(fmaxf(rintf(r), -127.0f), 127.0f);
-  const float e = fminf(fmaxf(rintf((r - c) * 128.0f), -127.0f), 127.0f);
-  p0 = static_cast<int>(a);
-  p1 = static_cast<int>(c);
-  p2 = static_cast<int>(e);
+// Three int8 digits of v, |v| < 64, in the low bytes: adding 1.5 * 2^23 leaves the
+// nearest integer in the mantissa's low bits.
+__device__ __forceinline__ void digits3(float v, uint32_t& p0, uint32_t& p1, uint32_t& p2) {
+  const float m = 12582912.0f;
+  const float a = v + m;
+  const float r = (v - (a - m)) * 128.0f;
+  const float c = r + m;
+  const float e = (r - (c - m)) * 128.0f + m;
+  p0 = __float_as_uint(a);
+  p1 = __float_as_uint(c);
+  p2 = __float_as_uint(e);
 }
-// 2^E above the largest |value| of 16-bit bits `top`, as (2^-E * 128, 2^E / 128);
+// 2^E above the largest |value| of 16-bit bits `top`, as (2^-E * 64, 2^E / 64);
 // NaN for a row holding inf or NaN.
 __device__ __forceinline__ void digit_scale(uint32_t top, int f16, float* down, float* up) {
   const uint16_t tb = static_cast<uint16_t>(top);
@@ -730,8 +702,12 @@ __device__ __forceinline__ void digit_scale(uint32_t top, int f16, float* down, 
   int ex = static_cast<int>(__float_as_uint(m) >> 23);  // biased: m < 2^(ex - 126)
   const bool bad = ex == 255;
   ex = min(max(ex, 8), 254);
-  *down = __uint_as_float(static_cast<uint32_t>(126 - ex + 127 + 7) << 23);
-  *up = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(ex - 126 + 127 - 7) << 23);
+  *down = __uint_as_float(static_cast<uint32_t>(259 - ex) << 23);
+  *up = bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(static_cast<uint32_t>(ex - 5) << 23);
+}
+// The low bytes of four words as one.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 template <int D>
@@ -744,7 +720,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   __shared__ float sm_ml[kAttnWarps][8][2];
   __shared__ float sm_fin[8][2];
   AttnRing<D>* ring = attn_ring<D>();
-  attn_ring_init<D>(ring);
+  attn_ring_init<D>(ring, &tk, &tv);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -754,48 +730,51 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   const int lim = attn_limit(a, len, min(g, rows - 1) / a.G);
   const int lim_max = attn_limit(a, len, (rows - 1) / a.G), lim_min = attn_limit(a, len, 0);
   const int tiles = (lim_max + 15) >> 4;
-  const int chunks = (tiles + 3) >> 2;
+  const int chunks = (tiles + kAttnWarps - 1) / kAttnWarps;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
   const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
   if (warp == kAttnWarps) attn_produce<D>(a, &tk, &tv, ring, b, h, c0, c1, tiles);
 
-  // ---- q digits of row g, quarter t
+  // ---- q digits of row g, quarter t: each warp makes its share of the words
+  __shared__ uint32_t sm_q[3][D / 16][32];
   uint32_t q01[KS][4], q2[KS][2];
   float sc = 0.0f;
   if (warp < kAttnWarps) {
     const int r = min(g, rows - 1), ti = r / a.G, hi = h * a.G + (r - ti * a.G);
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qb + hi * a.qh + ti * a.qt + t * (D / 4);
-    uint32_t raw[D / 8];
     uint32_t top = 0;
 #pragma unroll
     for (int j = 0; j < D / 32; ++j) {
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
-      raw[4 * j] = v.x; raw[4 * j + 1] = v.y; raw[4 * j + 2] = v.z; raw[4 * j + 3] = v.w;
-    }
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < D / 8; ++j) top = max(top, max(raw[j] & 0x7FFFu, (raw[j] >> 16) & 0x7FFFu));
+      for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7FFFu, (u[i] >> 16) & 0x7FFFu));
+    }
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     float down, up;
     digit_scale(top, a.q_f16, &down, &up);
     sc = a.scale_log2 * up;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j) {  // 4 values: word j of the lane's K bytes
-      uint32_t w[3] = {0, 0, 0};
+    for (int j = warp; j < D / 16; j += kAttnWarps) {  // 4 values: word j of the lane's K bytes
+      const uint2 u2 = *reinterpret_cast<const uint2*>(src + 4 * j);
+      const uint32_t u[2] = {u2.x, u2.y};
+      uint32_t p[3][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint16_t e = static_cast<uint16_t>(raw[2 * j + (i >> 1)] >> (16 * (i & 1)));
+        const uint16_t e = static_cast<uint16_t>(u[i >> 1] >> (16 * (i & 1)));
         const float v = a.q_f16 ? __half2float(*reinterpret_cast<const __half*>(&e))
                                 : __uint_as_float(static_cast<uint32_t>(e) << 16);
-        int p0, p1, p2;
-        digits3(v * down, p0, p1, p2);
-        w[0] |= static_cast<uint32_t>(p0 & 255) << (8 * i);
-        w[1] |= static_cast<uint32_t>(p1 & 255) << (8 * i);
-        w[2] |= static_cast<uint32_t>(p2 & 255) << (8 * i);
+        digits3(v * down, p[0][i], p[1][i], p[2][i]);
       }
-      q01[j >> 1][2 * (j & 1)] = w[0];
-      q01[j >> 1][2 * (j & 1) + 1] = w[1];
-      q2[j >> 1][j & 1] = w[2];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) sm_q[i][j][lane] = low_bytes(p[i][0], p[i][1], p[i][2], p[i][3]);
+    }
+    named_bar_sync(1, 32 * kAttnWarps);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      q01[j >> 1][2 * (j & 1)] = sm_q[0][j][lane];
+      q01[j >> 1][2 * (j & 1) + 1] = sm_q[1][j][lane];
+      q2[j >> 1][j & 1] = sm_q[2][j][lane];
     }
   }
 
@@ -839,7 +818,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
         s[2 * i + j] = fmaf(fmaf(fmaf(f2, 0.0078125f, f1), 0.0078125f, f0), ksc, lv);
       }
     }
-    const int pos = ((c0 + n) * 4 + warp) << 4;
+    const int pos = ((c0 + n) * kAttnWarps + warp) << 4;
     if (pos + 16 > lim_min) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -909,37 +888,75 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   attn_epilogue<D, 8>(a, buf, sm_ml, sm_fin, b, h, split, 0, rows);
 }
 
-// Joins the splits of each row in split order: one CTA of D threads per row, a
-// thread per value; the splits' loads are independent of one another.
+// Joins up to 64 splits of a row: one CTA per row.  Every warp weighs all splits
+// (lane i has splits i and i + 32) and sums every kJoinWarps-th split's D values;
+// the warps' sums are added in order.  All loads are independent of one another.
+constexpr int kJoinWarps = 8;
 template <int D>
-__global__ void __launch_bounds__(D) kv8_attn_join_kernel(const Kv8AttnArgs a) {
-  __shared__ float ml[kAttnMaxSplits][2];
+__global__ void __launch_bounds__(kJoinWarps * 32) kv8_attn_join_kernel(const Kv8AttnArgs a) {
+  constexpr int VL = D / 32;  // values per lane
+  __shared__ float sums[kJoinWarps][D];
   griddep_wait();
   griddep_launch_dependents();
   const int64_t flat = blockIdx.x, rows = gridDim.x;
-  for (int i = threadIdx.x; i < a.splits; i += D) {
-    const float2 v = *reinterpret_cast<const float2*>(a.part_ml + (i * rows + flat) * 2);
-    ml[i][0] = v.x;
-    ml[i][1] = v.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (lane + 32 * i < a.splits) {
+      const float2 v = *reinterpret_cast<const float2*>(a.part_ml + ((lane + 32 * i) * rows + flat) * 2);
+      m[i] = v.x;
+      l[i] = v.y;
+    }
+  float x[kAttnMaxSplits / kJoinWarps][VL];
+#pragma unroll
+  for (int k = 0; k < kAttnMaxSplits / kJoinWarps; ++k) {
+    const int s = warp + kJoinWarps * k;
+    if (s < a.splits) {
+      const float* p = a.part_o + (s * rows + flat) * D + lane * VL;
+      if constexpr (VL == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        x[k][0] = v.x; x[k][1] = v.y;
+      }
+    }
   }
+  float top = fmaxf(m[0], m[1]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float f[2] = {safe_ex2_diff(m[0], top), safe_ex2_diff(m[1], top)};
+  float lt = l[0] * f[0] + l[1] * f[1];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) lt += __shfl_xor_sync(0xffffffffu, lt, o);
+  float acc[VL];
+#pragma unroll
+  for (int i = 0; i < VL; ++i) acc[i] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kAttnMaxSplits / kJoinWarps; ++k) {
+    const int s = warp + kJoinWarps * k;
+    const float fs = __shfl_sync(0xffffffffu, k < 32 / kJoinWarps ? f[0] : f[1], s & 31);
+    if (s < a.splits) {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) acc[i] = fmaf(x[k][i], fs, acc[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VL; ++i) sums[warp][lane * VL + i] = acc[i];
   __syncthreads();
-  float mt = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) mt = fmaxf(mt, ml[s][0]);
-  const float* p = a.part_o + flat * D + threadIdx.x;
-  float lt = 0.0f, acc = 0.0f;
-#pragma unroll 8
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = safe_ex2_diff(ml[s][0], mt);
-    lt = fmaf(ml[s][1], f, lt);
-    acc = fmaf(p[s * rows * D], f, acc);
+  if (threadIdx.x < D) {
+    float o = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) o += sums[w][threadIdx.x];
+    o = lt == 0.0f ? 0.0f : o / lt;
+    const int ti = static_cast<int>(flat % a.Tq);
+    const int64_t bh = flat / a.Tq, b = bh / a.Hq, hi = bh - b * a.Hq;
+    const int64_t at = b * a.ob + hi * a.oh + ti * a.ot + threadIdx.x;
+    if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(o);
+    else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(o);
+    if (threadIdx.x == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (top + log2f(lt)) * 0.6931471805599453f;
   }
-  acc = lt == 0.0f ? 0.0f : acc / lt;
-  const int ti = static_cast<int>(flat % a.Tq);
-  const int64_t bh = flat / a.Tq, b = bh / a.Hq, hi = bh - b * a.Hq;
-  const int64_t at = b * a.ob + hi * a.oh + ti * a.ot + threadIdx.x;
-  if (a.q_f16) static_cast<__half*>(a.out)[at] = __float2half_rn(acc);
-  else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(acc);
-  if (threadIdx.x == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
 }
 
 }  // namespace b200q

@@ -41,12 +41,6 @@ int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, 
     cudaGetLastError();
     return B200Q_ERR_CUDA;
   }
-  // a cluster above 8 CTAs has to be asked for
-  if (cluster > 8 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
-    cudaGetLastError();
-    return B200Q_ERR_CUDA;
-  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(block));
@@ -182,28 +176,20 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
 
 // How many CTAs share a sequence's length: enough to give every SM two, and at
 // most 4096 tokens each so that ragged batches balance; at least 128 tokens each.
-// Up to 16 of them are one cluster and join over distributed shared memory; more
-// (few sequences and heads) leave partials for the join kernel.
-struct AttnPlan {
-  int splits;
-  bool cluster;
-};
-AttnPlan attn_plan(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
+// More than one leave fp32 partials for the join kernel.  (A cluster of up to 16
+// CTAs joining over distributed shared memory was no faster: 8 heads x 2048 tokens
+// 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
+int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t base = B * heads * cdiv(Hq / heads * Tq, 16);
   int64_t s = cdiv(int64_t(sms) * 2, base);
   if (s < cdiv(max_len, 4096)) s = cdiv(max_len, 4096);
   const int64_t most = cdiv(max_len, 128);
   if (s > most) s = most;
-  if (s <= 1) return {1, false};
-  if (s <= kAttnMaxCluster || base * kAttnMaxCluster * 10 >= int64_t(sms) * 8) {
-    int c = 2;
-    while (c < s && c < kAttnMaxCluster) c *= 2;
-    return {c, true};
-  }
-  return {static_cast<int>(s > kAttnMaxSplits ? kAttnMaxSplits : s), false};
+  if (s > kAttnMaxSplits) s = kAttnMaxSplits;
+  return s < 1 ? 1 : static_cast<int>(s);
 }
-size_t attn_work_bytes(const AttnPlan& p, int64_t rows, int64_t D) {
-  return p.splits > 1 && !p.cluster ? size_t(p.splits) * rows * (D + 2) * 4 : 0;
+size_t attn_work_bytes(int splits, int64_t rows, int64_t D) {
+  return splits > 1 ? size_t(splits) * rows * (D + 2) * 4 : 0;
 }
 bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
   return B >= 0 && B <= 65535 && heads >= 1 && Hq >= heads && Hq % heads == 0 && Tq >= 0 &&
@@ -388,7 +374,7 @@ size_t b200q_kv8_attention_workspace_size(int64_t B, int64_t Hq, int64_t heads, 
                                           int64_t D, int64_t max_len) {
   const int sms = host::device_sms();
   if (!sms || !attn_dims(B, Hq, heads, Tq) || B * Tq == 0) return 0;
-  return attn_work_bytes(attn_plan(sms, B, Hq, heads, Tq, max_len), B * Hq * Tq, D);
+  return attn_work_bytes(attn_splits(sms, B, Hq, heads, Tq, max_len), B * Hq * Tq, D);
 }
 
 int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t Tq,
@@ -412,8 +398,8 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   const int sms = host::device_sms();
   if (!sms) return B200Q_ERR_UNSUPPORTED;
   const int64_t rows = B * Hq * Tq;
-  const AttnPlan plan = attn_plan(sms, B, Hq, heads, Tq, max_len);
-  const size_t need = attn_work_bytes(plan, rows, D);
+  const int splits = attn_splits(sms, B, Hq, heads, Tq, max_len);
+  const size_t need = attn_work_bytes(splits, rows, D);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) return B200Q_ERR_WORKSPACE;
   a.q = q; a.q_f16 = dtype == B200Q_F16;
   a.qb = q_strides[0]; a.qh = q_strides[1]; a.qt = q_strides[2];
@@ -421,37 +407,36 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   a.ob = out_strides[0]; a.oh = out_strides[1]; a.ot = out_strides[2];
   a.lse = lse;
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o + (need ? size_t(plan.splits) * rows * D : 0);
+  a.part_ml = a.part_o + (need ? size_t(splits) * rows * D : 0);
   a.lens = lens;
   a.B = static_cast<int>(B); a.Hq = static_cast<int>(Hq); a.G = static_cast<int>(Hq / heads);
   a.Tq = static_cast<int>(Tq); a.causal = causal != 0;
-  a.splits = plan.splits; a.cluster = plan.cluster;
+  a.splits = splits;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(plan.splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
+  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
                   static_cast<unsigned>(B));
   // the pool as rows of D bytes; a page's rows of one head are contiguous
   const int64_t pool_rows = pages * heads * block;
-  const uint32_t box = static_cast<uint32_t>(block < kAttnChunk ? block : kAttnChunk);
+  const uint32_t box = static_cast<uint32_t>(block < kAttnBox ? block : kAttnBox);
   const CUtensorMapSwizzle sw = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap tk, tv;
   if (!host::tmap_u8(&tk, k_codes, D, pool_rows, D, static_cast<uint32_t>(D), box, sw) ||
       !host::tmap_u8(&tv, v_codes, D, pool_rows, D, static_cast<uint32_t>(D), box, sw))
     return B200Q_ERR_CUDA;
-  const int cl = plan.cluster ? plan.splits : 1;
   int s;
   // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel)
   if (a.G * Tq <= 8) {
-    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), cl, st, tk, tv, a)
-                 : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), cl, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
+                 : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   } else {
-    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), cl, st, tk, tv, a)
-                 : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), cl, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
+                 : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   }
   if (s != B200Q_OK || !need) return s;
   const dim3 jgrid(static_cast<unsigned>(rows));
-  return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, 128, 0, 1, st, a)
-                  : launch(kv8_attn_join_kernel<64>, jgrid, 64, 0, 1, st, a);
+  return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, kJoinWarps * 32, 0, 1, st, a)
+                  : launch(kv8_attn_join_kernel<64>, jgrid, kJoinWarps * 32, 0, 1, st, a);
 }
 
 }  // extern "C"
