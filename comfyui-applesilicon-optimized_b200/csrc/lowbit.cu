@@ -108,6 +108,43 @@ int launch_w4(const W4Args& a, const EpiArgs& ep, const W4Plan& p, int nt, cudaS
   }
 }
 
+// The integer kernel for few tokens, when x's digits fit beside the rings: at most
+// 24 digit columns, M * K up to about 20,000.
+struct WdPlan {
+  int smem, grid, threads;
+};
+bool wd_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WdPlan* p) {
+  if (M > 8 || M * K > 24 * 1024) return false;
+  const int nc = M <= 2 ? 1 : M <= 5 ? 2 : 3;
+  int teams = wd_teams(nc);
+  for (; teams > 0; --teams) {
+    p->smem = wd_layout(int(M), int(K), G, nc, teams).total;
+    if (p->smem <= 227 * 1024) break;
+  }
+  if (!teams) return false;
+  // no more teams than tiles per SM, and the fewest CTAs that need as few rounds
+  const int64_t tiles = cdiv(N, 16);
+  teams = static_cast<int>(cdiv(tiles, sms) < teams ? cdiv(tiles, sms) : teams);
+  const int64_t rounds = cdiv(tiles, int64_t(sms) * teams);
+  p->smem = wd_layout(int(M), int(K), G, nc, teams).total;
+  p->threads = teams * kW4Warps * 32;
+  p->grid = static_cast<int>(cdiv(tiles, rounds * teams));
+  return true;
+}
+template <typename T, int LW>
+int launch_digits_cols(const W4DigitArgs& a, const EpiArgs& ep, const WdPlan& p, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.grid));
+  if (a.M <= 2) return launch(w4_digit_kernel<T, LW, 1>, grid, p.threads, p.smem, 1, st, a, ep);
+  if (a.M <= 5) return launch(w4_digit_kernel<T, LW, 2>, grid, p.threads, p.smem, 1, st, a, ep);
+  return launch(w4_digit_kernel<T, LW, 3>, grid, p.threads, p.smem, 1, st, a, ep);
+}
+template <typename T>
+int launch_digits(const W4DigitArgs& a, int G, const EpiArgs& ep, const WdPlan& p, cudaStream_t st) {
+  if (G == 32) return launch_digits_cols<T, 1>(a, ep, p, st);
+  if (G == 64) return launch_digits_cols<T, 2>(a, ep, p, st);
+  return launch_digits_cols<T, 4>(a, ep, p, st);
+}
+
 struct W4Work {
   size_t w, x, row, col, total;  // byte offsets
 };
@@ -233,6 +270,24 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   ep.M = static_cast<int>(M);
   ep.N = static_cast<int>(N);
   const bool x_vec = aligned(x, 16) && ldx % 8 == 0;
+  WdPlan wd;
+  if (wd_plan(sms, M, N, K, int(group), &wd)) {
+    W4DigitArgs a{};
+    a.x = x;
+    a.ldx = ldx;
+    a.w = w;
+    a.ldw = ldw;
+    a.scales = scales;
+    a.scale_dtype = scale_dtype;
+    a.zeros = zeros;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.K = static_cast<int>(K);
+    a.x_vec = x_vec;
+    a.tiles = static_cast<int>(cdiv(N, 16));
+    return x_dtype == B200Q_F16 ? launch_digits<__half>(a, int(group), ep, wd, st)
+                                : launch_digits<__nv_bfloat16>(a, int(group), ep, wd, st);
+  }
   if (M <= kW4MaxSmallM) {
     W4Args a{};
     a.x = x;

@@ -23,6 +23,7 @@
 // bank conflicts.
 #pragma once
 
+#include "digits.cuh"
 #include "numerics.cuh"
 #include "ptx.cuh"
 
@@ -54,6 +55,7 @@ template <typename T>
 struct W4Num;
 template <>
 struct W4Num<__nv_bfloat16> {
+  static constexpr bool kF16 = false;
   static constexpr uint32_t kMagic = 0x43004300u;  // 128, 128
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
@@ -71,6 +73,7 @@ struct W4Num<__nv_bfloat16> {
 };
 template <>
 struct W4Num<__half> {
+  static constexpr bool kF16 = true;
   static constexpr uint32_t kMagic = 0x64006400u;  // 1024, 1024
   static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
@@ -274,6 +277,344 @@ __global__ void __launch_bounds__(kW4Warps * 32)
     if (n < a.N) store_out(ep, col, n, epi_scaled(v, 1.0f, 1.0f, xs_scale, ep, n));
   }
   if (a.splits > 1) cluster_sync();  // the other CTAs may still be reading this one's partials
+}
+
+// ---------------------------------------------------------------- few tokens, integer
+// One to a few tokens, whose time is the weight stream: the instructions per weight
+// are what has to be few, so the products run on the integer tensor path, where a
+// nibble is an operand after one AND.
+//
+// x is split, group by group, into three int8 digits: with 2^E above the group's
+// largest |x|, x 2^-E 64 = p0 + p1 / 128 + p2 / 128^2, within 2^-21 of 2^E.  Then
+//   sum_k x_k (c_k - z) = 2^E / 64 sum_p 128^-p (sum_k p_k c_k - z sum_k p_k)
+// with exact integer sums (|.| <= 128 * 15 * 64 < 2^17).  MMA m16n8k32: 16 weight
+// rows x the 3 M digit columns; a word's 8 codes are two operand registers, w &
+// 0x0F0F0F0F and (w >> 4) & 0x0F0F0F0F, with the digits staged in that order.  The
+// accumulators start at the bits of 1.5 * 2^23, so one subtraction gives the fp32
+// value.  A group holding inf or NaN gets a NaN scale.
+//
+// One CTA per SM makes the digits once for its teams of 8 warps; a team is persistent
+// over 16-row tiles and its warps split K.  Each warp streams its rows' bytes through
+// a ring of its own (cp.async, 128 bytes per row and stage, 16-byte chunks
+// XOR-swizzled by the row so that the fragment reads have no bank conflicts); the ring
+// runs on across tiles, so the loads of the next tile are in flight while one is
+// summed.  A stage's scales and zero points travel with it: loaded to registers when
+// its bytes are asked for, converted and put into the stage's slot one step later
+// (waiting for them at the start of each tile cost more than the tile).  A tile's sums
+// are double-buffered: one barrier per tile, and a different warp each time adds and
+// stores them while the others go on.
+constexpr int kWdStages = 3;
+// Most teams per CTA, by the digit columns' register need.
+constexpr int wd_teams(int nc) { return nc == 3 ? 2 : 3; }
+
+struct W4DigitArgs {
+  const void* x;
+  int64_t ldx;
+  const uint8_t* w;
+  int64_t ldw;
+  const void* scales;
+  int scale_dtype;
+  const uint8_t* zeros;
+  int M, N, K;
+  int x_vec;
+  int tiles;  // ceil(N / 16)
+};
+
+// A scale as its raw bits, and their value.
+__device__ __forceinline__ uint32_t load_scale_bits(const void* p, int dtype, int64_t i) {
+  return dtype == kBiasF32 ? __ldg(static_cast<const uint32_t*>(p) + i)
+                           : static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(p) + i));
+}
+__device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
+  if (dtype == kBiasF32) return __uint_as_float(bits);
+  if (dtype == kBiasBF16) return __uint_as_float(bits << 16);
+  const uint16_t h = static_cast<uint16_t>(bits);
+  return __half2float(*reinterpret_cast<const __half*>(&h));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ int rev3(int r) { return ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1); }
+
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Shared memory: rings, digits [3M][pitch], {2^E / (64 * 128^p), digit sum}
+// [groups][8 NC], {scale, -zero} [warp][stage][groups of a stage][16], warp sums.
+__host__ __device__ __forceinline__ int wd_pitch(int K) { return K + ((K & 127) == 64 ? 0 : (64 + 128 - (K & 127)) & 127); }
+struct WdLayout {
+  int digits, table, sz, red, total;  // byte offsets
+};
+__host__ __device__ __forceinline__ WdLayout wd_layout(int M, int K, int G, int nc, int teams) {
+  WdLayout l;
+  const int KG = K / G;
+  l.digits = teams * kW4Warps * kWdStages * 2048;
+  l.table = l.digits + 3 * M * wd_pitch(K);
+  l.sz = l.table + KG * 8 * nc * 8;
+  l.red = l.sz + teams * kW4Warps * kWdStages * (256 / G) * 16 * 8;
+  l.total = l.red + 2 * teams * kW4Warps * 16 * 8 * nc * 4;
+  return l;
+}
+
+template <typename T, int LW, int NC>
+__global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4DigitArgs a, const EpiArgs ep) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int G = 32 * LW;
+  constexpr int GS = 8 / LW;           // groups per stage (128 bytes of a row)
+  constexpr int LG = LW == 1 ? 4 : 8;  // lanes per group while making digits
+  constexpr int EL = G / LG;           // values per lane there
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int KG = a.K / G;
+  const int teams = blockDim.x / (kW4Warps * 32);
+  const WdLayout L = wd_layout(a.M, a.K, G, NC, teams);
+  const int pitch = wd_pitch(a.K);
+  const int team = warp / kW4Warps, tw = warp % kW4Warps;
+  const int g0 = static_cast<int>(int64_t(KG) * tw / kW4Warps);
+  const int ng = static_cast<int>(int64_t(KG) * (tw + 1) / kW4Warps) - g0;
+  const int spt = (ng + GS - 1) / GS;  // stages per tile
+  uint8_t* ring = smem + warp * (kWdStages * 2048);
+  const uint32_t ring_u = smem_u32(ring);
+  float2* sz = reinterpret_cast<float2*>(smem + L.sz) + warp * (kWdStages * GS * 16);
+  float* red = reinterpret_cast<float*>(smem + L.red) + team * (2 * kW4Warps * 16 * 8 * NC);
+  const int tile0 = blockIdx.x * teams + team, tile_step = gridDim.x * teams;
+
+  griddep_wait();
+  griddep_launch_dependents();
+
+  // ---- the ring: lane copies chunk lane % 8 of rows lane / 8 + 4 j, and loads entries
+  // lane + 32 k = (group e / 16, row e % 16) of the stage's scales
+  constexpr int SL = GS / 2;
+  int it_tile = tile0, it_stage = 0, it_slot = 0;
+  const int cp_row = lane >> 3, cp_ch = lane & 7;
+  uint32_t s_next[SL], z_next[SL];
+#pragma unroll
+  for (int k = 0; k < SL; ++k) s_next[k] = z_next[k] = 0;
+  const uint8_t* src[4];   // this lane's rows of the tile being fetched
+  int64_t s_at = 0;
+  auto aim = [&]() {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      src[j] = a.w + static_cast<int64_t>(min(it_tile * 16 + cp_row + 4 * j, a.N - 1)) * a.ldw + g0 * (LW * 16) + cp_ch * 16;
+    s_at = static_cast<int64_t>(min(it_tile * 16 + (lane & 15), a.N - 1)) * KG + g0;
+  };
+  if (spt == 0) it_tile = a.tiles;  // fewer groups than warps: nothing to fetch
+  aim();
+  const uint32_t dst0 = ring_u + cp_row * 128;
+  uint32_t dst[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[j] = dst0 + 512 * j + ((cp_ch ^ rev3((cp_row + 4 * j) & 7)) << 4);
+  auto issue = [&]() {
+    {  // the previous stage's scales have arrived by now
+      float2* to = sz + (it_slot == 0 ? kWdStages - 1 : it_slot - 1) * (GS * 16) + lane;
+#pragma unroll
+      for (int k = 0; k < SL; ++k)
+        to[32 * k] = make_float2(scale_value(s_next[k], a.scale_dtype), __int_as_float(-static_cast<int>(z_next[k] & 15u)));
+    }
+    if (it_tile < a.tiles) {
+      if (it_stage * 8 + cp_ch < ng * LW) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) cp_async16(dst[j] + it_slot * 2048, src[j] + it_stage * 128);
+      }
+#pragma unroll
+      for (int k = 0; k < SL; ++k) {
+        const int64_t at = s_at + min(it_stage * GS + 2 * k + (lane >> 4), ng - 1);
+        s_next[k] = load_scale_bits(a.scales, a.scale_dtype, at);
+        z_next[k] = a.zeros ? __ldg(a.zeros + at) : 8;
+      }
+      if (++it_stage == spt) {
+        it_stage = 0;
+        it_tile += tile_step;
+        aim();
+      }
+    }
+    it_slot = it_slot == kWdStages - 1 ? 0 : it_slot + 1;
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kWdStages - 1; ++i) issue();
+
+  // ---- digits of x, one (token, group) per LG lanes
+  {
+    const int unit0 = warp * (32 / LG) + lane / LG, li = lane % LG;
+    for (int u = unit0; u < a.M * KG + unit0 % (32 / LG); u += teams * kW4Warps * (32 / LG)) {
+      // (the whole warp runs the same iterations: the shuffles need every lane)
+      const bool live = u < a.M * KG;
+      const int m = live ? u / KG : 0, gi = live ? u - m * KG : 0;
+      const uint16_t* src = static_cast<const uint16_t*>(a.x) + m * a.ldx + gi * G + li * EL;
+      uint32_t raw[EL / 2];
+      if (a.x_vec) {
+#pragma unroll
+        for (int j = 0; j < EL / 8; ++j) {
+          const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+          raw[4 * j] = v.x; raw[4 * j + 1] = v.y; raw[4 * j + 2] = v.z; raw[4 * j + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < EL / 2; ++j) raw[j] = __ldg(src + 2 * j) | (uint32_t(__ldg(src + 2 * j + 1)) << 16);
+      }
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < EL / 2; ++j) top = max(top, max(raw[j] & 0x7FFFu, (raw[j] >> 16) & 0x7FFFu));
+#pragma unroll
+      for (int o = LG / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      float down, up;
+      digit_scale(top, W4Num<T>::kF16, &down, &up);
+      int sum[3] = {0, 0, 0};
+#pragma unroll
+      for (int wv = 0; wv < EL / 8; ++wv) {  // one 8-code word: digits of codes 0 2 4 6 | 1 3 5 7
+        uint32_t p[3][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint16_t e = static_cast<uint16_t>(raw[4 * wv + (i >> 1)] >> (16 * (i & 1)));
+          digits3(to_float<T>(*reinterpret_cast<const T*>(&e)) * down, p[0][i], p[1][i], p[2][i]);
+        }
+        const int word = LW == 4 ? (li & 1) * 2 + wv : LW == 2 ? (li & 1) : 0;
+        const int q = LW == 1 ? li : li >> 1;
+        const int at = LW == 1 ? (gi * 4 + q) * 8
+                     : LW == 2 ? (gi * 4 + q) * 16 + word * 8
+                               : ((gi * 2 + word / 2) * 4 + q) * 16 + (word & 1) * 8;
+#pragma unroll
+        for (int d = 0; d < 3; ++d) {
+          const uint32_t lo = low_bytes(p[d][0], p[d][2], p[d][4], p[d][6]);
+          const uint32_t hi = low_bytes(p[d][1], p[d][3], p[d][5], p[d][7]);
+          sum[d] = __dp4a(static_cast<int>(lo), 0x01010101, sum[d]);
+          sum[d] = __dp4a(static_cast<int>(hi), 0x01010101, sum[d]);
+          if (live)
+            *reinterpret_cast<uint2*>(smem + L.digits + (3 * m + d) * pitch + at) = make_uint2(lo, hi);
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < 3; ++d) {
+#pragma unroll
+        for (int o = LG / 2; o > 0; o >>= 1) sum[d] += __shfl_xor_sync(0xffffffffu, sum[d], o);
+        if (live && li == d) {
+          const float f = d == 0 ? up : d == 1 ? up * 0.0078125f : up * 0.00006103515625f;
+          reinterpret_cast<float2*>(smem + L.table)[gi * 8 * NC + 3 * m + d] =
+              make_float2(f, __int_as_float(sum[d]));
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  const uint8_t* xs[NC];
+#pragma unroll
+  for (int j = 0; j < NC; ++j)  // columns past 3 M read the last one; their results are not used
+    xs[j] = smem + L.digits + min(8 * j + g, 3 * a.M - 1) * pitch + t * (LW == 1 ? 8 : 16);
+  const float4* table = reinterpret_cast<const float4*>(smem + L.table);
+  const int swz = rev3(g & 7);
+
+  int slot = 0, turn = 0;
+  for (int tile = tile0; tile < a.tiles; tile += tile_step) {
+    float acc[NC][4];
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    for (int st = 0; st < spt; ++st) {
+      cp_async_wait<kWdStages - 2>();
+      __syncwarp();  // the stage has landed for every lane, and the slot read last is free
+      issue();
+      const uint8_t* buf = ring + slot * 2048;
+      const float2* szs = sz + slot * (GS * 16);
+      slot = slot == kWdStages - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < GS; ++q) {
+        const int gl = st * GS + q;
+        if (gl >= ng) break;
+        uint32_t wa[LW], wb[LW];
+        if constexpr (LW == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(buf + g * 128 + (((q * 4 + t) ^ swz) << 4));
+          const uint4 v = *reinterpret_cast<const uint4*>(buf + 1024 + g * 128 + (((q * 4 + t) ^ swz) << 4));
+          wa[0] = u.x; wa[1] = u.y; wa[2] = u.z; wa[3] = u.w;
+          wb[0] = v.x; wb[1] = v.y; wb[2] = v.z; wb[3] = v.w;
+        } else if constexpr (LW == 2) {
+          const int o = g * 128 + (((q * 2 + (t >> 1)) ^ swz) << 4) + (t & 1) * 8;
+          const uint2 u = *reinterpret_cast<const uint2*>(buf + o), v = *reinterpret_cast<const uint2*>(buf + 1024 + o);
+          wa[0] = u.x; wa[1] = u.y;
+          wb[0] = v.x; wb[1] = v.y;
+        } else {
+          const int o = g * 128 + ((q ^ swz) << 4) + t * 4;
+          wa[0] = *reinterpret_cast<const uint32_t*>(buf + o);
+          wb[0] = *reinterpret_cast<const uint32_t*>(buf + 1024 + o);
+        }
+        int d[NC][4];
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[j][i] = 0x4B400000;
+#pragma unroll
+        for (int wi = 0; wi < LW; wi += 2) {
+          const uint32_t a0 = wa[wi] & 0x0F0F0F0Fu, a2 = (wa[wi] >> 4) & 0x0F0F0F0Fu;
+          const uint32_t a1 = wb[wi] & 0x0F0F0F0Fu, a3 = (wb[wi] >> 4) & 0x0F0F0F0Fu;
+          if constexpr (LW > 1) {
+            const uint32_t e0 = wa[wi + 1] & 0x0F0F0F0Fu, e2 = (wa[wi + 1] >> 4) & 0x0F0F0F0Fu;
+            const uint32_t e1 = wb[wi + 1] & 0x0F0F0F0Fu, e3 = (wb[wi + 1] >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+              const uint4 b = *reinterpret_cast<const uint4*>(xs[j] + ((g0 + gl) * (LW / 2) + wi / 2) * 64);
+              mma_u8s8(d[j], a0, a1, a2, a3, b.x, b.y);
+              mma_u8s8(d[j], e0, e1, e2, e3, b.z, b.w);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < NC; ++j) {
+              const uint2 b = *reinterpret_cast<const uint2*>(xs[j] + (g0 + gl) * 32);
+              mma_u8s8(d[j], a0, a1, a2, a3, b.x, b.y);
+            }
+          }
+        }
+        const float2 sa = szs[q * 16 + g], sb = szs[q * 16 + g + 8];
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+          const float4 tb = table[(g0 + gl) * 4 * NC + 4 * j + t];  // columns 2t, 2t + 1
+          const int za = __float_as_int(sa.y), zb = __float_as_int(sb.y);
+          const int s0 = __float_as_int(tb.y), s1 = __float_as_int(tb.w);
+          const float v0 = __int_as_float(d[j][0] + za * s0) - 12582912.0f;
+          const float v1 = __int_as_float(d[j][1] + za * s1) - 12582912.0f;
+          const float v2 = __int_as_float(d[j][2] + zb * s0) - 12582912.0f;
+          const float v3 = __int_as_float(d[j][3] + zb * s1) - 12582912.0f;
+          acc[j][0] = fmaf(v0 * tb.x, sa.x, acc[j][0]);
+          acc[j][1] = fmaf(v1 * tb.z, sa.x, acc[j][1]);
+          acc[j][2] = fmaf(v2 * tb.x, sb.x, acc[j][2]);
+          acc[j][3] = fmaf(v3 * tb.z, sb.x, acc[j][3]);
+        }
+      }
+    }
+    // ---- join the warps' K ranges and the digits, in a fixed order
+    float* sums = red + (turn & 1) * (kW4Warps * 16 * 8 * NC);
+    float* mine = sums + tw * (16 * 8 * NC);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      mine[(8 * j + 2 * t) * 16 + g] = acc[j][0];
+      mine[(8 * j + 2 * t + 1) * 16 + g] = acc[j][1];
+      mine[(8 * j + 2 * t) * 16 + g + 8] = acc[j][2];
+      mine[(8 * j + 2 * t + 1) * 16 + g + 8] = acc[j][3];
+    }
+    named_bar_sync(1 + team, kW4Warps * 32);
+    if (tw == turn % kW4Warps) {
+      for (int e = lane; e < 16 * a.M; e += 32) {
+        const int m = e >> 4, row = e & 15, n = tile * 16 + row;
+        float v = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kW4Warps; ++k)
+#pragma unroll
+          for (int p = 2; p >= 0; --p) v += sums[k * (16 * 8 * NC) + (3 * m + p) * 16 + row];
+        if (n < a.N) store_out(ep, m, n, epi_scaled(v, 1.0f, 1.0f, 1.0f, ep, n));
+      }
+    }
+    ++turn;
+  }
 }
 
 // ---------------------------------------------------------------- many tokens
