@@ -271,14 +271,14 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   ep.N = static_cast<int>(N);
   const bool x_vec = aligned(x, 16) && ldx % 8 == 0;
   WdPlan wd;
-  if (wd_plan(sms, M, N, K, int(group), &wd)) {
+  // (scales of x's type; N * K / G below 2^31)
+  if (scale_dtype == x_dtype + 1 && N * (K / group) <= kIntMax && wd_plan(sms, M, N, K, int(group), &wd)) {
     W4DigitArgs a{};
     a.x = x;
     a.ldx = ldx;
     a.w = w;
     a.ldw = ldw;
     a.scales = scales;
-    a.scale_dtype = scale_dtype;
     a.zeros = zeros;
     a.M = static_cast<int>(M);
     a.N = static_cast<int>(N);

@@ -299,11 +299,11 @@ __global__ void __launch_bounds__(kW4Warps * 32)
 // XOR-swizzled by the row so that the fragment reads have no bank conflicts); the ring
 // runs on across tiles, so the loads of the next tile are in flight while one is
 // summed.  A stage's scales and zero points travel with it: loaded to registers when
-// its bytes are asked for, converted and put into the stage's slot one step later
+// its bytes are asked for, converted and put into the stage's slot just before it is read
 // (waiting for them at the start of each tile cost more than the tile).  A tile's sums
 // are double-buffered: one barrier per tile, and a different warp each time adds and
 // stores them while the others go on.
-constexpr int kWdStages = 3;
+constexpr int kWdStages = 3;  // issue() relies on three
 // Most teams per CTA, by the digit columns' register need.
 constexpr int wd_teams(int nc) { return nc == 3 ? 2 : 3; }
 
@@ -312,25 +312,12 @@ struct W4DigitArgs {
   int64_t ldx;
   const uint8_t* w;
   int64_t ldw;
-  const void* scales;
-  int scale_dtype;
+  const void* scales;  // of x's type
   const uint8_t* zeros;
   int M, N, K;
   int x_vec;
   int tiles;  // ceil(N / 16)
 };
-
-// A scale as its raw bits, and their value.
-__device__ __forceinline__ uint32_t load_scale_bits(const void* p, int dtype, int64_t i) {
-  return dtype == kBiasF32 ? __ldg(static_cast<const uint32_t*>(p) + i)
-                           : static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(p) + i));
-}
-__device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
-  if (dtype == kBiasF32) return __uint_as_float(bits);
-  if (dtype == kBiasBF16) return __uint_as_float(bits << 16);
-  const uint16_t h = static_cast<uint16_t>(bits);
-  return __half2float(*reinterpret_cast<const __half*>(&h));
-}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -347,6 +334,15 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, 
   asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with the accumulators starting at the bits of 1.5 * 2^23.
+__device__ __forceinline__ void mma_u8s8_start(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  const int z = 0x4B400000;
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(z));
 }
 
 // Shared memory: rings, digits [3M][pitch], {2^E / (64 * 128^p), digit sum}
@@ -396,16 +392,16 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
   constexpr int SL = GS / 2;
   int it_tile = tile0, it_stage = 0, it_slot = 0;
   const int cp_row = lane >> 3, cp_ch = lane & 7;
-  uint32_t s_next[SL], z_next[SL];
+  uint32_t s_next[2][SL], z_next[2][SL];  // of the last stage asked for, and the one before
 #pragma unroll
-  for (int k = 0; k < SL; ++k) s_next[k] = z_next[k] = 0;
+  for (int k = 0; k < SL; ++k) s_next[0][k] = z_next[0][k] = s_next[1][k] = z_next[1][k] = 0;
   const uint8_t* src[4];   // this lane's rows of the tile being fetched
-  int64_t s_at = 0;
+  uint32_t s_at = 0;
   auto aim = [&]() {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       src[j] = a.w + static_cast<int64_t>(min(it_tile * 16 + cp_row + 4 * j, a.N - 1)) * a.ldw + g0 * (LW * 16) + cp_ch * 16;
-    s_at = static_cast<int64_t>(min(it_tile * 16 + (lane & 15), a.N - 1)) * KG + g0;
+    s_at = static_cast<uint32_t>(min(it_tile * 16 + (lane & 15), a.N - 1)) * KG + g0;
   };
   if (spt == 0) it_tile = a.tiles;  // fewer groups than warps: nothing to fetch
   aim();
@@ -414,11 +410,16 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 #pragma unroll
   for (int j = 0; j < 4; ++j) dst[j] = dst0 + 512 * j + ((cp_ch ^ rev3((cp_row + 4 * j) & 7)) << 4);
   auto issue = [&]() {
-    {  // the previous stage's scales have arrived by now
-      float2* to = sz + (it_slot == 0 ? kWdStages - 1 : it_slot - 1) * (GS * 16) + lane;
+    {  // the scales asked for two steps ago have arrived by now: the stage read next
+      float2* to = sz + (it_slot == kWdStages - 1 ? 0 : it_slot + 1) * (GS * 16) + lane;
 #pragma unroll
-      for (int k = 0; k < SL; ++k)
-        to[32 * k] = make_float2(scale_value(s_next[k], a.scale_dtype), __int_as_float(-static_cast<int>(z_next[k] & 15u)));
+      for (int k = 0; k < SL; ++k) {
+        const uint16_t bits = static_cast<uint16_t>(s_next[1][k]);
+        to[32 * k] = make_float2(to_float<T>(*reinterpret_cast<const T*>(&bits)),
+                                 __int_as_float(-static_cast<int>(z_next[1][k] & 15u)));
+        s_next[1][k] = s_next[0][k];
+        z_next[1][k] = z_next[0][k];
+      }
     }
     if (it_tile < a.tiles) {
       if (it_stage * 8 + cp_ch < ng * LW) {
@@ -427,9 +428,9 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
       }
 #pragma unroll
       for (int k = 0; k < SL; ++k) {
-        const int64_t at = s_at + min(it_stage * GS + 2 * k + (lane >> 4), ng - 1);
-        s_next[k] = load_scale_bits(a.scales, a.scale_dtype, at);
-        z_next[k] = a.zeros ? __ldg(a.zeros + at) : 8;
+        const uint32_t at = s_at + min(it_stage * GS + 2 * k + (lane >> 4), ng - 1);
+        s_next[0][k] = __ldg(static_cast<const uint16_t*>(a.scales) + at);
+        z_next[0][k] = a.zeros ? __ldg(a.zeros + at) : 8;
       }
       if (++it_stage == spt) {
         it_stage = 0;
@@ -525,6 +526,7 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
       cp_async_wait<kWdStages - 2>();
       __syncwarp();  // the stage has landed for every lane, and the slot read last is free
       issue();
+      __syncwarp();  // this stage's scales are in place
       const uint8_t* buf = ring + slot * 2048;
       const float2* szs = sz + slot * (GS * 16);
       slot = slot == kWdStages - 1 ? 0 : slot + 1;
@@ -550,10 +552,6 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
         }
         int d[NC][4];
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) d[j][i] = 0x4B400000;
-#pragma unroll
         for (int wi = 0; wi < LW; wi += 2) {
           const uint32_t a0 = wa[wi] & 0x0F0F0F0Fu, a2 = (wa[wi] >> 4) & 0x0F0F0F0Fu;
           const uint32_t a1 = wb[wi] & 0x0F0F0F0Fu, a3 = (wb[wi] >> 4) & 0x0F0F0F0Fu;
@@ -563,14 +561,15 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
               const uint4 b = *reinterpret_cast<const uint4*>(xs[j] + ((g0 + gl) * (LW / 2) + wi / 2) * 64);
-              mma_u8s8(d[j], a0, a1, a2, a3, b.x, b.y);
+              if (wi == 0) mma_u8s8_start(d[j], a0, a1, a2, a3, b.x, b.y);
+              else mma_u8s8(d[j], a0, a1, a2, a3, b.x, b.y);
               mma_u8s8(d[j], e0, e1, e2, e3, b.z, b.w);
             }
           } else {
 #pragma unroll
             for (int j = 0; j < NC; ++j) {
               const uint2 b = *reinterpret_cast<const uint2*>(xs[j] + (g0 + gl) * 32);
-              mma_u8s8(d[j], a0, a1, a2, a3, b.x, b.y);
+              mma_u8s8_start(d[j], a0, a1, a2, a3, b.x, b.y);
             }
           }
         }
@@ -580,14 +579,12 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
           const float4 tb = table[(g0 + gl) * 4 * NC + 4 * j + t];  // columns 2t, 2t + 1
           const int za = __float_as_int(sa.y), zb = __float_as_int(sb.y);
           const int s0 = __float_as_int(tb.y), s1 = __float_as_int(tb.w);
-          const float v0 = __int_as_float(d[j][0] + za * s0) - 12582912.0f;
-          const float v1 = __int_as_float(d[j][1] + za * s1) - 12582912.0f;
-          const float v2 = __int_as_float(d[j][2] + zb * s0) - 12582912.0f;
-          const float v3 = __int_as_float(d[j][3] + zb * s1) - 12582912.0f;
-          acc[j][0] = fmaf(v0 * tb.x, sa.x, acc[j][0]);
-          acc[j][1] = fmaf(v1 * tb.z, sa.x, acc[j][1]);
-          acc[j][2] = fmaf(v2 * tb.x, sb.x, acc[j][2]);
-          acc[j][3] = fmaf(v3 * tb.z, sb.x, acc[j][3]);
+          // (i + 1.5 * 2^23) f - 1.5 * 2^23 f: both products are exact, f a power of two
+          const float m0 = -12582912.0f * tb.x, m1 = -12582912.0f * tb.z;
+          acc[j][0] = fmaf(fmaf(__int_as_float(d[j][0] + za * s0), tb.x, m0), sa.x, acc[j][0]);
+          acc[j][1] = fmaf(fmaf(__int_as_float(d[j][1] + za * s1), tb.z, m1), sa.x, acc[j][1]);
+          acc[j][2] = fmaf(fmaf(__int_as_float(d[j][2] + zb * s0), tb.x, m0), sb.x, acc[j][2]);
+          acc[j][3] = fmaf(fmaf(__int_as_float(d[j][3] + zb * s1), tb.z, m1), sb.x, acc[j][3]);
         }
       }
     }
