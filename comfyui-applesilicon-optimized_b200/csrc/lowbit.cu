@@ -65,47 +65,52 @@ int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, 
 }
 
 // ------------------------------------------------------------ 4-bit linear
-// Largest M of the warp-MMA kernel; above it the weight is decoded once per call
-// for the tile GEMM.
-constexpr int64_t kW4MaxSmallM = 32;
+// Largest M of the warp-MMA kernels, which run 32 tokens at a time; above it the
+// weight is decoded once per call for the tile GEMM.
+constexpr int64_t kW4MaxSmallM = 64;
 
-struct W4Plan {
-  int wr, splits, smem;
+// K slices and row parts of the slice kernel: the split whose busiest warp has the
+// fewest groups to go through, x's slice beside the rings.
+struct WsPlan {
+  int slices, parts, smem;
 };
-
-// Rows per CTA (16 * wr) and cluster size.  With few tokens a CTA takes one
-// 16-row tile and its 8 warps split K; more tokens make staging x per CTA cost
-// more than it gives, so a CTA takes 64 rows and a cluster splits K.
-W4Plan w4_plan(int64_t M, int64_t N, int64_t K, int G, int cols) {
-  W4Plan p{};
-  const int64_t KG = K / G;
-  p.wr = M <= 4 ? 1 : 4;
-  p.splits = 1;
-  const int64_t want = M <= 4 ? 296 : 592;  // CTAs of 8 warps
-  while (p.splits < 8 && cdiv(N, 16 * p.wr) * p.splits < want && 2 * p.splits * (kW4Warps / p.wr) <= KG)
-    p.splits *= 2;
-  auto bytes = [&](int s) { return w4_smem_bytes(int(M), int(cdiv(KG, s)) * G, cols, p.wr); };
-  while (p.splits < 8 && bytes(p.splits) > 100 * 1024) p.splits *= 2;
-  p.smem = bytes(p.splits);
-  return p;
+bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
+  const int64_t KG = K / G, tiles = cdiv(N, 16);
+  int64_t best = -1;
+  for (int s = 1; s <= 32 && s <= KG && s <= sms; ++s) {
+    const int64_t gs = cdiv(KG, s);
+    const int smem = ws_smem_bytes(int(M), int(gs) * G, G);
+    if (smem > 227 * 1024) continue;
+    const int64_t parts = sms / s;
+    // a slice more costs its partial sums' round trip, about 2 groups of a warp
+    const int64_t cost = cdiv(tiles, parts * kWsWarps) * gs * G / 32 + (s > 1 ? 8 + s / 4 : 0);
+    if (best < 0 || cost < best) {
+      best = cost;
+      p->slices = s;
+      p->parts = static_cast<int>(parts < cdiv(tiles, kWsWarps) ? parts : cdiv(tiles, kWsWarps));
+      p->smem = smem;
+    }
+  }
+  return best >= 0;
 }
+// The slices' sums for one launch of at most 32 tokens.
+size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(32) * (M < 32 ? M : 32) * N * 4; }
 
 template <typename T, int LW>
-int launch_w4_cols(const W4Args& a, const EpiArgs& ep, const W4Plan& p, int nt, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(cdiv(a.N, 16 * p.wr) * p.splits));
-  switch (nt) {
-    case 1: return launch(w4a16_kernel<T, LW, 1>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
-    case 2: return launch(w4a16_kernel<T, LW, 2>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
-    default: return launch(w4a16_kernel<T, LW, 4>, grid, kW4Warps * 32, p.smem, p.splits, st, a, ep);
-  }
+int launch_slice_cols(const W4SliceArgs& a, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>(p.slices * p.parts));
+  if (a.M <= 8) return launch(w4_slice_kernel<T, LW, 1>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  if (a.M <= 16) return launch(w4_slice_kernel<T, LW, 2>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  return launch(w4_slice_kernel<T, LW, 4>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
 }
 template <typename T>
-int launch_w4(const W4Args& a, const EpiArgs& ep, const W4Plan& p, int nt, cudaStream_t st) {
-  switch (a.G) {
-    case 32: return launch_w4_cols<T, 1>(a, ep, p, nt, st);
-    case 64: return launch_w4_cols<T, 2>(a, ep, p, nt, st);
-    default: return launch_w4_cols<T, 4>(a, ep, p, nt, st);
-  }
+int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
+  int s = G == 32   ? launch_slice_cols<T, 1>(a, ep, p, st)
+          : G == 64 ? launch_slice_cols<T, 2>(a, ep, p, st)
+                    : launch_slice_cols<T, 4>(a, ep, p, st);
+  if (s != B200Q_OK || !a.part) return s;
+  const dim3 grid(static_cast<unsigned>(cdiv(int64_t(a.M) * a.N, 256)));
+  return launch(w4_join_kernel, grid, 256, 0, 1, st, static_cast<const float*>(a.part), a.slices, ep);
 }
 
 // The integer kernel for few tokens, when x's digits fit beside the rings: at most
@@ -238,8 +243,14 @@ bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
 extern "C" {
 
 size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K) {
-  if (M <= kW4MaxSmallM || N <= 0 || K <= 0) return 0;
-  return w4_work(M, N, K).total;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M > kW4MaxSmallM) return w4_work(M, N, K).total;
+  // the integer kernel for few tokens needs none
+  const int sms = host::device_sms();
+  WdPlan wd;
+  if (sms && wd_plan(sms, M, N, K, 32, &wd) && wd_plan(sms, M, N, K, 64, &wd) && wd_plan(sms, M, N, K, 128, &wd))
+    return 0;
+  return ws_work_bytes(M, N);
 }
 
 int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw,
@@ -269,6 +280,8 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   ep.act = act;
   ep.M = static_cast<int>(M);
   ep.N = static_cast<int>(N);
+  const size_t need = b200q_w4a16_workspace_size(M, N, K);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return B200Q_ERR_WORKSPACE;
   const bool x_vec = aligned(x, 16) && ldx % 8 == 0;
   WdPlan wd;
   // (scales of x's type; N * K / G below 2^31)
@@ -288,30 +301,37 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     return x_dtype == B200Q_F16 ? launch_digits<__half>(a, int(group), ep, wd, st)
                                 : launch_digits<__nv_bfloat16>(a, int(group), ep, wd, st);
   }
-  if (M <= kW4MaxSmallM) {
-    W4Args a{};
-    a.x = x;
-    a.ldx = ldx;
-    a.w = w;
-    a.ldw = ldw;
-    a.scales = scales;
-    a.scale_dtype = scale_dtype;
-    a.zeros = zeros;
-    a.M = static_cast<int>(M);
-    a.N = static_cast<int>(N);
-    a.K = static_cast<int>(K);
-    a.G = static_cast<int>(group);
-    a.x_vec = x_vec;
-    const int nt = M <= 8 ? 1 : M <= 16 ? 2 : 4;
-    const W4Plan p = w4_plan(M, N, K, a.G, 8 * nt);
-    if (p.smem > 227 * 1024) return B200Q_ERR_UNSUPPORTED;  // K beyond about 50,000 at 32 tokens
-    a.wr = p.wr;
-    a.splits = p.splits;
-    return x_dtype == B200Q_F16 ? launch_w4<__half>(a, ep, p, nt, st)
-                                : launch_w4<__nv_bfloat16>(a, ep, p, nt, st);
+  WsPlan ws;
+  const int64_t step = M < 32 ? M : 32;
+  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, step, N, K, int(group), &ws)) {
+    for (int64_t m0 = 0; m0 < M; m0 += step) {
+      const int64_t rows = M - m0 < step ? M - m0 : step;
+      W4SliceArgs a{};
+      a.x = static_cast<const uint16_t*>(x) + m0 * ldx;
+      a.ldx = ldx;
+      a.w = w;
+      a.ldw = ldw;
+      a.scales = scales;
+      a.scale_dtype = scale_dtype;
+      a.zeros = zeros;
+      a.part = ws.slices > 1 ? static_cast<float*>(workspace) : nullptr;
+      a.M = static_cast<int>(rows);
+      a.N = static_cast<int>(N);
+      a.K = static_cast<int>(K);
+      a.x_vec = x_vec;
+      a.slices = ws.slices;
+      a.parts = ws.parts;
+      EpiArgs e = ep;
+      e.M = static_cast<int>(rows);
+      e.out = static_cast<char*>(out) + m0 * ldo * (out_dtype == B200Q_F32 ? 4 : 2);
+      const int s = x_dtype == B200Q_F16 ? launch_slice<__half>(a, int(group), e, ws, st)
+                                         : launch_slice<__nv_bfloat16>(a, int(group), e, ws, st);
+      if (s != B200Q_OK) return s;
+    }
+    return B200Q_OK;
   }
+  if (M <= kW4MaxSmallM) return B200Q_ERR_UNSUPPORTED;  // N * K / group above 2^31
   const W4Work o = w4_work(M, N, K);
-  if (!workspace || workspace_bytes < o.total || !aligned(workspace, 256)) return B200Q_ERR_WORKSPACE;
   uint8_t* base = static_cast<uint8_t*>(workspace);
   __half* w16 = reinterpret_cast<__half*>(base);
   float* col = reinterpret_cast<float*>(base + o.col);

@@ -14,13 +14,12 @@
 // columns; nothing is rounded before the output.
 //
 // Layout.  The order of k inside a group is free as long as both operands
-// agree.  Lane (g, t) = (lane / 4, lane % 4) reads the G/4 codes of its quarter t
-// of the group for rows g and g + 8 as they are stored (one 16-byte load each at
-// G = 128); pair i of an 8-code word w is (w >> 4i) & 0x000F000F = codes i and
-// i + 4.  x is staged once per CTA in shared memory in that order (8 values as
-// 0 4 1 5 2 6 3 7; quarter-major), so one 16-byte shared load feeds two MMAs,
-// and the row pitch is 64 modulo 128 bytes, which makes those loads free of
-// bank conflicts.
+// agree.  Lane (g, t) = (lane / 4, lane % 4) takes the G/4 codes of its quarter t
+// of the group for rows g and g + 8 as they are stored; pair i of an 8-code word w
+// is (w >> 4i) & 0x000F000F = codes i and i + 4.  x is staged in shared memory in
+// that order (8 values as 0 4 1 5 2 6 3 7; quarter-major), so one 16-byte shared
+// load feeds two MMAs, and the row pitch is 64 modulo 128 bytes, which makes those
+// loads free of bank conflicts.  Few tokens take an integer form of the same sums.
 #pragma once
 
 #include "digits.cuh"
@@ -29,26 +28,48 @@
 
 namespace b200q {
 
-constexpr int kW4Warps = 8;
-
-struct W4Args {
-  const void* x;         // [M, K] bf16 / fp16
-  int64_t ldx;           // elements
-  const uint8_t* w;      // [N, K / 2]
-  int64_t ldw;           // bytes
-  const void* scales;    // [N, K / G]
-  int scale_dtype;       // kBiasBF16 / kBiasF16 / kBiasF32
-  const uint8_t* zeros;  // [N, K / G] or null (8)
-  int M, N, K, G;
-  int x_vec;             // rows of x are 16-byte aligned
-  int wr;                // warps along the rows: the CTA's tile is 16 * wr rows
-  int splits;            // cluster size: CTAs that share a row tile's K
-};
+constexpr int kW4Warps = 8;  // warps that split a row tile's K in the integer kernel
 
 __device__ __forceinline__ float load_scale(const void* p, int dtype, int64_t i) {
   if (dtype == kBiasBF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
   if (dtype == kBiasF16) return __half2float(static_cast<const __half*>(p)[i]);
   return static_cast<const float*>(p)[i];
+}
+// A scale as its raw bits, and their value.
+__device__ __forceinline__ uint32_t load_scale_bits(const void* p, int dtype, uint32_t i) {
+  return dtype == kBiasF32 ? __ldg(static_cast<const uint32_t*>(p) + i)
+                           : static_cast<uint32_t>(__ldg(static_cast<const uint16_t*>(p) + i));
+}
+__device__ __forceinline__ float scale_value(uint32_t bits, int dtype) {
+  if (dtype == kBiasF32) return __uint_as_float(bits);
+  if (dtype == kBiasBF16) return __uint_as_float(bits << 16);
+  const uint16_t h = static_cast<uint16_t>(bits);
+  return __half2float(*reinterpret_cast<const __half*>(&h));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ int rev3(int r) { return ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1); }
+
+// This lane's LW words of group q (of a stage) of row g, from a ring stage: 128 bytes
+// per row, 16-byte chunks XOR-swizzled by rev3(row & 7) (`swz`, rows 8 apart alike).
+template <int LW>
+__device__ __forceinline__ void w4_words(const uint8_t* buf, int g, int t, int q, int swz, uint32_t (&w)[LW]) {
+  if constexpr (LW == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(buf + g * 128 + (((q * 4 + t) ^ swz) << 4));
+    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  } else if constexpr (LW == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(buf + g * 128 + (((q * 2 + (t >> 1)) ^ swz) << 4) + (t & 1) * 8);
+    w[0] = u.x; w[1] = u.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(buf + g * 128 + ((q ^ swz) << 4) + t * 4);
+  }
 }
 
 template <typename T>
@@ -64,7 +85,7 @@ struct W4Num<__nv_bfloat16> {
   }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -82,7 +103,7 @@ struct W4Num<__half> {
   }
   static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                              uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -98,185 +119,231 @@ __device__ __forceinline__ void w4_decode(uint32_t w, uint32_t zp, uint32_t (&p)
     p[i] = W4Num<T>::sub(((w >> (4 * i)) & 0x000F000Fu) | W4Num<T>::kMagic, zp);
 }
 
-// Shared bytes per token row for a slice of `k` codes.
-__host__ __device__ __forceinline__ int w4_pitch(int k) {
-  const int b = 2 * k;
-  return b + ((b & 127) == 64 ? 0 : 64);
-}
-// Dynamic shared memory: x slice, warp partials, CTA partials.
-__host__ __device__ __forceinline__ int w4_smem_bytes(int M, int k_slice, int cols, int wr) {
-  return M * w4_pitch(k_slice) + (kW4Warps * 16 + 16 * wr) * cols * 4;
+// ---------------------------------------------------------------- up to 32 tokens
+// x does not fit one CTA's shared memory whole, so K is cut into slices: a CTA keeps
+// its slice of x and its warps, each on its own, go through 16-row tiles of the
+// weight's slice (persistent, no barrier after x is staged).  With more than one
+// slice the fp32 sums go to the workspace, [slice][token][row], and w4_join_kernel
+// adds them in slice order.  Rings as in the integer kernel below: 128 bytes per row
+// and stage, scales travelling along.
+constexpr int kWsWarps = 16;
+constexpr int kWsStages = 3;  // issue() relies on three
+
+struct W4SliceArgs {
+  const void* x;         // [M, K] bf16 / fp16
+  int64_t ldx;           // elements
+  const uint8_t* w;      // [N, K / 2]
+  int64_t ldw;           // bytes
+  const void* scales;    // [N, K / G]
+  int scale_dtype;       // kBiasBF16 / kBiasF16 / kBiasF32
+  const uint8_t* zeros;  // [N, K / G] or null (8)
+  float* part;           // [slices][M][N], or null: one slice, the epilogue runs here
+  int M, N, K;
+  int x_vec;             // rows of x are 16-byte aligned
+  int slices, parts;     // grid = slices * parts
+};
+
+// Shared bytes per token row for a slice of `k` codes: 64 modulo 128.
+__host__ __device__ __forceinline__ int ws_pitch(int k) { return 2 * k + ((2 * k & 127) == 64 ? 0 : 64); }
+__host__ __device__ __forceinline__ int ws_smem_bytes(int M, int k_slice, int G) {
+  return kWsWarps * kWsStages * (2048 + (256 / G) * 16 * 8) + M * ws_pitch(k_slice);
 }
 
-template <int LW>
-__device__ __forceinline__ void w4_load(uint32_t (&r)[LW], const uint8_t* p) {
-  if constexpr (LW == 4) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    r[0] = v.x; r[1] = v.y; r[2] = v.z; r[3] = v.w;
-  } else if constexpr (LW == 2) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    r[0] = v.x; r[1] = v.y;
-  } else {
-    r[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
-  }
-}
-
-// LW = G / 32 words per lane, row and group; NT = 8-token columns of the MMA.
+// LW = G / 32 words per lane, row and group; NT = 8-token columns.
 template <typename T, int LW, int NT>
-__global__ void __launch_bounds__(kW4Warps * 32)
-    w4a16_kernel(const W4Args a, const EpiArgs ep) {
+__global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceArgs a, const EpiArgs ep) {
   extern __shared__ __align__(128) uint8_t smem[];
   constexpr int G = 32 * LW;
-  constexpr int U = LW == 4 ? 2 : LW == 2 ? 4 : 8;  // groups per load batch
-  constexpr int kCols = 8 * NT;
+  constexpr int GS = 8 / LW;  // groups per stage
+  constexpr int SL = GS / 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int rank = a.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
-  const int tile = blockIdx.x / a.splits;
+  const int slice = blockIdx.x % a.slices, part = blockIdx.x / a.slices;
   const int KG = a.K / G;
-  const int wk_n = kW4Warps / a.wr;
-  const int wr_i = warp % a.wr, wk_i = warp / a.wr;
-  // this CTA's groups, then this warp's
-  const int cg0 = static_cast<int>(int64_t(KG) * rank / a.splits);
-  const int cg1 = static_cast<int>(int64_t(KG) * (rank + 1) / a.splits);
-  const int g0 = cg0 + (cg1 - cg0) * wk_i / wk_n;
-  const int g1 = cg0 + (cg1 - cg0) * (wk_i + 1) / wk_n;
-  const int max_slice = (KG + a.splits - 1) / a.splits * G;
-  const int pitch = w4_pitch(max_slice);
-  float* red = reinterpret_cast<float*>(smem + a.M * pitch);  // [warp][col][16]
-  float* part = red + kW4Warps * 16 * kCols;                  // [col][16 * wr]
+  const int g0 = static_cast<int>(int64_t(KG) * slice / a.slices);
+  const int ng = static_cast<int>(int64_t(KG) * (slice + 1) / a.slices) - g0;
+  const int spt = (ng + GS - 1) / GS;
+  const int pitch = ws_pitch((KG + a.slices - 1) / a.slices * G);
+  uint8_t* ring = smem + warp * (kWsStages * 2048);
+  float2* sz = reinterpret_cast<float2*>(smem + kWsWarps * kWsStages * 2048) + warp * (kWsStages * GS * 16);
+  uint8_t* xsm = smem + kWsWarps * kWsStages * (2048 + GS * 16 * 8);
+  const int tiles = (a.N + 15) / 16;
+  const int tile0 = part * kWsWarps + warp, tile_step = a.parts * kWsWarps;
 
   griddep_wait();
   griddep_launch_dependents();
 
-  // ---- stage x[:, cg0*G .. cg1*G) in fragment order
-  {
-    const int pieces = (cg1 - cg0) * (G / 8);
-    for (int i = tid; i < pieces * a.M; i += kW4Warps * 32) {
-      const int m = i / pieces, p = i - m * pieces;
-      const T* src = static_cast<const T*>(a.x) + m * a.ldx + int64_t(cg0) * G + p * 8;
-      uint16_t e[8];
-      if (a.x_vec) {
-        *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(src));
-      } else {
+  // ---- the ring: lane copies chunk lane % 8 of rows lane / 8 + 4 j, and loads entries
+  // e = lane + 32 k = (group e / 16, row e % 16) of the stage's scales
+  int it_tile = tile0, it_stage = 0, it_slot = 0;
+  const int cp_row = lane >> 3, cp_ch = lane & 7;
+  uint32_t s_next[2][SL], z_next[2][SL];  // of the last stage asked for, and the one before
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = __ldg(reinterpret_cast<const uint16_t*>(src) + j);
-      }
-      const int grp = p / (G / 8), r = p - grp * (G / 8);
-      const int at = (grp * LW + r % LW) * 4 + r / LW;  // [group][word][quarter]
-      uint4 v;
-      v.x = e[0] | (uint32_t(e[4]) << 16);
-      v.y = e[1] | (uint32_t(e[5]) << 16);
-      v.z = e[2] | (uint32_t(e[6]) << 16);
-      v.w = e[3] | (uint32_t(e[7]) << 16);
-      *reinterpret_cast<uint4*>(smem + m * pitch + at * 16) = v;
-    }
-  }
-  __syncthreads();
-
-  // ---- this warp's 16 rows x its groups
-  const int n0 = (tile * a.wr + wr_i) * 16;
-  const int rA = min(n0 + g, a.N - 1), rB = min(n0 + g + 8, a.N - 1);
-  const uint8_t* wA = a.w + int64_t(rA) * a.ldw + t * (4 * LW);
-  const uint8_t* wB = a.w + int64_t(rB) * a.ldw + t * (4 * LW);
-  const int64_t sA = int64_t(rA) * KG, sB = int64_t(rB) * KG;
-  const uint8_t* xs[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)  // columns past M read row M - 1; their results are not used
-    xs[j] = smem + min(8 * j + g, a.M - 1) * pitch + t * 16;
-
-  float acc[NT][4];
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
-
-  uint32_t ca[U][LW], cb[U][LW];
-  float fa[U], fb[U];
-  uint32_t za[U], zb[U];
-  auto load = [&](int gi) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int q = min(gi + u, g1 - 1);
-      w4_load<LW>(ca[u], wA + int64_t(q) * (G / 2));
-      w4_load<LW>(cb[u], wB + int64_t(q) * (G / 2));
-      fa[u] = load_scale(a.scales, a.scale_dtype, sA + q);
-      fb[u] = load_scale(a.scales, a.scale_dtype, sB + q);
-      za[u] = a.zeros ? a.zeros[sA + q] & 15u : 8u;
-      zb[u] = a.zeros ? a.zeros[sB + q] & 15u : 8u;
-    }
+  for (int k = 0; k < SL; ++k) s_next[0][k] = z_next[0][k] = s_next[1][k] = z_next[1][k] = 0;
+  const uint8_t* src0 = nullptr;
+  auto aim = [&]() {
+    src0 = a.w + static_cast<int64_t>(it_tile * 16 + cp_row) * a.ldw + g0 * (LW * 16) + cp_ch * 16;
   };
-  for (int gi = g0; gi < g1; gi += U) {
-    load(gi);
+  aim();
+  const uint32_t dst0 = smem_u32(ring) + cp_row * 128;
+  auto issue = [&]() {
+    {  // the scales asked for two steps ago have arrived by now: the stage read next
+      float2* to = sz + (it_slot == kWsStages - 1 ? 0 : it_slot + 1) * (GS * 16);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (gi + u >= g1) break;
-      float part_[NT][4];
+      for (int k = 0; k < SL; ++k) {
+        to[lane + 32 * k] = make_float2(scale_value(s_next[1][k], a.scale_dtype),
+                                          __uint_as_float(W4Num<T>::kMagic | (z_next[1][k] & 15u) * 0x00010001u));
+        s_next[1][k] = s_next[0][k];
+        z_next[1][k] = z_next[0][k];
+      }
+    }
+    if (it_tile < tiles) {
+      if (it_stage * 8 + cp_ch < ng * LW) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) part_[j][i] = 0.0f;
-      const uint32_t zpa = W4Num<T>::kMagic | za[u] * 0x00010001u;
-      const uint32_t zpb = W4Num<T>::kMagic | zb[u] * 0x00010001u;
-      const int xo = (gi + u - cg0) * LW * 64;
-#pragma unroll
-      for (int wi = 0; wi < LW; ++wi) {
-        uint32_t pa[4], pb[4];
-        w4_decode<T>(ca[u][wi], zpa, pa);
-        w4_decode<T>(cb[u][wi], zpb, pb);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const uint4 xv = *reinterpret_cast<const uint4*>(xs[j] + xo + wi * 64);
-          W4Num<T>::mma(part_[j], pa[0], pb[0], pa[1], pb[1], xv.x, xv.y);
-          W4Num<T>::mma(part_[j], pa[2], pb[2], pa[3], pb[3], xv.z, xv.w);
+        for (int j = 0; j < 4; ++j) {
+          // rows past N repeat row N - 1
+          const int over = min(a.N - 1 - (it_tile * 16 + cp_row + 4 * j), 0);
+          cp_async16(dst0 + 512 * j + it_slot * 2048 + ((cp_ch ^ rev3((cp_row + 4 * j) & 7)) << 4),
+                     src0 + static_cast<int64_t>(4 * j + over) * a.ldw + it_stage * 128);
         }
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        acc[j][0] = fmaf(fa[u], part_[j][0], acc[j][0]);
-        acc[j][1] = fmaf(fa[u], part_[j][1], acc[j][1]);
-        acc[j][2] = fmaf(fb[u], part_[j][2], acc[j][2]);
-        acc[j][3] = fmaf(fb[u], part_[j][3], acc[j][3]);
+      for (int k = 0; k < SL; ++k) {
+        const int e = lane + 32 * k;
+        const int n = min(it_tile * 16 + e % 16, a.N - 1);
+        const uint32_t at = static_cast<uint32_t>(n) * KG + g0 + min(it_stage * GS + e / 16, ng - 1);
+        s_next[0][k] = load_scale_bits(a.scales, a.scale_dtype, at);
+        z_next[0][k] = a.zeros ? __ldg(a.zeros + at) : 8;
+      }
+      if (++it_stage == spt) {
+        it_stage = 0;
+        it_tile += tile_step;
+        aim();
       }
     }
-  }
-
-  // ---- join the warps' K ranges, then the cluster's, in a fixed order
-  float* mine = red + warp * 16 * kCols;
+    it_slot = it_slot == kWsStages - 1 ? 0 : it_slot + 1;
+    cp_async_commit();
+  };
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    mine[(8 * j + 2 * t) * 16 + g] = acc[j][0];
-    mine[(8 * j + 2 * t + 1) * 16 + g] = acc[j][1];
-    mine[(8 * j + 2 * t) * 16 + g + 8] = acc[j][2];
-    mine[(8 * j + 2 * t + 1) * 16 + g + 8] = acc[j][3];
+  for (int i = 0; i < kWsStages - 1; ++i) issue();
+
+  // ---- stage x[:, slice] in fragment order, four pieces of 8 values at a time
+  {
+    const int pieces = ng * (G / 8), total = pieces * a.M;
+    for (int i0 = tid; i0 < total; i0 += 4 * kWsWarps * 32) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kWsWarps * 32;
+        if (i < total) {
+          const int m = i / pieces, p = i - m * pieces;
+          const uint16_t* src = static_cast<const uint16_t*>(a.x) + m * a.ldx + int64_t(g0) * G + p * 8;
+          if (a.x_vec) {
+            v[u] = __ldg(reinterpret_cast<const uint4*>(src));
+          } else {
+            uint32_t e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = __ldg(src + 2 * j) | (uint32_t(__ldg(src + 2 * j + 1)) << 16);
+            v[u] = make_uint4(e[0], e[1], e[2], e[3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + u * kWsWarps * 32;
+        if (i < total) {
+          const int m = i / pieces, p = i - m * pieces;
+          const int grp = p / (G / 8), r = p - grp * (G / 8);
+          const int at = (grp * LW + r % LW) * 4 + r / LW;  // [group][word][quarter]
+          // values 0 4 1 5 2 6 3 7
+          *reinterpret_cast<uint4*>(xsm + m * pitch + at * 16) =
+              make_uint4(__byte_perm(v[u].x, v[u].z, 0x5410), __byte_perm(v[u].x, v[u].z, 0x7632),
+                         __byte_perm(v[u].y, v[u].w, 0x5410), __byte_perm(v[u].y, v[u].w, 0x7632));
+        }
+      }
+    }
   }
   __syncthreads();
-  const int rows = 16 * a.wr;
-  for (int e = tid; e < rows * a.M; e += kW4Warps * 32) {
-    const int col = e / rows, row = e - col * rows;
-    float v = 0.0f;
-    for (int k = 0; k < wk_n; ++k)
-      v += red[((k * a.wr + row / 16) * kCols + col) * 16 + (row & 15)];
-    part[col * rows + row] = v;
-  }
-  if (a.splits > 1) cluster_sync(); else __syncthreads();
-  const float xs_scale = 1.0f;
-  for (int e = tid + kW4Warps * 32 * rank; e < rows * a.M; e += kW4Warps * 32 * a.splits) {
-    const int col = e / rows, row = e - col * rows;
-    const int n = tile * rows + row;
-    float v = 0.0f;
-    if (a.splits > 1) {
-      const uint32_t at = smem_u32(part + col * rows + row);
-      for (int r = 0; r < a.splits; ++r) {
-        float f;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(mapa_shared(at, r)) : "memory");
-        v += f;
+
+  const uint8_t* xs[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)  // columns past M read row M - 1; their results are not used
+    xs[j] = xsm + min(8 * j + g, a.M - 1) * pitch + t * 16;
+  const int swz = rev3(g & 7);
+
+  int slot = 0;
+  for (int tile = tile0; tile < tiles; tile += tile_step) {
+    float acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.0f;
+    for (int st = 0; st < spt; ++st) {
+      cp_async_wait<kWsStages - 2>();
+      __syncwarp();  // the stage has landed for every lane, and the slot read last is free
+      issue();
+      __syncwarp();  // this stage's scales are in place
+      const uint8_t* buf = ring + slot * 2048;
+      const float2* szs = sz + slot * (GS * 16);
+      slot = slot == kWsStages - 1 ? 0 : slot + 1;
+#pragma unroll
+      for (int q = 0; q < GS; ++q) {
+        const int gl = st * GS + q;
+        if (gl >= ng) break;
+        uint32_t wa[LW], wb[LW];
+        w4_words<LW>(buf, g, t, q, swz, wa);
+        w4_words<LW>(buf + 1024, g, t, q, swz, wb);
+        const float2 sa = szs[q * 16 + g], sb = szs[q * 16 + g + 8];
+        float sum[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[j][i] = 0.0f;
+#pragma unroll
+        for (int wi = 0; wi < LW; ++wi) {
+          uint32_t pa[4], pb[4];
+          w4_decode<T>(wa[wi], __float_as_uint(sa.y), pa);
+          w4_decode<T>(wb[wi], __float_as_uint(sb.y), pb);
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            const uint4 xv = *reinterpret_cast<const uint4*>(xs[j] + (gl * LW + wi) * 64);
+            W4Num<T>::mma(sum[j], pa[0], pb[0], pa[1], pb[1], xv.x, xv.y);
+            W4Num<T>::mma(sum[j], pa[2], pb[2], pa[3], pb[3], xv.z, xv.w);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          acc[j][0] = fmaf(sa.x, sum[j][0], acc[j][0]);
+          acc[j][1] = fmaf(sa.x, sum[j][1], acc[j][1]);
+          acc[j][2] = fmaf(sb.x, sum[j][2], acc[j][2]);
+          acc[j][3] = fmaf(sb.x, sum[j][3], acc[j][3]);
+        }
       }
-    } else {
-      v = part[col * rows + row];
     }
-    if (n < a.N) store_out(ep, col, n, epi_scaled(v, 1.0f, 1.0f, xs_scale, ep, n));
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int n = tile * 16 + g + 8 * (i >> 1), m = 8 * j + 2 * t + (i & 1);
+        if (n < a.N && m < a.M) {
+          if (a.part) a.part[(static_cast<int64_t>(slice) * a.M + m) * a.N + n] = acc[j][i];
+          else store_out(ep, m, n, epi_scaled(acc[j][i], 1.0f, 1.0f, 1.0f, ep, n));
+        }
+      }
   }
-  if (a.splits > 1) cluster_sync();  // the other CTAs may still be reading this one's partials
+}
+
+// Adds the slices of each output in order and runs the epilogue.
+__global__ void __launch_bounds__(256) w4_join_kernel(const float* __restrict__ part, int slices, const EpiArgs ep) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t total = static_cast<int64_t>(ep.M) * ep.N;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= total) return;
+  float v = 0.0f;
+#pragma unroll 8
+  for (int s = 0; s < slices; ++s) v += part[s * total + i];
+  const int m = static_cast<int>(i / ep.N), n = static_cast<int>(i - static_cast<int64_t>(m) * ep.N);
+  store_out(ep, m, n, epi_scaled(v, 1.0f, 1.0f, 1.0f, ep, n));
 }
 
 // ---------------------------------------------------------------- few tokens, integer
@@ -318,16 +385,6 @@ struct W4DigitArgs {
   int x_vec;
   int tiles;  // ceil(N / 16)
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ int rev3(int r) { return ((r & 1) << 2) | (r & 2) | ((r >> 2) & 1); }
 
 __device__ __forceinline__ void mma_u8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -535,21 +592,8 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
         const int gl = st * GS + q;
         if (gl >= ng) break;
         uint32_t wa[LW], wb[LW];
-        if constexpr (LW == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(buf + g * 128 + (((q * 4 + t) ^ swz) << 4));
-          const uint4 v = *reinterpret_cast<const uint4*>(buf + 1024 + g * 128 + (((q * 4 + t) ^ swz) << 4));
-          wa[0] = u.x; wa[1] = u.y; wa[2] = u.z; wa[3] = u.w;
-          wb[0] = v.x; wb[1] = v.y; wb[2] = v.z; wb[3] = v.w;
-        } else if constexpr (LW == 2) {
-          const int o = g * 128 + (((q * 2 + (t >> 1)) ^ swz) << 4) + (t & 1) * 8;
-          const uint2 u = *reinterpret_cast<const uint2*>(buf + o), v = *reinterpret_cast<const uint2*>(buf + 1024 + o);
-          wa[0] = u.x; wa[1] = u.y;
-          wb[0] = v.x; wb[1] = v.y;
-        } else {
-          const int o = g * 128 + ((q ^ swz) << 4) + t * 4;
-          wa[0] = *reinterpret_cast<const uint32_t*>(buf + o);
-          wb[0] = *reinterpret_cast<const uint32_t*>(buf + 1024 + o);
-        }
+        w4_words<LW>(buf, g, t, q, swz, wa);
+        w4_words<LW>(buf + 1024, g, t, q, swz, wb);
         int d[NC][4];
 #pragma unroll
         for (int wi = 0; wi < LW; wi += 2) {
