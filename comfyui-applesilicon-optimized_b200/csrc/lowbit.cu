@@ -71,13 +71,14 @@ constexpr int64_t kW4MaxSmallM = 64;
 
 // K slices and row parts of the slice kernel: the split whose busiest warp has the
 // fewest groups to go through, x's slice beside the rings.
+constexpr int kWsMaxSlices = 32;
 struct WsPlan {
   int slices, parts, smem;
 };
-bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
+bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, int max_slices, WsPlan* p) {
   const int64_t KG = K / G, tiles = cdiv(N, 16);
   int64_t best = -1;
-  for (int s = 1; s <= 32 && s <= KG && s <= sms; ++s) {
+  for (int s = 1; s <= max_slices && s <= KG && s <= sms; ++s) {
     const int64_t gs = cdiv(KG, s);
     const int smem = ws_smem_bytes(int(M), int(gs) * G, G);
     if (smem > 227 * 1024) continue;
@@ -94,20 +95,19 @@ bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
   return best >= 0;
 }
 // The slices' sums for one launch of at most 32 tokens.
-size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(32) * (M < 32 ? M : 32) * N * 4; }
+size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(kWsMaxSlices) * (M < 32 ? M : 32) * N * 4; }
 
-template <typename T, int LW>
+template <int LW>
 int launch_slice_cols(const W4SliceArgs& a, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.slices * p.parts));
-  if (a.M <= 8) return launch(w4_slice_kernel<T, LW, 1>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
-  if (a.M <= 16) return launch(w4_slice_kernel<T, LW, 2>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
-  return launch(w4_slice_kernel<T, LW, 4>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  if (a.M <= 8) return launch(w4_slice_kernel<LW, 1>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  if (a.M <= 16) return launch(w4_slice_kernel<LW, 2>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  return launch(w4_slice_kernel<LW, 4>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
 }
-template <typename T>
 int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
-  int s = G == 32   ? launch_slice_cols<T, 1>(a, ep, p, st)
-          : G == 64 ? launch_slice_cols<T, 2>(a, ep, p, st)
-                    : launch_slice_cols<T, 4>(a, ep, p, st);
+  int s = G == 32   ? launch_slice_cols<1>(a, ep, p, st)
+          : G == 64 ? launch_slice_cols<2>(a, ep, p, st)
+                    : launch_slice_cols<4>(a, ep, p, st);
   if (s != B200Q_OK || !a.part) return s;
   const dim3 grid(static_cast<unsigned>(cdiv(int64_t(a.M) * a.N, 256)));
   return launch(w4_join_kernel, grid, 256, 0, 1, st, static_cast<const float*>(a.part), a.slices, ep);
@@ -303,11 +303,12 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   }
   WsPlan ws;
   const int64_t step = M < 32 ? M : 32;
-  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, step, N, K, int(group), &ws)) {
+  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, step, N, K, int(group), need ? kWsMaxSlices : 1, &ws)) {
     for (int64_t m0 = 0; m0 < M; m0 += step) {
       const int64_t rows = M - m0 < step ? M - m0 : step;
       W4SliceArgs a{};
       a.x = static_cast<const uint16_t*>(x) + m0 * ldx;
+      a.x_f16 = x_dtype == B200Q_F16;
       a.ldx = ldx;
       a.w = w;
       a.ldw = ldw;
@@ -324,8 +325,7 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
       EpiArgs e = ep;
       e.M = static_cast<int>(rows);
       e.out = static_cast<char*>(out) + m0 * ldo * (out_dtype == B200Q_F32 ? 4 : 2);
-      const int s = x_dtype == B200Q_F16 ? launch_slice<__half>(a, int(group), e, ws, st)
-                                         : launch_slice<__nv_bfloat16>(a, int(group), e, ws, st);
+      const int s = launch_slice(a, int(group), e, ws, st);
       if (s != B200Q_OK) return s;
     }
     return B200Q_OK;

@@ -7,11 +7,12 @@
 // Mathematics.  Inside a group the scale is a constant, so the group's sum is
 // taken over the exact integers c - z, and one fp32 multiply-add per group
 // joins it to the row's accumulator:  acc += s * sum_{k in group} x_k (c_k - z).
-// c - z is exact in bf16 and fp16: OR-ing a nibble into the mantissa of 128
-// (bf16) or 1024 (fp16) gives 128 + c / 1024 + c, and subtracting 128 + z /
-// 1024 + z is exact.  Products and sums run on warp MMAs (m16n8k16, fp32
-// accumulation) with 16 weight rows as the MMA's rows and 8 tokens as its
-// columns; nothing is rounded before the output.
+// c - z is exact in fp16: OR-ing a nibble into the mantissa of 1024 gives 1024 + c,
+// and subtracting 1024 + z is exact.  Products and sums run on warp MMAs (m16n8k16,
+// fp32 accumulation) with 16 weight rows as the MMA's rows and 8 tokens as its
+// columns.  A bf16 token row is scaled by the power of two of its largest |x| and is
+// then exact in fp16 down to 2^-17 of it, within 2^-25 of it below; nothing else is
+// rounded before the output.
 //
 // Layout.  The order of k inside a group is free as long as both operands
 // agree.  Lane (g, t) = (lane / 4, lane % 4) takes the G/4 codes of its quarter t
@@ -21,6 +22,8 @@
 // load feeds two MMAs, and the row pitch is 64 modulo 128 bytes, which makes those
 // loads free of bank conflicts.  Few tokens take an integer form of the same sums.
 #pragma once
+
+#include <type_traits>
 
 #include "digits.cuh"
 #include "numerics.cuh"
@@ -72,51 +75,43 @@ __device__ __forceinline__ void w4_words(const uint8_t* buf, int g, int t, int q
   }
 }
 
-template <typename T>
-struct W4Num;
-template <>
-struct W4Num<__nv_bfloat16> {
-  static constexpr bool kF16 = false;
-  static constexpr uint32_t kMagic = 0x43004300u;  // 128, 128
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
-                                     *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                             uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
-template <>
-struct W4Num<__half> {
-  static constexpr bool kF16 = true;
-  static constexpr uint32_t kMagic = 0x64006400u;  // 1024, 1024
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
-                              *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                             uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
-        "{%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-};
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same with a zero accumulator.
+__device__ __forceinline__ void mma_f16_start(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                              uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// (a & mask) | bits in one instruction (the compiler makes two of it).
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
+// A row's zero point for w4_decode: 1024 + z (low half) and -(64 + z) as fp16.
+__device__ __forceinline__ uint32_t w4_zero(uint32_t z) { return 0xD4006400u | (z << 20) | z; }
 
-// The four exact pairs (c_i - z, c_{i+4} - z) of one 8-code word; zp = magic | z.
-template <typename T>
-__device__ __forceinline__ void w4_decode(uint32_t w, uint32_t zp, uint32_t (&p)[4]) {
+// The four exact fp16 pairs (c_i - z, c_{i+4} - z) of one 8-code word, from its row's
+// pairs z0 = (1024 + z) twice and z1 = -(64 + z) twice: a low nibble OR-ed into 1024
+// is 1024 + c, the nibble above it 1024 + 16 c (one shift per word).
+__device__ __forceinline__ void w4_decode(uint32_t w, uint32_t z0, uint32_t z1, uint32_t (&p)[4]) {
+  const uint32_t m = 0x64006400u, sixteenth = 0x2C002C00u;
+  const uint32_t v = w >> 8;
+  const uint32_t a[4] = {and_or(w, 0x000F000Fu, m), and_or(w, 0x00F000F0u, m), and_or(v, 0x000F000Fu, m),
+                         and_or(v, 0x00F000F0u, m)};
+  const __half2 h0 = *reinterpret_cast<const __half2*>(&z0), h1 = *reinterpret_cast<const __half2*>(&z1);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    p[i] = W4Num<T>::sub(((w >> (4 * i)) & 0x000F000Fu) | W4Num<T>::kMagic, zp);
+  for (int i = 0; i < 4; ++i) {
+    const __half2 x = *reinterpret_cast<const __half2*>(&a[i]);
+    const __half2 r = i & 1 ? __hfma2(x, *reinterpret_cast<const __half2*>(&sixteenth), h1) : __hsub2(x, h0);
+    p[i] = *reinterpret_cast<const uint32_t*>(&r);
+  }
 }
 
 // ---------------------------------------------------------------- up to 32 tokens
@@ -132,6 +127,7 @@ constexpr int kWsStages = 3;  // issue() relies on three
 struct W4SliceArgs {
   const void* x;         // [M, K] bf16 / fp16
   int64_t ldx;           // elements
+  int x_f16;
   const uint8_t* w;      // [N, K / 2]
   int64_t ldw;           // bytes
   const void* scales;    // [N, K / G]
@@ -150,9 +146,10 @@ __host__ __device__ __forceinline__ int ws_smem_bytes(int M, int k_slice, int G)
 }
 
 // LW = G / 32 words per lane, row and group; NT = 8-token columns.
-template <typename T, int LW, int NT>
+template <int LW, int NT>
 __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceArgs a, const EpiArgs ep) {
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float x_pow[8 * NT];
   constexpr int G = 32 * LW;
   constexpr int GS = 8 / LW;  // groups per stage
   constexpr int SL = GS / 2;
@@ -191,7 +188,7 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
 #pragma unroll
       for (int k = 0; k < SL; ++k) {
         to[lane + 32 * k] = make_float2(scale_value(s_next[1][k], a.scale_dtype),
-                                          __uint_as_float(W4Num<T>::kMagic | (z_next[1][k] & 15u) * 0x00010001u));
+                                          __uint_as_float(w4_zero(z_next[1][k] & 15u)));
         s_next[1][k] = s_next[0][k];
         z_next[1][k] = z_next[0][k];
       }
@@ -226,38 +223,59 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
 #pragma unroll
   for (int i = 0; i < kWsStages - 1; ++i) issue();
 
-  // ---- stage x[:, slice] in fragment order, four pieces of 8 values at a time
+  // ---- stage x[:, slice] in fragment order: warp w takes tokens w, w + 16, ...; four
+  // pieces of 8 values per lane at a time
   {
-    const int pieces = ng * (G / 8), total = pieces * a.M;
-    for (int i0 = tid; i0 < total; i0 += 4 * kWsWarps * 32) {
-      uint4 v[4];
+    const int pieces = ng * (G / 8);
+    for (int m = warp; m < a.M; m += kWsWarps) {
+      const uint16_t* row = static_cast<const uint16_t*>(a.x) + m * a.ldx + int64_t(g0) * G;
+      auto load = [&](int p) {
+        if (a.x_vec) return __ldg(reinterpret_cast<const uint4*>(row + p * 8));
+        uint32_t e[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kWsWarps * 32;
-        if (i < total) {
-          const int m = i / pieces, p = i - m * pieces;
-          const uint16_t* src = static_cast<const uint16_t*>(a.x) + m * a.ldx + int64_t(g0) * G + p * 8;
-          if (a.x_vec) {
-            v[u] = __ldg(reinterpret_cast<const uint4*>(src));
-          } else {
-            uint32_t e[4];
+        for (int j = 0; j < 4; ++j) e[j] = __ldg(row + p * 8 + 2 * j) | (uint32_t(__ldg(row + p * 8 + 2 * j + 1)) << 16);
+        return make_uint4(e[0], e[1], e[2], e[3]);
+      };
+      float inv = 1.0f, pow = 1.0f;
+      if (!a.x_f16) {  // the power of two of the largest |x| of the slice
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int p = lane; p < pieces; p += 32) {
+          const uint4 v = load(p);
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = __ldg(src + 2 * j) | (uint32_t(__ldg(src + 2 * j + 1)) << 16);
-            v[u] = make_uint4(e[0], e[1], e[2], e[3]);
-          }
+          for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
         }
-      }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int i = i0 + u * kWsWarps * 32;
-        if (i < total) {
-          const int m = i / pieces, p = i - m * pieces;
-          const int grp = p / (G / 8), r = p - grp * (G / 8);
-          const int at = (grp * LW + r % LW) * 4 + r / LW;  // [group][word][quarter]
-          // values 0 4 1 5 2 6 3 7
-          *reinterpret_cast<uint4*>(xsm + m * pitch + at * 16) =
-              make_uint4(__byte_perm(v[u].x, v[u].z, 0x5410), __byte_perm(v[u].x, v[u].z, 0x7632),
-                         __byte_perm(v[u].y, v[u].w, 0x5410), __byte_perm(v[u].y, v[u].w, 0x7632));
+        for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        int ex = static_cast<int>(top >> 7);
+        ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+        inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+        pow = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+      }
+      if (lane == 0) x_pow[m] = pow;
+      for (int p0 = lane; p0 < pieces; p0 += 128) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (p0 + 32 * u < pieces) v[u] = load(p0 + 32 * u);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int p = p0 + 32 * u;
+          if (p < pieces) {
+            uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            if (!a.x_f16) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                e[j] = pack_f16x2(__uint_as_float(e[j] << 16) * inv, __uint_as_float(e[j] & 0xFFFF0000u) * inv);
+            }
+            const int grp = p / (G / 8), r = p % (G / 8);
+            const int at = (grp * LW + r % LW) * 4 + r / LW;  // [group][word][quarter]
+            // values 0 4 1 5 2 6 3 7
+            *reinterpret_cast<uint4*>(xsm + m * pitch + at * 16) =
+                make_uint4(__byte_perm(e[0], e[2], 0x5410), __byte_perm(e[0], e[2], 0x7632),
+                           __byte_perm(e[1], e[3], 0x5410), __byte_perm(e[1], e[3], 0x7632));
+          }
         }
       }
     }
@@ -293,21 +311,21 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
         w4_words<LW>(buf, g, t, q, swz, wa);
         w4_words<LW>(buf + 1024, g, t, q, swz, wb);
         const float2 sa = szs[q * 16 + g], sb = szs[q * 16 + g + 8];
+        const uint32_t za = __float_as_uint(sa.y), zb = __float_as_uint(sb.y);
+        const uint32_t za0 = __byte_perm(za, 0, 0x1010), za1 = __byte_perm(za, 0, 0x3232);
+        const uint32_t zb0 = __byte_perm(zb, 0, 0x1010), zb1 = __byte_perm(zb, 0, 0x3232);
         float sum[NT][4];
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sum[j][i] = 0.0f;
 #pragma unroll
         for (int wi = 0; wi < LW; ++wi) {
           uint32_t pa[4], pb[4];
-          w4_decode<T>(wa[wi], __float_as_uint(sa.y), pa);
-          w4_decode<T>(wb[wi], __float_as_uint(sb.y), pb);
+          w4_decode(wa[wi], za0, za1, pa);
+          w4_decode(wb[wi], zb0, zb1, pb);
 #pragma unroll
           for (int j = 0; j < NT; ++j) {
             const uint4 xv = *reinterpret_cast<const uint4*>(xs[j] + (gl * LW + wi) * 64);
-            W4Num<T>::mma(sum[j], pa[0], pb[0], pa[1], pb[1], xv.x, xv.y);
-            W4Num<T>::mma(sum[j], pa[2], pb[2], pa[3], pb[3], xv.z, xv.w);
+            if (wi == 0) mma_f16_start(sum[j], pa[0], pb[0], pa[1], pb[1], xv.x, xv.y);
+            else mma_f16(sum[j], pa[0], pb[0], pa[1], pb[1], xv.x, xv.y);
+            mma_f16(sum[j], pa[2], pb[2], pa[3], pb[3], xv.z, xv.w);
           }
         }
 #pragma unroll
@@ -325,8 +343,9 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
       for (int i = 0; i < 4; ++i) {
         const int n = tile * 16 + g + 8 * (i >> 1), m = 8 * j + 2 * t + (i & 1);
         if (n < a.N && m < a.M) {
-          if (a.part) a.part[(static_cast<int64_t>(slice) * a.M + m) * a.N + n] = acc[j][i];
-          else store_out(ep, m, n, epi_scaled(acc[j][i], 1.0f, 1.0f, 1.0f, ep, n));
+          const float v = acc[j][i] * x_pow[m];
+          if (a.part) a.part[(static_cast<int64_t>(slice) * a.M + m) * a.N + n] = v;
+          else store_out(ep, m, n, epi_scaled(v, 1.0f, 1.0f, 1.0f, ep, n));
         }
       }
   }
@@ -526,7 +545,7 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 #pragma unroll
       for (int o = LG / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       float down, up;
-      digit_scale(top, W4Num<T>::kF16, &down, &up);
+      digit_scale(top, std::is_same<T, __half>::value, &down, &up);
       int sum[3] = {0, 0, 0};
 #pragma unroll
       for (int wv = 0; wv < EL / 8; ++wv) {  // one 8-code word: digits of codes 0 2 4 6 | 1 3 5 7
