@@ -223,29 +223,46 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
 #pragma unroll
   for (int i = 0; i < kWsStages - 1; ++i) issue();
 
-  // ---- stage x[:, slice] in fragment order: warp w takes tokens w, w + 16, ...; four
-  // pieces of 8 values per lane at a time
+  // ---- stage x[:, slice] in fragment order: warp w takes tokens w, w + 16, ..., 256
+  // pieces of 8 values (8 per lane, all in flight) at a time.  A bf16 row longer than
+  // that is read once more, for its largest |x|.
   {
     const int pieces = ng * (G / 8);
     for (int m = warp; m < a.M; m += kWsWarps) {
       const uint16_t* row = static_cast<const uint16_t*>(a.x) + m * a.ldx + int64_t(g0) * G;
-      auto load = [&](int p) {
-        if (a.x_vec) return __ldg(reinterpret_cast<const uint4*>(row + p * 8));
-        uint32_t e[4];
+      uint4 v[8];
+      auto load = [&](int p0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = __ldg(row + p * 8 + 2 * j) | (uint32_t(__ldg(row + p * 8 + 2 * j + 1)) << 16);
-        return make_uint4(e[0], e[1], e[2], e[3]);
-      };
-      float inv = 1.0f, pow = 1.0f;
-      if (!a.x_f16) {  // the power of two of the largest |x| of the slice
-        uint32_t top = 0;
-#pragma unroll 4
-        for (int p = lane; p < pieces; p += 32) {
-          const uint4 v = load(p);
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + 32 * u + lane;
+          v[u] = make_uint4(0, 0, 0, 0);
+          if (p < pieces) {
+            if (a.x_vec) {
+              v[u] = __ldg(reinterpret_cast<const uint4*>(row + p * 8));
+            } else {
+              uint32_t e[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
+              for (int j = 0; j < 4; ++j) e[j] = __ldg(row + p * 8 + 2 * j) | (uint32_t(__ldg(row + p * 8 + 2 * j + 1)) << 16);
+              v[u] = make_uint4(e[0], e[1], e[2], e[3]);
+            }
+          }
         }
+      };
+      load(0);
+      float inv = 1.0f, pow = 1.0f;
+      if (!a.x_f16) {
+        uint32_t top = 0;
+        for (int p0 = 0;;) {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = max(top, max(e[j] & 0x7FFFu, (e[j] >> 16) & 0x7FFFu));
+          }
+          if ((p0 += 256) >= pieces) break;
+          load(p0);
+        }
+        if (pieces > 256) load(0);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         int ex = static_cast<int>(top >> 7);
@@ -254,14 +271,10 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
         pow = __uint_as_float(static_cast<uint32_t>(ex) << 23);
       }
       if (lane == 0) x_pow[m] = pow;
-      for (int p0 = lane; p0 < pieces; p0 += 128) {
-        uint4 v[4];
+      for (int p0 = 0;;) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (p0 + 32 * u < pieces) v[u] = load(p0 + 32 * u);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int p = p0 + 32 * u;
+        for (int u = 0; u < 8; ++u) {
+          const int p = p0 + 32 * u + lane;
           if (p < pieces) {
             uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
             if (!a.x_f16) {
@@ -277,6 +290,8 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
                            __byte_perm(e[1], e[3], 0x5410), __byte_perm(e[1], e[3], 0x7632));
           }
         }
+        if ((p0 += 256) >= pieces) break;
+        load(p0);
       }
     }
   }
