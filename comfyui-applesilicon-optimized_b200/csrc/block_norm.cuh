@@ -9,9 +9,19 @@
 // A row stays in fp32 registers from its one load to its one store: the second
 // norm and the quantization take the unrounded h and out, so each stored value
 // is rounded once.  The variance is centred (a second pass over registers, not
-// sum(v^2) - mean^2, which cancels for rows with a large mean).
+// sum(v^2) - mean^2, which cancels for rows with a large mean): each warp centres its
+// values on its own mean, and the warps' means and squares are joined by
+//   D var = sum_w [ M2_w + n_w (mean_w - mean)^2 ],
+// so one barrier per norm is enough.
+//
+// Bound: HBM.  Wan-shaped rows (65,520 x 5,120 bf16, 2.68 GB with h and out written)
+// run persistent CTAs: a CTA's rows share their modulation, which is folded once into
+// three fp32 vectors in shared memory (gate * post_w, w * (1 + scale), shift) instead
+// of being read again from L2 for every row, and the next row's loads are in flight
+// while one is reduced.
 #pragma once
 
+#include "digits.cuh"
 #include "numerics.cuh"
 #include "ptx.cuh"
 
@@ -105,7 +115,8 @@ __device__ __forceinline__ void store_vals16(void* p, int dtype, int64_t i, cons
   }
 }
 
-// One CTA per row; thread i holds vectors i, i + threads, ... (NPT of VEC values).
+// One CTA per row; thread i holds values i, i + threads, ...  The form for any D,
+// stride and alignment.
 template <int DTYPE, int VEC, int NPT>
 __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
   __shared__ float bufs[2][32];
@@ -219,6 +230,240 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
     else
       a.q[row * a.ldq + c] = o[0];
   });
+}
+
+// ---------------------------------------------------------------- aligned rows
+// Rows of 8-value vectors, NPT per thread (16-byte aligned operands): thread i holds
+// vectors i, i + threads, ...; absent ones are zeros.  inv_n_w: 1 / this warp's values, n_l:
+// those of warp `lane`; buf: one pair of 32 words per norm in flight.
+template <int NPT, bool FULL>
+__device__ __forceinline__ void row_norm(float (&v)[NPT][8], int kind, const bool (&on)[NPT], float inv_n_w, float n_l,
+                                         float inv_n_l, float inv_d, float eps, float (*buf)[32]) {
+  if (kind == kNormNone) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const bool layer = kind == kNormLayer;
+  float mean_w = 0.0f, s = 0.0f;
+  if (layer) {
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += v[k][j];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    mean_w = s * inv_n_w;
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int k = 0; k < NPT; ++k)
+    if (FULL || on[k]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q = fmaf(v[k][j] - mean_w, v[k][j] - mean_w, q);
+    }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+  if (lane == 0) {
+    buf[0][warp] = s;
+    buf[1][warp] = q;
+  }
+  __syncthreads();
+  // every warp joins all warps: lane w has warp w's sums
+  float mean = 0.0f, sq = lane < warps ? buf[1][lane] : 0.0f;
+  if (layer) {
+    const float sw = lane < warps ? buf[0][lane] : 0.0f;
+    mean = sw;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+    mean *= inv_d;
+    const float d = fmaf(sw, inv_n_l, -mean);
+    if (lane < warps) sq = fmaf(n_l * d, d, sq);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  const float r = rsqrtf(fmaf(sq, inv_d, eps));
+#pragma unroll
+  for (int k = 0; k < NPT; ++k)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[k][j] = (v[k][j] - mean) * r;
+}
+
+template <int DTYPE>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+  const uint32_t uv[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (DTYPE == kBiasBF16) {
+      v[2 * j] = __uint_as_float(uv[j] << 16);
+      v[2 * j + 1] = __uint_as_float(uv[j] & 0xFFFF0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&uv[j]));
+      v[2 * j] = f.x;
+      v[2 * j + 1] = f.y;
+    }
+  }
+}
+// The three vectors of 8 columns at c for modulation row `mod`: gate * post_w, w *
+// (1 + scale), shift.
+__device__ __forceinline__ void fold_mods(const NormArgs& a, int64_t mod, int c, float (&g)[8], float (&w)[8], float (&b)[8]) {
+  float u[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    g[j] = w[j] = 1.0f;
+    b[j] = 0.0f;
+  }
+  if (a.post_w) load_vals<8>(a.post_w, a.post_w_dtype, c, g);
+  if (a.gate) {
+    load_vals<8>(a.gate, a.mod_dtype, mod * a.ld_gate + c, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] *= u[j];
+  }
+  if (a.w) load_vals<8>(a.w, a.w_dtype, c, w);
+  if (a.scale) {
+    load_vals<8>(a.scale, a.mod_dtype, mod * a.ld_scale + c, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] *= 1.0f + u[j];
+  }
+  if (a.shift) load_vals<8>(a.shift, a.mod_dtype, mod * a.ld_shift + c, b);
+}
+
+// PERSIST: CTAs loop over contiguous rows, the folded vectors in shared memory ([3][D]
+// floats, a thread writes and reads its own columns).  Otherwise one row per CTA, one
+// vector per thread, every load in flight at once.  FULL: no thread has an absent
+// vector.
+template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT>
+__global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) float folded[];
+  __shared__ float bufs[3][2][32];
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const float inv_d = 1.0f / static_cast<float>(a.D);
+  int col[NPT];
+  bool on[NPT];
+  int nw = 0, nl = 0;
+#pragma unroll
+  for (int k = 0; k < NPT; ++k) {
+    col[k] = (threadIdx.x + k * blockDim.x) * 8;
+    on[k] = col[k] < a.D;
+    nw += min(max(a.D - static_cast<int>(k * blockDim.x + warp * 32) * 8, 0), 256);
+    nl += min(max(a.D - static_cast<int>(k * blockDim.x + lane * 32) * 8, 0), 256);
+  }
+  const float n_l = static_cast<float>(max(nl, 1)), inv_n_l = 1.0f / n_l, inv_n_w = 1.0f / static_cast<float>(max(nw, 1));
+  const int64_t r0 = PERSIST ? static_cast<int64_t>(a.rows) * blockIdx.x / gridDim.x : blockIdx.x;
+  const int64_t r1 = PERSIST ? static_cast<int64_t>(a.rows) * (blockIdx.x + 1) / gridDim.x : r0 + 1;
+  uint4 xn[NPT], yn[NPT];  // the row after this one
+  const uint16_t* xp = static_cast<const uint16_t*>(a.x) + r0 * a.ldx;
+  const uint16_t* yp = static_cast<const uint16_t*>(a.y) + r0 * a.ldy;
+  auto fetch = [&]() {
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) {
+      xn[k] = yn[k] = make_uint4(0, 0, 0, 0);
+      if (FULL || on[k]) {
+        xn[k] = __ldg(reinterpret_cast<const uint4*>(xp + col[k]));
+        if (a.y) yn[k] = __ldg(reinterpret_cast<const uint4*>(yp + col[k]));
+      }
+    }
+    xp += a.ldx;
+    yp += a.ldy;
+  };
+  if (r0 < r1) fetch();
+  int64_t mod_end = r0;  // the first row that needs other vectors
+  float g[8], w[8], b[8];  // (not PERSIST) the folded vectors
+  char* hp = static_cast<char*>(a.h) + r0 * a.ldh * 2;
+  char* op = static_cast<char*>(a.out) + r0 * a.ldo * 2;
+  for (int64_t row = r0; row < r1; ++row, hp += a.ldh * 2, op += a.ldo * 2) {
+    uint4 x0[NPT], y0[NPT];
+#pragma unroll
+    for (int k = 0; k < NPT; ++k) {
+      x0[k] = xn[k];
+      y0[k] = yn[k];
+    }
+    if (row + 1 < r1) fetch();
+    if (row >= mod_end) {
+      const int64_t mod = row / a.rows_per_mod;
+      mod_end = (mod + 1) * a.rows_per_mod;
+#pragma unroll
+      for (int k = 0; k < NPT; ++k)
+        if (FULL || on[k]) {
+          fold_mods(a, mod, col[k], g, w, b);
+          if (PERSIST) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+              *reinterpret_cast<float4*>(folded + col[k] + j) = make_float4(g[j], g[j + 1], g[j + 2], g[j + 3]);
+              *reinterpret_cast<float4*>(folded + a.D + col[k] + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
+              *reinterpret_cast<float4*>(folded + 2 * a.D + col[k] + j) = make_float4(b[j], b[j + 1], b[j + 2], b[j + 3]);
+            }
+          }
+        }
+    }
+    auto vec = [&](int which, int c, float (&u)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(folded + which * a.D + c + j);
+        u[j] = f.x; u[j + 1] = f.y; u[j + 2] = f.z; u[j + 3] = f.w;
+      }
+    };
+    float v[NPT][8];
+    if (a.y) {
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(y0[k], v[k]);
+      row_norm<NPT, FULL>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[0]);
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) {
+        if (FULL || on[k]) {
+          float u[8];
+          unpack8<DTYPE>(x0[k], u);
+          if (PERSIST) vec(0, col[k], g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = fmaf(a.res_scale, u[j], v[k][j] * g[j]);
+          if (a.h) store_vals16<8>(hp, DTYPE, col[k], v[k]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[k][j] = 0.0f;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(x0[k], v[k]);
+    }
+    if (!a.out && !a.q) continue;
+    row_norm<NPT, FULL>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[1]);
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+      if (FULL || on[k]) {
+        if (PERSIST) {
+          vec(1, col[k], w);
+          vec(2, col[k], b);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[k][j] = fmaf(v[k][j], w[j], b[j]);
+          if (QUANT) top = max(top, __float_as_uint(v[k][j]) & 0x7FFFFFFFu);  // as bits: NaN sorts above
+        }
+        if (!QUANT) store_vals16<8>(op, DTYPE, col[k], v[k]);
+      }
+    if (!QUANT) continue;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) bufs[2][row & 1][warp] = __uint_as_float(top);
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(bufs[2][row & 1][lane]) : 0u);
+    // a row holding inf or NaN gets a NaN scale
+    const float t = __uint_as_float(top);
+    const float s = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);
+    if (threadIdx.x == 0) a.q_scale[row] = s;
+    // out / s as a product with 1 / s, within 2^-23 of the quotient; the nearest integer
+    // is the low byte of the sum with 1.5 * 2^23 (at most 127 in magnitude)
+    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+      if (FULL || on[k]) {
+        uint32_t o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(fmaf(v[k][j], inv, 12582912.0f));
+        *reinterpret_cast<uint2*>(a.q + row * a.ldq + col[k]) =
+            make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));
+      }
+  }
 }
 
 }  // namespace b200q

@@ -163,20 +163,40 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
   return o;
 }
 
-int norm_threads(int64_t D, int vec, int npt) {
-  const int64_t t = cdiv(cdiv(D, vec), npt);
-  return static_cast<int>(cdiv(t, 32) * 32);
+template <int DTYPE, bool PERSIST, int NPT>
+int launch_norm_rows(const NormArgs& a, dim3 grid, int threads, int smem, cudaStream_t st) {
+  const bool full = threads * NPT * 8 == a.D;
+  if (a.q) return full ? launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, true, true>, grid, threads, smem, 1, st, a)
+                       : launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, false, true>, grid, threads, smem, 1, st, a);
+  return full ? launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, true, false>, grid, threads, smem, 1, st, a)
+              : launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, false, false>, grid, threads, smem, 1, st, a);
 }
+// Aligned rows of up to 8192 values: one row per CTA and one 8-value vector per thread
+// while all rows find a place at once, else persistent CTAs with four vectors per
+// thread (two for short rows: fewer reductions per value, more CTAs per SM).  Anything
+// else takes the form that holds 8 or 32 single values per thread.
 template <int DTYPE>
-int launch_norm(const NormArgs& a, bool vec, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(a.rows));
-  if (vec) {
-    if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 8, 1>, grid, norm_threads(a.D, 8, 1), 0, 1, st, a);
-    if (a.D <= 8 * 1024) return launch(block_norm_kernel<DTYPE, 8, 2>, grid, norm_threads(a.D, 8, 2), 0, 1, st, a);
-    return launch(block_norm_kernel<DTYPE, 8, 4>, grid, norm_threads(a.D, 8, 4), 0, 1, st, a);
+int launch_norm(const NormArgs& a, bool vec, int sms, cudaStream_t st) {
+  const dim3 rows(static_cast<unsigned>(a.rows));
+  if (vec && a.D <= 8192) {
+    const int vecs = a.D / 8;
+    if (a.rows <= 2 * int64_t(sms))
+      return launch_norm_rows<DTYPE, false, 1>(a, rows, static_cast<int>(cdiv(vecs, 32) * 32), 0, st);
+    // the vectors per thread that leave the fewest lanes idle
+    const int npt = cdiv(vecs, 4 * 32) * 4 <= cdiv(vecs, 2 * 32) * 2 ? 4 : 2;
+    const int threads = static_cast<int>(cdiv(vecs, npt * 32) * 32);
+    const int smem = 3 * a.D * 4;
+    int per_sm = 65536 / (threads * (npt == 4 ? 128 : 80));  // by registers, then by shared memory
+    if (per_sm > 220 * 1024 / (smem + 2048)) per_sm = 220 * 1024 / (smem + 2048);
+    if (per_sm > 16) per_sm = 16;
+    if (per_sm < 1) per_sm = 1;
+    const dim3 grid(static_cast<unsigned>(a.rows < int64_t(sms) * per_sm ? a.rows : sms * per_sm));
+    return npt == 4 ? launch_norm_rows<DTYPE, true, 4>(a, grid, threads, smem, st)
+                    : launch_norm_rows<DTYPE, true, 2>(a, grid, threads, smem, st);
   }
-  if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 1, 8>, grid, norm_threads(a.D, 1, 8), 0, 1, st, a);
-  return launch(block_norm_kernel<DTYPE, 1, 32>, grid, norm_threads(a.D, 1, 32), 0, 1, st, a);
+  auto threads = [&](int npt) { return static_cast<int>(cdiv(cdiv(a.D, npt), 32) * 32); };
+  if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 1, 8>, rows, threads(8), 0, 1, st, a);
+  return launch(block_norm_kernel<DTYPE, 1, 32>, rows, threads(32), 0, 1, st, a);
 }
 
 // ------------------------------------------------------------ 8-bit cache
@@ -375,7 +395,8 @@ int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int
     return B200Q_ERR_INVALID;
   if (rows == 0) return B200Q_OK;
   if (!x || (!out && !q && !h)) return B200Q_ERR_INVALID;
-  if (!host::device_sms()) return B200Q_ERR_UNSUPPORTED;
+  const int sms = host::device_sms();
+  if (!sms) return B200Q_ERR_UNSUPPORTED;
   NormArgs a{};
   a.x = x; a.ldx = ldx; a.y = y; a.ldy = ldy;
   a.post_w = post_w; a.post_w_dtype = post_w_dtype;
@@ -394,7 +415,7 @@ int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int
                    ok(gate, ld_gate) && ok(scale, ld_scale) && ok(shift, ld_shift) &&
                    ok(post_w, 0) && ok(w, 0) && (!q || (aligned(q, 8) && ldq % 8 == 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == B200Q_F16 ? launch_norm<kBiasF16>(a, vec, st) : launch_norm<kBiasBF16>(a, vec, st);
+  return dtype == B200Q_F16 ? launch_norm<kBiasF16>(a, vec, sms, st) : launch_norm<kBiasBF16>(a, vec, sms, st);
 }
 
 int b200q_kv8_append(const void* k, const void* v, int dtype, int64_t B, int64_t S,
