@@ -325,18 +325,20 @@ __device__ __forceinline__ void fold_mods(const NormArgs& a, int64_t mod, int c,
   if (a.shift) load_vals<8>(a.shift, a.mod_dtype, mod * a.ld_shift + c, b);
 }
 
-// PERSIST: CTAs loop over contiguous rows, the folded vectors in shared memory ([3][D]
-// floats, a thread writes and reads its own columns).  Otherwise one row per CTA, one
+// PERSIST: CTAs loop over contiguous rows, the folded vectors in shared memory (AFTER 3,
+// else 2; a thread writes and reads its own columns; the first four values of all
+// vectors, then the other four, so that neighbouring threads read neighbouring words).  Otherwise one row per CTA, one
 // vector per thread, every load in flight at once.  FULL: no thread has an absent
 // vector.
-template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT>
+template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
 __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(const NormArgs a) {
-  extern __shared__ __align__(16) float folded[];
+  extern __shared__ float4 folded[];
   __shared__ float bufs[3][2][32];
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const float inv_d = 1.0f / static_cast<float>(a.D);
+  const int nv = a.D >> 3;
   int col[NPT];
   bool on[NPT];
   int nw = 0, nl = 0;
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
       xn[k] = yn[k] = make_uint4(0, 0, 0, 0);
       if (FULL || on[k]) {
         xn[k] = __ldg(reinterpret_cast<const uint4*>(xp + col[k]));
-        if (a.y) yn[k] = __ldg(reinterpret_cast<const uint4*>(yp + col[k]));
+        if (AFTER) yn[k] = __ldg(reinterpret_cast<const uint4*>(yp + col[k]));
       }
     }
     xp += a.ldx;
@@ -386,24 +388,25 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
         if (FULL || on[k]) {
           fold_mods(a, mod, col[k], g, w, b);
           if (PERSIST) {
+            float4* f = folded + (col[k] >> 3);
 #pragma unroll
-            for (int j = 0; j < 8; j += 4) {
-              *reinterpret_cast<float4*>(folded + col[k] + j) = make_float4(g[j], g[j + 1], g[j + 2], g[j + 3]);
-              *reinterpret_cast<float4*>(folded + a.D + col[k] + j) = make_float4(w[j], w[j + 1], w[j + 2], w[j + 3]);
-              *reinterpret_cast<float4*>(folded + 2 * a.D + col[k] + j) = make_float4(b[j], b[j + 1], b[j + 2], b[j + 3]);
+            for (int j = 0; j < 2; ++j) {
+              f[j * nv] = make_float4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+              f[(2 + j) * nv] = make_float4(b[4 * j], b[4 * j + 1], b[4 * j + 2], b[4 * j + 3]);
+              if (AFTER) f[(4 + j) * nv] = make_float4(g[4 * j], g[4 * j + 1], g[4 * j + 2], g[4 * j + 3]);
             }
           }
         }
     }
     auto vec = [&](int which, int c, float (&u)[8]) {
 #pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const float4 f = *reinterpret_cast<const float4*>(folded + which * a.D + c + j);
-        u[j] = f.x; u[j + 1] = f.y; u[j + 2] = f.z; u[j + 3] = f.w;
+      for (int j = 0; j < 2; ++j) {
+        const float4 f = folded[(2 * which + j) * nv + (c >> 3)];
+        u[4 * j] = f.x; u[4 * j + 1] = f.y; u[4 * j + 2] = f.z; u[4 * j + 3] = f.w;
       }
     };
     float v[NPT][8];
-    if (a.y) {
+    if (AFTER) {
 #pragma unroll
       for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(y0[k], v[k]);
       row_norm<NPT, FULL>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[0]);
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
         if (FULL || on[k]) {
           float u[8];
           unpack8<DTYPE>(x0[k], u);
-          if (PERSIST) vec(0, col[k], g);
+          if (PERSIST) vec(2, col[k], g);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[k][j] = fmaf(a.res_scale, u[j], v[k][j] * g[j]);
           if (a.h) store_vals16<8>(hp, DTYPE, col[k], v[k]);
@@ -425,15 +428,15 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
 #pragma unroll
       for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(x0[k], v[k]);
     }
-    if (!a.out && !a.q) continue;
+    if (!QUANT && !a.out) continue;
     row_norm<NPT, FULL>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[1]);
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
       if (FULL || on[k]) {
         if (PERSIST) {
-          vec(1, col[k], w);
-          vec(2, col[k], b);
+          vec(0, col[k], w);
+          vec(1, col[k], b);
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {

@@ -163,13 +163,32 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
   return o;
 }
 
+// PERSIST: as many CTAs as are resident at once (at most one per row).
+template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
+int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
+  auto kern = block_norm_rows_kernel<DTYPE, PERSIST, NPT, FULL, QUANT, AFTER>;
+  if (!PERSIST) return launch(kern, dim3(static_cast<unsigned>(a.rows)), threads, 0, 1, st, a);
+  const int smem = (AFTER ? 3 : 2) * a.D * 4;
+  int per_sm = 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
+    cudaGetLastError();
+    return B200Q_ERR_CUDA;
+  }
+  const int64_t ctas = int64_t(sms) * per_sm;
+  return launch(kern, dim3(static_cast<unsigned>(a.rows < ctas ? a.rows : ctas)), threads, smem, 1, st, a);
+}
+template <int DTYPE, bool PERSIST, int NPT, bool FULL>
+int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
+  if (a.y) return a.q ? launch_norm_rows<DTYPE, PERSIST, NPT, FULL, true, true>(a, threads, sms, st)
+                      : launch_norm_rows<DTYPE, PERSIST, NPT, FULL, false, true>(a, threads, sms, st);
+  return a.q ? launch_norm_rows<DTYPE, PERSIST, NPT, FULL, true, false>(a, threads, sms, st)
+             : launch_norm_rows<DTYPE, PERSIST, NPT, FULL, false, false>(a, threads, sms, st);
+}
 template <int DTYPE, bool PERSIST, int NPT>
-int launch_norm_rows(const NormArgs& a, dim3 grid, int threads, int smem, cudaStream_t st) {
-  const bool full = threads * NPT * 8 == a.D;
-  if (a.q) return full ? launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, true, true>, grid, threads, smem, 1, st, a)
-                       : launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, false, true>, grid, threads, smem, 1, st, a);
-  return full ? launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, true, false>, grid, threads, smem, 1, st, a)
-              : launch(block_norm_rows_kernel<DTYPE, PERSIST, NPT, false, false>, grid, threads, smem, 1, st, a);
+int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
+  return threads * NPT * 8 == a.D ? launch_norm_rows<DTYPE, PERSIST, NPT, true>(a, threads, sms, st)
+                                  : launch_norm_rows<DTYPE, PERSIST, NPT, false>(a, threads, sms, st);
 }
 // Aligned rows of up to 8192 values: one row per CTA and one 8-value vector per thread
 // while all rows find a place at once, else persistent CTAs with four vectors per
@@ -181,18 +200,12 @@ int launch_norm(const NormArgs& a, bool vec, int sms, cudaStream_t st) {
   if (vec && a.D <= 8192) {
     const int vecs = a.D / 8;
     if (a.rows <= 2 * int64_t(sms))
-      return launch_norm_rows<DTYPE, false, 1>(a, rows, static_cast<int>(cdiv(vecs, 32) * 32), 0, st);
+      return launch_norm_rows<DTYPE, false, 1>(a, static_cast<int>(cdiv(vecs, 32) * 32), sms, st);
     // the vectors per thread that leave the fewest lanes idle
     const int npt = cdiv(vecs, 4 * 32) * 4 <= cdiv(vecs, 2 * 32) * 2 ? 4 : 2;
     const int threads = static_cast<int>(cdiv(vecs, npt * 32) * 32);
-    const int smem = 3 * a.D * 4;
-    int per_sm = 65536 / (threads * (npt == 4 ? 128 : 80));  // by registers, then by shared memory
-    if (per_sm > 220 * 1024 / (smem + 2048)) per_sm = 220 * 1024 / (smem + 2048);
-    if (per_sm > 16) per_sm = 16;
-    if (per_sm < 1) per_sm = 1;
-    const dim3 grid(static_cast<unsigned>(a.rows < int64_t(sms) * per_sm ? a.rows : sms * per_sm));
-    return npt == 4 ? launch_norm_rows<DTYPE, true, 4>(a, grid, threads, smem, st)
-                    : launch_norm_rows<DTYPE, true, 2>(a, grid, threads, smem, st);
+    return npt == 4 ? launch_norm_rows<DTYPE, true, 4>(a, threads, sms, st)
+                    : launch_norm_rows<DTYPE, true, 2>(a, threads, sms, st);
   }
   auto threads = [&](int npt) { return static_cast<int>(cdiv(cdiv(a.D, npt), 32) * 32); };
   if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 1, 8>, rows, threads(8), 0, 1, st, a);
