@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
     if (threadIdx.x == 0) a.q_scale[row] = s;
     // out / s as a product with 1 / s, within 2^-23 of the quotient; the nearest integer
     // is the low byte of the sum with 1.5 * 2^23 (at most 127 in magnitude)
-    const float inv = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    const float inv = s > 0.0f ? fminf(__fdiv_rn(1.0f, s), 3.402823466e38f) : 0.0f;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
       if (FULL || on[k]) {

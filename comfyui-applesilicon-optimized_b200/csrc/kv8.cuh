@@ -53,7 +53,11 @@ struct Kv8AppendArgs {
 constexpr int kKvThreads = 256;
 
 // One CTA per (block, head, sequence, K or V).  NV: 8-value vectors a thread
-// holds (T * D <= 2048 * NV).
+// holds (T * D <= 2048 * NV).  Bound: HBM; the quotient x / scale is a product with
+// the scale's reciprocal (within 2^-23 of it, so a code differs from the quotient's
+// nearest integer only where that is a tie to seven digits), and the nearest integer
+// is the low byte of its sum with 1.5 * 2^23: division and clamping cost twice the
+// memory's time.
 template <typename T, int NV>
 __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendArgs a) {
   __shared__ uint32_t wmax[kKvThreads / 32];
@@ -73,7 +77,7 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
   if (page < 0) return;
   const int old = static_cast<int>(first < start ? start - first : 0);  // tokens already there
   const int upto = static_cast<int>(end - first < c.T ? end - first : c.T);
-  const int dv = c.D >> 3;  // vectors per token
+  const int ldv = c.D == 128 ? 4 : 3, dv = 1 << ldv;  // vectors per token
   const T* src = static_cast<const T*>(is_v ? a.v : a.k) + b * (is_v ? a.vb : a.kb) + h * (is_v ? a.vh : a.kh);
   const int64_t st = is_v ? a.vt : a.kt;
   int8_t* codes = (is_v ? c.v : c.k) + (static_cast<int64_t>(page) * c.heads + h) * (static_cast<int64_t>(c.T) * c.D);
@@ -85,8 +89,8 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
   for (int k = 0; k < NV; ++k) {
     const int i = (old * dv) + tid + k * kKvThreads;
     if (i < upto * dv) {
-      const int tok = i / dv;
-      raw[k] = __ldg(reinterpret_cast<const uint4*>(src + (first + tok - start) * st + (i - tok * dv) * 8));
+      const int tok = i >> ldv;
+      raw[k] = __ldg(reinterpret_cast<const uint4*>(src + (first + tok - start) * st + (i & (dv - 1)) * 8));
       const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) top = max(top, max(u[j] & 0x7FFFu, (u[j] >> 16) & 0x7FFFu));
@@ -105,24 +109,26 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
   // a NaN on either side must win, so that the block reads back as NaN
   const float s = before > grown || before != before ? before : grown;
   if (tid == 0) *scale = s;
-  const float div = s > 0.0f || s != s ? s : 1.0f;
+  // a zero scale's block holds zeros, an infinite or NaN one's reads back as NaN anyway;
+  // a scale below 2^-128 would have an infinite reciprocal
+  const float inv = s > 0.0f && s <= 3.402823466e38f ? fminf(__fdiv_rn(1.0f, s), 3.402823466e38f) : 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int i = (old * dv) + tid + k * kKvThreads;
     if (i < upto * dv) {
       const uint32_t u[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-      __align__(8) int8_t o[8];
+      uint32_t o[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint16_t e = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
-        const float f = rintf(__fdiv_rn(to_float<T>(*reinterpret_cast<const T*>(&e)), div));
-        o[j] = static_cast<int8_t>(fminf(fmaxf(f, -127.0f), 127.0f));
+        o[j] = __float_as_uint(fmaf(to_float<T>(*reinterpret_cast<const T*>(&e)), inv, 12582912.0f));
       }
-      *reinterpret_cast<uint2*>(codes + i * 8) = *reinterpret_cast<const uint2*>(o);
+      *reinterpret_cast<uint2*>(codes + i * 8) =
+          make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));
     }
   }
   if (old > 0 && s != before) {
-    const float ratio = __fdiv_rn(before, div);
+    const float ratio = s > 0.0f && s <= 3.402823466e38f ? __fdiv_rn(before, s) : 0.0f;
     for (int i = tid; i < old * dv; i += kKvThreads) {
       __align__(8) int8_t o[8];
       *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(codes + i * 8);
@@ -146,45 +152,63 @@ struct Kv8GatherArgs {
   int B, S;
 };
 
-// One thread per 8 codes; grid (vectors of a head, heads, 2 B).
+// Four vectors of 8 codes per thread, their loads in flight together; grid (vectors of
+// a head, heads, 2 B).  Bound: HBM.
+constexpr int kGatherVecs = 4;
 __global__ void __launch_bounds__(kKvThreads) kv8_gather_kernel(const Kv8GatherArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
   const bool is_v = blockIdx.z & 1;
-  const int b = blockIdx.z >> 1, h = blockIdx.y, dv = c.D >> 3;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kKvThreads + threadIdx.x;
-  if (i >= static_cast<int64_t>(a.S) * dv) return;
-  const int tok = static_cast<int>(i / dv), d = static_cast<int>(i - static_cast<int64_t>(tok) * dv) * 8;
+  const int b = blockIdx.z >> 1, h = blockIdx.y, ldv = c.D == 128 ? 4 : 3;
   const int first = a.first[b];
-  float f[8];
+  const int count = first >= 0 ? a.counts[b] : 0;
+  const int64_t i0 = static_cast<int64_t>(blockIdx.x) * (kKvThreads * kGatherVecs) + threadIdx.x;
+  const int8_t* codes = is_v ? c.v : c.k;
+  const float* scales = is_v ? c.vs : c.ks;
+  uint2 raw[kGatherVecs];
+  float s[kGatherVecs];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = 0.0f;
-  if (first >= 0 && tok < a.counts[b]) {
-    const int64_t pos = static_cast<int64_t>(first) + tok;
-    const int page = kv8_page(c, b, static_cast<int>(pos >> c.log_t));
-    if (page >= 0) {
-      const int64_t at = static_cast<int64_t>(page) * c.heads + h;
-      const float s = __ldg((is_v ? c.vs : c.ks) + at);
-      const int8_t* p = (is_v ? c.v : c.k) + (at * c.T + (pos & (c.T - 1))) * c.D + d;
-      __align__(8) int8_t o[8];
-      *reinterpret_cast<uint2*>(o) = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = __fmul_rn(static_cast<float>(o[j]), s);
+  for (int u = 0; u < kGatherVecs; ++u) {
+    const int64_t i = i0 + u * kKvThreads;
+    const int64_t tok = i >> ldv;
+    raw[u] = make_uint2(0, 0);
+    s[u] = 0.0f;
+    if (tok < a.S && tok < count) {
+      const int64_t pos = first + tok;
+      const int page = kv8_page(c, b, static_cast<int>(pos >> c.log_t));
+      if (page >= 0) {
+        const int64_t at = static_cast<int64_t>(page) * c.heads + h;
+        s[u] = __ldg(scales + at);
+        raw[u] = __ldg(reinterpret_cast<const uint2*>(codes + (((at << c.log_t) + (pos & (c.T - 1))) << (ldv + 3)) +
+                                                      ((i & ((1 << ldv) - 1)) << 3)));
+      }
     }
   }
-  const int64_t dst = ((static_cast<int64_t>(b) * c.heads + h) * a.S + tok) * c.D + d;
   void* out = is_v ? a.v : a.k;
-  if (a.out_dtype == kOutF32) {
-    float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + dst);
-    p[0] = make_float4(f[0], f[1], f[2], f[3]);
-    p[1] = make_float4(f[4], f[5], f[6], f[7]);
-  } else {
-    uint32_t o[4];
+  const int64_t base = ((static_cast<int64_t>(b) * c.heads + h) * a.S) << (ldv + 3);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      o[j] = a.out_dtype == kOutBF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+  for (int u = 0; u < kGatherVecs; ++u) {
+    const int64_t i = i0 + u * kKvThreads;
+    if ((i >> ldv) >= a.S) break;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t w = j < 4 ? raw[u].x : raw[u].y;
+      f[j] = __fmul_rn(static_cast<float>(static_cast<int8_t>(w >> (8 * (j & 3)))), s[u]);
+    }
+    const int64_t dst = base + (i << 3);
+    if (a.out_dtype == kOutF32) {
+      float4* p = reinterpret_cast<float4*>(static_cast<float*>(out) + dst);
+      p[0] = make_float4(f[0], f[1], f[2], f[3]);
+      p[1] = make_float4(f[4], f[5], f[6], f[7]);
+    } else {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        o[j] = a.out_dtype == kOutBF16 ? pack_bf16x2(f[2 * j], f[2 * j + 1]) : pack_f16x2(f[2 * j], f[2 * j + 1]);
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
   }
 }
 

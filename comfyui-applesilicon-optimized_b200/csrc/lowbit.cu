@@ -474,7 +474,7 @@ int b200q_kv8_gather(const int8_t* k_codes, const int8_t* v_codes, const float* 
   a.k = k; a.v = v; a.out_dtype = out_dtype;
   a.first = first; a.counts = counts;
   a.B = static_cast<int>(B); a.S = static_cast<int>(S);
-  const dim3 grid(static_cast<unsigned>(cdiv(S * (D / 8), kKvThreads)), static_cast<unsigned>(heads),
+  const dim3 grid(static_cast<unsigned>(cdiv(S * (D / 8), kKvThreads * kGatherVecs)), static_cast<unsigned>(heads),
                   static_cast<unsigned>(2 * B));
   return launch(kv8_gather_kernel, grid, kKvThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
 }
