@@ -260,12 +260,12 @@ constexpr int kAttnThreads = (kAttnWarps + 1) * 32;  // and a producer warp
 // The CTA's ring: stages of 64 tokens of K and V, brought by TMA with the row
 // swizzle; 16-token tile w of a stage belongs to consumer warp w.  meta: per tile
 // {ks, log2 vs, 1 / vs, state}, state 0 = skip (bad page), 1 = ok, 2 = vs is 0.
-template <int D>
+template <int D, int ST = kAttnStages>
 struct AttnRing {
-  uint8_t k[kAttnStages][16 * kAttnWarps * D];
-  uint8_t v[kAttnStages][16 * kAttnWarps * D];
-  float4 meta[kAttnStages][kAttnWarps];
-  uint64_t full[kAttnStages], empty[kAttnStages];
+  uint8_t k[ST][16 * kAttnWarps * D];
+  uint8_t v[ST][16 * kAttnWarps * D];
+  float4 meta[ST][kAttnWarps];
+  uint64_t full[ST], empty[ST];
   int abort;
 };
 template <int D>
@@ -277,14 +277,16 @@ __device__ __forceinline__ AttnRing<D>* attn_ring() {
   extern __shared__ uint8_t attn_smem[];  // the swizzle pattern is anchored at 1024 bytes
   return reinterpret_cast<AttnRing<D>*>((reinterpret_cast<uintptr_t>(attn_smem) + 1023) & ~uintptr_t(1023));
 }
-template <int D>
-__device__ __forceinline__ void attn_ring_init(AttnRing<D>* ring, const CUtensorMap* tk, const CUtensorMap* tv) {
+// `readers`: warps that release a stage.
+template <int D, int ST>
+__device__ __forceinline__ void attn_ring_init(AttnRing<D, ST>* ring, const CUtensorMap* tk, const CUtensorMap* tv,
+                                               int readers = kAttnWarps) {
   if (threadIdx.x == 0) {
     tma_prefetch_desc(tk);
     tma_prefetch_desc(tv);
-    for (int i = 0; i < kAttnStages; ++i) {
+    for (int i = 0; i < ST; ++i) {
       mbar_init(&ring->full[i], 2);  // the copies and the meta words
-      mbar_init(&ring->empty[i], kAttnWarps);
+      mbar_init(&ring->empty[i], readers);
     }
     ring->abort = 0;
     fence_mbarrier_init();
@@ -346,9 +348,9 @@ __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
 // min(T, 64) rows per page.  Tiles at or past `tiles` are not fetched.  The first
 // stages' copies start before the scales are waited for: a stage is full after two
 // arrivals, the copies' and the one behind its meta words.
-template <int D>
+template <int D, int ST>
 __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtensorMap* tk, const CUtensorMap* tv,
-                                             AttnRing<D>* ring, int b, int h, int c0, int c1, int tiles) {
+                                             AttnRing<D, ST>* ring, int b, int h, int c0, int c1, int tiles) {
   const Kv8Cache& c = a.c;
   const int lane = threadIdx.x & 31;
   const int box = c.T < kAttnBox ? c.T : kAttnBox;
@@ -375,14 +377,14 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     };
     const int many = min(32 / kAttnWarps, c1 - base);
     if (n == 0)
-      for (int i = 0; i < min(many, kAttnStages); ++i) copy(i, i);
+      for (int i = 0; i < min(many, ST); ++i) copy(i, i);
     float4 meta = make_float4(ks, 0.0f, 1.0f, 2.0f);
     if (vs != 0.0f) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
     if (page < 0) meta.w = 0.0f;
     for (int i = 0; i < many; ++i, ++n) {
-      const int s = n % kAttnStages;
-      if (n >= kAttnStages) {
-        if (!mbar_wait_warp(&ring->empty[s], ((n / kAttnStages) - 1) & 1, &ring->abort)) {
+      const int s = n % ST;
+      if (n >= ST) {
+        if (!mbar_wait_warp(&ring->empty[s], ((n / ST) - 1) & 1, &ring->abort)) {
           live = false;
           break;
         }
@@ -394,8 +396,8 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     }
   }
   if (!live && lane == 0) {  // gave up: let the copies in flight land before the CTA ends
-    for (int i = n > kAttnStages ? n - kAttnStages : 0; i < n; ++i)
-      mbar_wait_drain(&ring->full[i % kAttnStages], (i / kAttnStages) & 1);
+    for (int i = n > ST ? n - ST : 0; i < n; ++i)
+      mbar_wait_drain(&ring->full[i % ST], (i / ST) & 1);
   }
 }
 // This lane's K words of a 16-token tile: tokens g and g + 8, quarter t.
@@ -491,7 +493,7 @@ __global__ void __launch_bounds__(kAttnThreads)
   __shared__ float sm_ml[kAttnWarps][16][2];
   __shared__ float sm_fin[16][2];
   AttnRing<D>* ring = attn_ring<D>();
-  attn_ring_init<D>(ring, &tk, &tv);
+  attn_ring_init(ring, &tk, &tv);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -561,7 +563,7 @@ __global__ void __launch_bounds__(kAttnThreads)
     for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
-  if (warp == kAttnWarps) attn_produce<D>(a, &tk, &tv, ring, b, h, c0, c1, tiles);
+  if (warp == kAttnWarps) attn_produce(a, &tk, &tv, ring, b, h, c0, c1, tiles);
   for (int n = 0; warp < kAttnWarps && n < c1 - c0; ++n) {
     const int s_ = n % kAttnStages;
     if (!mbar_wait_warp(&ring->full[s_], (n / kAttnStages) & 1, &ring->abort)) break;
@@ -716,7 +718,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   __shared__ float sm_ml[kAttnWarps][8][2];
   __shared__ float sm_fin[8][2];
   AttnRing<D>* ring = attn_ring<D>();
-  attn_ring_init<D>(ring, &tk, &tv);
+  attn_ring_init(ring, &tk, &tv);
   griddep_wait();
   griddep_launch_dependents();
   const Kv8Cache& c = a.c;
@@ -729,7 +731,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   const int chunks = (tiles + kAttnWarps - 1) / kAttnWarps;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
   const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
-  if (warp == kAttnWarps) attn_produce<D>(a, &tk, &tv, ring, b, h, c0, c1, tiles);
+  if (warp == kAttnWarps) attn_produce(a, &tk, &tv, ring, b, h, c0, c1, tiles);
 
   // ---- q digits of row g, quarter t: each warp makes its share of the words
   __shared__ uint32_t sm_q[3][D / 16][32];

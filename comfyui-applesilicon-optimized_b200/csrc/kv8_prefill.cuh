@@ -1,0 +1,341 @@
+// Attention over the paged 8-bit cache for many rows per key/value head (a prompt's
+// chunk, or many grouped heads): 128 packed rows (token * G + head) per CTA on the
+// tensor cores' tcgen05 MMAs, fp16 operands, fp32 accumulators in TMEM.
+//
+// The mathematics is that of kv8.cuh: codes are exact in fp16, q's rows are scaled by
+// a power of two, the weights are P = 2^(sigma + log2 vs - m) and the sum of P / vs
+// divides at the end.  m is only raised when a row's maximum has grown by more than
+// 2^8 (P <= 256 fits fp16 as well as P <= 1 does), so the accumulator in TMEM is
+// rarely rescaled.
+//
+// Per 64-token stage:
+//   warp 8      TMA producer (the ring of kv8.cuh, two stages)
+//   warps 4-7   int8 -> fp16: K and V as 64 x D tiles, rows of 128 bytes with the
+//               128-byte swizzle
+//   warp 9      MMAs, one thread: S[128 x 64] = Q K^T (both K-major), then
+//               O[128 x D] += P V with P from TMEM and V as the N-major operand its
+//               rows are (no transpose)
+//   warps 0-3   softmax, one thread per row: S from TMEM, P back to TMEM
+// Two CTAs per SM overlap one's softmax with the other's MMAs (256 TMEM columns and
+// about 97 KB of shared memory each).  Bound: the exponentials (64 per row and stage,
+// 16 a cycle and SM) and the conversion's instructions.
+#pragma once
+
+#include "kv8.cuh"
+
+namespace b200q {
+
+constexpr int kPfThreads = 320;
+constexpr int kPfRows = 128;
+constexpr int kPfStages = 2;
+constexpr uint32_t kPfCols = 256;  // TMEM: S 64, P 32 (at 64), O D (at 128)
+
+template <int D>
+struct PfSmem {
+  AttnRing<D, kPfStages> ring;
+  alignas(1024) uint8_t q[kPfRows * D * 2];  // D / 64 atoms of 128 rows x 128 bytes
+  alignas(1024) uint8_t k[64 * D * 2];       // D / 64 atoms of 64 rows x 128 bytes
+  alignas(1024) uint8_t v[64 * D * 2];
+  uint64_t k_full, k_empty, v_full, v_empty, s_full, p_full;
+  uint32_t tmem;
+};
+template <int D>
+constexpr int pf_smem_bytes() {
+  return static_cast<int>(sizeof(PfSmem<D>)) + 1024;
+}
+
+__device__ __forceinline__ void pf_tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void pf_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D(tmem) (+)= A(tmem) x B(smem desc), kind::f16, one thread.
+__device__ __forceinline__ void pf_umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// Descriptor of an N-major operand in the same tiles: rows of 64 values of N (128
+// bytes, swizzled), 8-row groups of K 1024 bytes apart (the stride field), 64-value
+// atoms of N `atom` bytes apart (the leading field).
+__device__ __forceinline__ uint64_t pf_nmajor_desc(uint32_t smem_addr, uint32_t atom) {
+  return (make_sw128_desc(smem_addr) & ~(uint64_t(0x3FFF) << 16)) | (uint64_t((atom >> 4) & 0x3FFFu) << 16);
+}
+
+// 16 int8 codes as 16 fp16 values.
+__device__ __forceinline__ void pf_widen(const uint4& c, uint4& lo, uint4& hi) {
+  const uint32_t w[4] = {c.x ^ 0x80808080u, c.y ^ 0x80808080u, c.z ^ 0x80808080u, c.w ^ 0x80808080u};
+  lo = make_uint4(i8_lo(w[0]), i8_hi(w[0]), i8_lo(w[1]), i8_hi(w[1]));
+  hi = make_uint4(i8_lo(w[2]), i8_hi(w[2]), i8_lo(w[3]), i8_hi(w[3]));
+}
+// Widens a 64 x D tile with 128 threads (x = 0 .. 127).  Eight lanes take four chunks
+// of rows r and r ^ 5: with the two swizzles neither the reads nor the writes collide.
+template <int D>
+__device__ __forceinline__ void pf_convert(const uint8_t* src, uint8_t* dst, int x) {
+  constexpr int HALVES = D / 64;  // groups of four 16-byte chunks per row
+#pragma unroll
+  for (int it = 0; it < 2 * HALVES; ++it) {
+    const int c = (x & 3) + 4 * (it % HALVES);
+    const int idx = (x >> 3) + 16 * (it / HALVES);
+    const int row = (idx >> 2) * 8 + ((idx & 3) ^ (((x >> 2) & 1) * 5));
+    uint4 lo, hi;
+    pf_widen(*reinterpret_cast<const uint4*>(src + attn_at<D>(row, c)), lo, hi);
+    uint8_t* to = dst + ((2 * c) >> 3) * (64 * 128) + row * 128;
+    *reinterpret_cast<uint4*>(to + ((((2 * c) & 7) ^ (row & 7)) << 4)) = lo;
+    *reinterpret_cast<uint4*>(to + ((((2 * c + 1) & 7) ^ (row & 7)) << 4)) = hi;
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPfThreads, 2)
+    kv8_prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                       const Kv8AttnArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  PfSmem<D>& sm = *reinterpret_cast<PfSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  AttnRing<D, kPfStages>* ring = &sm.ring;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&sm.k_full, 128);
+    mbar_init(&sm.v_full, 128);
+    mbar_init(&sm.p_full, 128);
+    mbar_init(&sm.k_empty, 1);
+    mbar_init(&sm.v_empty, 1);
+    mbar_init(&sm.s_full, 1);
+  }
+  if (warp == 9) {
+    tmem_alloc(&sm.tmem, kPfCols);
+    tmem_relinquish();
+  }
+  attn_ring_init(ring, &tk, &tv, 8);  // converters and softmax warps; ends with a barrier
+  griddep_wait();
+  griddep_launch_dependents();
+
+  const Kv8Cache& c = a.c;
+  const int split = blockIdx.x, b = blockIdx.z, rows = a.G * a.Tq;
+  const int row_tiles = (rows + kPfRows - 1) / kPfRows;
+  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * kPfRows;
+  const int len = min(max(a.lens[b], 0), c.max_blocks << c.log_t);
+  const int last = min(r0 + kPfRows, rows) - 1;
+  const int lim_max = attn_limit(a, len, last / a.G), lim_min = attn_limit(a, len, r0 / a.G);
+  const int tiles = (lim_max + 15) >> 4, chunks = (tiles + 3) >> 2;
+  const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
+  const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (split + 1) / a.splits);
+  const int n_tiles = c1 - c0;
+  volatile int* abort = &ring->abort;
+
+  // ---- Q: one row per softmax thread, scaled to fp16, K-major tile
+  float sc = 0.0f;
+  int lim = 0, ti = 0, hi = 0;
+  if (warp < 4) {
+    const int r = min(r0 + tid, rows - 1);
+    ti = r / a.G;
+    hi = h * a.G + (r - ti * a.G);
+    lim = attn_limit(a, len, ti);
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qb + hi * a.qh + ti * a.qt;
+    float inv = 1.0f, up = 1.0f;
+    if (!a.q_f16) {
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int j = 0; j < D / 8; ++j) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7FFFu, (u[i] >> 16) & 0x7FFFu));
+      }
+      int ex = static_cast<int>(top >> 7);
+      ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+      inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+      up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+    }
+    sc = a.scale_log2 * up;
+#pragma unroll 4
+    for (int j = 0; j < D / 8; ++j) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      *reinterpret_cast<uint4*>(sm.q + (j >> 3) * (kPfRows * 128) + tid * 128 + (((j & 7) ^ (tid & 7)) << 4)) =
+          make_uint4(q_pair(v.x, a.q_f16, inv), q_pair(v.y, a.q_f16, inv), q_pair(v.z, a.q_f16, inv),
+                     q_pair(v.w, a.q_f16, inv));
+    }
+    fence_proxy_async_smem();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  const uint32_t tm_s = tmem, tm_p = tmem + 64, tm_o = tmem + 128;
+
+  float m = -INFINITY, l = 0.0f;
+  if (warp == 8) {
+    attn_produce(a, &tk, &tv, ring, b, h, c0, c1, tiles);
+  } else if (warp == 9) {
+    if (lane == 0) {
+      const uint64_t dq = make_sw128_desc(smem_u32(sm.q)), dk = make_sw128_desc(smem_u32(sm.k));
+      const uint64_t dv = pf_nmajor_desc(smem_u32(sm.v), 64 * 128);
+      constexpr uint32_t iqk = kind_idesc<MmaKind::F16>(kPfRows, 64);
+      constexpr uint32_t ipv = kind_idesc<MmaKind::F16>(kPfRows, D) | (1u << 16);  // B is N-major
+      auto scores = [&](int j) {
+        if (!mbar_wait(&sm.k_full, j & 1, abort)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          umma_ss<MmaKind::F16>(tm_s, dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
+                                dk + (s >> 2) * (64 * 128 >> 4) + (s & 3) * 2, iqk, s > 0);
+        umma_commit(&sm.k_empty);
+        umma_commit(&sm.s_full);
+        return true;
+      };
+      bool live = n_tiles > 0 && scores(0);
+      for (int j = 0; live && j < n_tiles; ++j) {
+        live = mbar_wait(&sm.p_full, j & 1, abort) && mbar_wait(&sm.v_full, j & 1, abort);
+        if (!live) break;
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < 4; ++s) pf_umma_ts(tm_o, tm_p + s * 8, dv + s * (16 * 128 >> 4), ipv, j > 0 || s > 0);
+        umma_commit(&sm.v_empty);
+        if (j + 1 < n_tiles) live = scores(j + 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int x = tid - 128;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int s = j % kPfStages;
+      if (!mbar_wait_warp(&ring->full[s], (j / kPfStages) & 1, abort)) break;
+      if (j > 0 && !mbar_wait_warp(&sm.k_empty, (j - 1) & 1, abort)) break;
+      pf_convert<D>(ring->k[s], sm.k, x);
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.k_full);
+      if (j > 0 && !mbar_wait_warp(&sm.v_empty, (j - 1) & 1, abort)) break;
+      pf_convert<D>(ring->v[s], sm.v, x);
+      fence_proxy_async_smem();
+      mbar_arrive(&sm.v_full);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->empty[s]);
+    }
+  } else {
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int st = j % kPfStages;
+      if (!mbar_wait_warp(&ring->full[st], (j / kPfStages) & 1, abort)) break;
+      float4 meta[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) meta[i] = ring->meta[st][i];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ring->empty[st]);
+      if (!mbar_wait_warp(&sm.s_full, j & 1, abort)) break;
+      tc_fence_after();
+      uint32_t s0[32], s1[32];
+      tmem_ld32(tm_s + lane_base, s0);
+      tmem_ld32(tm_s + lane_base + 32, s1);
+      tmem_ld_wait();
+      const int pos = (c0 + j) * 64;
+      const bool mask = pos + 64 > lim_min;
+      float top = -INFINITY;
+      auto score = [&](uint32_t (&r)[32], int half) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const float4& mt = meta[half * 2 + (i >> 4)];
+          float x = fmaf(__uint_as_float(r[i]), mt.x * sc, mt.y);
+          if (mt.w == 0.0f || (mask && pos + half * 32 + i >= lim)) x = -INFINITY;
+          top = fmaxf(top, x);
+          r[i] = __float_as_uint(x);
+        }
+      };
+      score(s0, 0);
+      score(s1, 1);
+      if (__any_sync(0xffffffffu, top > m + 8.0f)) {
+        const float mn = fmaxf(m, top);
+        const float corr = safe_ex2_diff(m, mn);
+        m = mn;
+        l *= corr;
+        if (j > 0) {  // the last P V has completed: S was computed behind it
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_ld32(tm_o + lane_base + 32 * q, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            pf_tmem_st32(tm_o + lane_base + 32 * q, o);
+          }
+          pf_tmem_st_wait();
+        }
+      }
+      uint32_t p[32];
+      auto weigh = [&](uint32_t (&r)[32], int half) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float4& mt = meta[half * 2 + (i >> 4)];
+          const float x = __uint_as_float(r[i]), y = __uint_as_float(r[i + 1]);
+          // a masked score is exactly -inf; a NaN one stays NaN
+          const float px = x == -INFINITY ? 0.0f : ex2f(x - m), py = y == -INFINITY ? 0.0f : ex2f(y - m);
+          l = fmaf(px + py, mt.z, l);
+          p[half * 16 + (i >> 1)] = mt.w == 2.0f ? 0u : pack_f16x2(px, py);
+        }
+      };
+      weigh(s0, 0);
+      weigh(s1, 1);
+      pf_tmem_st32(tm_p + lane_base, p);
+      pf_tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(&sm.p_full);
+    }
+    // ---- O: the last P V has to complete; every lane stores its own row
+    bool good = true;
+    if (n_tiles > 0) good = mbar_wait_warp(&sm.v_empty, (n_tiles - 1) & 1, abort);
+    tc_fence_after();
+    const bool stored = r0 + tid < rows && good;
+    const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
+    const int64_t part = static_cast<int64_t>(split) * a.B * a.Hq * a.Tq + flat;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot;
+#pragma unroll 1
+    for (int q = 0; q < D / 32; ++q) {
+      uint32_t o[32];
+      if (n_tiles > 0) {
+        tmem_ld32(tm_o + lane_base + 32 * q, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      if (stored && a.splits > 1) {
+        float4* to = reinterpret_cast<float4*>(a.part_o + part * D + 32 * q);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          to[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]),
+                              __uint_as_float(o[4 * i + 3]));
+      } else if (stored) {
+        uint4* to = reinterpret_cast<uint4*>(out + 32 * q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = __uint_as_float(o[8 * i + 2 * k]) * inv, y = __uint_as_float(o[8 * i + 2 * k + 1]) * inv;
+            w[k] = a.q_f16 ? pack_f16x2(x, y) : pack_bf16x2(x, y);
+          }
+          to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      __syncwarp();  // the next load wants the whole warp
+    }
+    if (stored) {
+      if (a.splits > 1) *reinterpret_cast<float2*>(a.part_ml + part * 2) = make_float2(m, l);
+      else a.lse[flat] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, kPfCols);
+}
+
+}  // namespace b200q

@@ -7,6 +7,7 @@
 #include "block_norm.cuh"
 #include "host.h"
 #include "kv8.cuh"
+#include "kv8_prefill.cuh"
 #include "w4a16.cuh"
 
 using namespace b200q;
@@ -254,8 +255,10 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
 // More than one leave fp32 partials for the join kernel.  (A cluster of up to 16
 // CTAs joining over distributed shared memory was no faster: 8 heads x 2048 tokens
 // 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
+int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : kPfRows; }
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
-  const int64_t base = B * heads * cdiv(Hq / heads * Tq, 16);
+  const int64_t rows = Hq / heads * Tq;
+  const int64_t base = B * heads * cdiv(rows, attn_row_tile(rows));
   int64_t s = cdiv(int64_t(sms) * 2, base);
   if (s < cdiv(max_len, 4096)) s = cdiv(max_len, 4096);
   const int64_t most = cdiv(max_len, 128);
@@ -523,7 +526,7 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   a.splits = splits;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, 16)),
+  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq))),
                   static_cast<unsigned>(B));
   // the pool as rows of D bytes; a page's rows of one head are contiguous
   const int64_t pool_rows = pages * heads * block;
@@ -534,8 +537,12 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
       !host::tmap_u8(&tv, v_codes, D, pool_rows, D, static_cast<uint32_t>(D), box, sw))
     return B200Q_ERR_CUDA;
   int s;
-  // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel)
-  if (a.G * Tq <= 8) {
+  // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel); more
+  // than 16: 128-row tiles on tcgen05
+  if (a.G * Tq > 16) {
+    s = D == 128 ? launch(kv8_prefill_kernel<128>, grid, kPfThreads, pf_smem_bytes<128>(), 1, st, tk, tv, a)
+                 : launch(kv8_prefill_kernel<64>, grid, kPfThreads, pf_smem_bytes<64>(), 1, st, tk, tv, a);
+  } else if (a.G * Tq <= 8) {
     s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
                  : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   } else {
