@@ -15,9 +15,10 @@
 //   warp 9      MMAs, one thread: S[128 x 64] = Q K^T (both K-major), then
 //               O[128 x D] += P V with P from TMEM and V as the N-major operand its
 //               rows are (no transpose)
-//   warps 0-3   softmax, one thread per row: S from TMEM, P back to TMEM
-// Two CTAs per SM overlap one's softmax with the other's MMAs (256 TMEM columns and
-// about 97 KB of shared memory each).  Bound: the exponentials (64 per row and stage,
+//   warps 0-3   softmax, one thread per row: S from TMEM, P back over it
+// S has two buffers: stage j + 1's scores are computed while stage j's softmax runs.
+// Two CTAs per SM (256 TMEM columns and about 97 KB of shared memory each) fill each
+// other's gaps.  Bound: the exponentials (64 per row and stage,
 // 16 a cycle and SM) and the conversion's instructions.
 #pragma once
 
@@ -28,7 +29,7 @@ namespace b200q {
 constexpr int kPfThreads = 320;
 constexpr int kPfRows = 128;
 constexpr int kPfStages = 2;
-constexpr uint32_t kPfCols = 256;  // TMEM: S 64, P 32 (at 64), O D (at 128)
+constexpr uint32_t kPfCols = 256;  // TMEM: S 2 x 64 (P over the first half of each), O D (at 128)
 
 template <int D>
 struct PfSmem {
@@ -44,15 +45,21 @@ constexpr int pf_smem_bytes() {
   return static_cast<int>(sizeof(PfSmem<D>)) + 1024;
 }
 
-__device__ __forceinline__ void pf_tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void pf_tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void pf_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -169,7 +176,7 @@ __global__ void __launch_bounds__(kPfThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const uint32_t tm_s = tmem, tm_p = tmem + 64, tm_o = tmem + 128;
+  const uint32_t tm_o = tmem + 128;  // S and P of stage j: tmem + 64 (j & 1)
 
   float m = -INFINITY, l = 0.0f;
   if (warp == 8) {
@@ -185,7 +192,7 @@ __global__ void __launch_bounds__(kPfThreads, 2)
         tc_fence_after();
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          umma_ss<MmaKind::F16>(tm_s, dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
+          umma_ss<MmaKind::F16>(tmem + 64 * (j & 1), dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
                                 dk + (s >> 2) * (64 * 128 >> 4) + (s & 3) * 2, iqk, s > 0);
         umma_commit(&sm.k_empty);
         umma_commit(&sm.s_full);
@@ -193,13 +200,15 @@ __global__ void __launch_bounds__(kPfThreads, 2)
       };
       bool live = n_tiles > 0 && scores(0);
       for (int j = 0; live && j < n_tiles; ++j) {
+        // (its buffer was last read by stage j - 1's P V, which is ahead in the pipe)
+        if (j + 1 < n_tiles && !scores(j + 1)) break;
         live = mbar_wait(&sm.p_full, j & 1, abort) && mbar_wait(&sm.v_full, j & 1, abort);
         if (!live) break;
         tc_fence_after();
+        const uint32_t tm_p = tmem + 64 * (j & 1);
 #pragma unroll
         for (int s = 0; s < 4; ++s) pf_umma_ts(tm_o, tm_p + s * 8, dv + s * (16 * 128 >> 4), ipv, j > 0 || s > 0);
         umma_commit(&sm.v_empty);
-        if (j + 1 < n_tiles) live = scores(j + 1);
       }
     }
     __syncwarp();
@@ -229,60 +238,97 @@ __global__ void __launch_bounds__(kPfThreads, 2)
       for (int i = 0; i < 4; ++i) meta[i] = ring->meta[st][i];
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->empty[st]);
+      const uint32_t tm_s = tmem + 64 * (j & 1) + lane_base;
       if (!mbar_wait_warp(&sm.s_full, j & 1, abort)) break;
       tc_fence_after();
       uint32_t s0[32], s1[32];
-      tmem_ld32(tm_s + lane_base, s0);
-      tmem_ld32(tm_s + lane_base + 32, s1);
+      tmem_ld32(tm_s, s0);
+      tmem_ld32(tm_s + 32, s1);
       tmem_ld_wait();
       const int pos = (c0 + j) * 64;
-      const bool mask = pos + 64 > lim_min;
-      float top = -INFINITY;
-      auto score = [&](uint32_t (&r)[32], int half) {
+      // exponents: fma(S, ks * sc, log2 vs); a bad page's are -inf
+      float ksc[4], add[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float4& mt = meta[half * 2 + (i >> 4)];
-          float x = fmaf(__uint_as_float(r[i]), mt.x * sc, mt.y);
-          if (mt.w == 0.0f || (mask && pos + half * 32 + i >= lim)) x = -INFINITY;
-          top = fmaxf(top, x);
-          r[i] = __float_as_uint(x);
+      for (int i = 0; i < 4; ++i) {
+        ksc[i] = meta[i].w == 0.0f ? 0.0f : meta[i].x * sc;
+        add[i] = meta[i].w == 0.0f ? -INFINITY : meta[i].y;
+      }
+      float top = -INFINITY;
+      const bool plain = pos + 64 <= lim_min && a.scale_log2 >= 0.0f;
+      if (plain) {  // every row sees all 64: a sub-tile's largest S has its largest exponent
+        auto largest = [&](const uint32_t (&r)[32], int half) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            float x = __uint_as_float(r[16 * q]);
+#pragma unroll
+            for (int i = 1; i < 16; ++i) x = fmaxf(x, __uint_as_float(r[16 * q + i]));
+            top = fmaxf(top, fmaf(x, ksc[2 * half + q], add[2 * half + q]));
+          }
+        };
+        largest(s0, 0);
+        largest(s1, 1);
+      } else {
+        auto score = [&](uint32_t (&r)[32], int half) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int q = half * 2 + (i >> 4);
+            float x = fmaf(__uint_as_float(r[i]), ksc[q], add[q]);
+            if (pos + half * 32 + i >= lim) x = -INFINITY;
+            top = fmaxf(top, x);
+            r[i] = __float_as_uint(x);
+          }
+        };
+        score(s0, 0);
+        score(s1, 1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // they are exponents now
+          ksc[i] = 1.0f;
+          add[i] = 0.0f;
         }
-      };
-      score(s0, 0);
-      score(s1, 1);
+      }
       if (__any_sync(0xffffffffu, top > m + 8.0f)) {
         const float mn = fmaxf(m, top);
         const float corr = safe_ex2_diff(m, mn);
         m = mn;
         l *= corr;
-        if (j > 0) {  // the last P V has completed: S was computed behind it
+        if (j > 0) {
+          if (!mbar_wait_warp(&sm.v_empty, (j - 1) & 1, abort)) break;  // the last P V
+          tc_fence_after();
 #pragma unroll 1
-          for (int q = 0; q < D / 32; ++q) {
-            uint32_t o[32];
-            tmem_ld32(tm_o + lane_base + 32 * q, o);
+          for (int q = 0; q < D / 16; ++q) {
+            uint32_t o[16];
+            tmem_ld16(tm_o + lane_base + 16 * q, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            pf_tmem_st32(tm_o + lane_base + 32 * q, o);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            pf_tmem_st16(tm_o + lane_base + 16 * q, o);
           }
           pf_tmem_st_wait();
         }
       }
-      uint32_t p[32];
-      auto weigh = [&](uint32_t (&r)[32], int half) {
+      // P = 2^(exponent - m); -inf gives 0 whatever m is
+      const float mf = m == -INFINITY ? 0.0f : m;
+      auto weigh = [&](const uint32_t (&r)[32], int half) {
+        uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float4& mt = meta[half * 2 + (i >> 4)];
-          const float x = __uint_as_float(r[i]), y = __uint_as_float(r[i + 1]);
-          // a masked score is exactly -inf; a NaN one stays NaN
-          const float px = x == -INFINITY ? 0.0f : ex2f(x - m), py = y == -INFINITY ? 0.0f : ex2f(y - m);
-          l = fmaf(px + py, mt.z, l);
-          p[half * 16 + (i >> 1)] = mt.w == 2.0f ? 0u : pack_f16x2(px, py);
+        for (int q = 0; q < 2; ++q) {
+          const int u = 2 * half + q;
+          const float shift = add[u] - mf;
+          const bool zero = meta[u].w == 2.0f;
+          float sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float px = ex2f(fmaf(__uint_as_float(r[16 * q + i]), ksc[u], shift));
+            const float py = ex2f(fmaf(__uint_as_float(r[16 * q + i + 1]), ksc[u], shift));
+            sum += px + py;
+            p[8 * q + (i >> 1)] = zero ? 0u : pack_f16x2(px, py);
+          }
+          l = fmaf(sum, meta[u].z, l);
         }
+        pf_tmem_st16(tm_s + 16 * half, p);
       };
       weigh(s0, 0);
       weigh(s1, 1);
-      pf_tmem_st32(tm_p + lane_base, p);
       pf_tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&sm.p_full);

@@ -250,15 +250,30 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
   return launch(kv8_append_kernel<T, 8>, grid, kKvThreads, 0, 1, st, a);
 }
 
-// How many CTAs share a sequence's length: enough to give every SM two, and at
-// most 4096 tokens each so that ragged batches balance; at least 128 tokens each.
-// More than one leave fp32 partials for the join kernel.  (A cluster of up to 16
-// CTAs joining over distributed shared memory was no faster: 8 heads x 2048 tokens
-// 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
+// How many CTAs share a sequence's length.  Up to 16 rows a head: enough to give every
+// SM two, and at most 4096 tokens each so that ragged batches balance; at least 128
+// tokens each.  More rows (128-row tiles, two CTAs per SM): the split with the fewest
+// rounds of stages.  More than one leave fp32 partials for the join kernel.  (A cluster
+// of up to 16 CTAs joining over distributed shared memory was no faster: 8 heads x 2048
+// tokens 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
 int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : kPfRows; }
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t rows = Hq / heads * Tq;
   const int64_t base = B * heads * cdiv(rows, attn_row_tile(rows));
+  if (rows > 16) {
+    const int64_t stages = cdiv(max_len, 64);
+    int best = 1;
+    int64_t least = -1;
+    for (int s = 1; s <= kAttnMaxSplits && (s == 1 || 4 * s <= stages); ++s) {
+      // a CTA's start and end cost about four stages
+      const int64_t cost = cdiv(base * s, 2 * int64_t(sms)) * (cdiv(stages, s) + 4);
+      if (least < 0 || cost < least) {
+        least = cost;
+        best = s;
+      }
+    }
+    return best;
+  }
   int64_t s = cdiv(int64_t(sms) * 2, base);
   if (s < cdiv(max_len, 4096)) s = cdiv(max_len, 4096);
   const int64_t most = cdiv(max_len, 128);
