@@ -886,6 +886,59 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
   attn_epilogue<D, 8>(a, buf, sm_ml, sm_fin, b, h, split, 0, rows);
 }
 
+// Joins up to 8 splits of each row, one warp per row.
+template <int D>
+__global__ void __launch_bounds__(256) kv8_attn_join_few_kernel(const Kv8AttnArgs a) {
+  constexpr int VL = D / 32;  // values per lane
+  griddep_wait();
+  griddep_launch_dependents();
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Tq;
+  const int64_t flat = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (flat >= rows) return;
+  const int lane = threadIdx.x & 31;
+  float2 ml = make_float2(-INFINITY, 0.0f);
+  if (lane < a.splits) ml = *reinterpret_cast<const float2*>(a.part_ml + (lane * rows + flat) * 2);
+  float x[8][VL];
+#pragma unroll
+  for (int s = 0; s < 8; ++s)
+    if (s < a.splits) {
+      const float* p = a.part_o + (s * rows + flat) * D + lane * VL;
+      if constexpr (VL == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        x[s][0] = v.x; x[s][1] = v.y; x[s][2] = v.z; x[s][3] = v.w;
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(p);
+        x[s][0] = v.x; x[s][1] = v.y;
+      }
+    }
+  float top = ml.x;
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  top = __shfl_sync(0xffffffffu, top, 0);
+  const float f = safe_ex2_diff(ml.x, top);
+  float lt = 0.0f, acc[VL];
+#pragma unroll
+  for (int i = 0; i < VL; ++i) acc[i] = 0.0f;
+#pragma unroll
+  for (int s = 0; s < 8; ++s) {
+    const float fs = __shfl_sync(0xffffffffu, f, s), ls = __shfl_sync(0xffffffffu, ml.y, s);
+    if (s < a.splits) {
+      lt = fmaf(ls, fs, lt);
+#pragma unroll
+      for (int i = 0; i < VL; ++i) acc[i] = fmaf(x[s][i], fs, acc[i]);
+    }
+  }
+  const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
+  const int ti = static_cast<int>(flat % a.Tq);
+  const int64_t bh = flat / a.Tq, b = bh / a.Hq, hi = bh - b * a.Hq;
+  uint16_t* dst = static_cast<uint16_t*>(a.out) + b * a.ob + hi * a.oh + ti * a.ot + lane * VL;
+#pragma unroll
+  for (int i = 0; i < VL; i += 2)
+    *reinterpret_cast<uint32_t*>(dst + i) = a.q_f16 ? pack_f16x2(acc[i] * inv, acc[i + 1] * inv)
+                                                    : pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
+  if (lane == 0) a.lse[flat] = lt == 0.0f ? -INFINITY : (top + log2f(lt)) * 0.6931471805599453f;
+}
+
 // Joins up to 64 splits of a row: one CTA per row.  Every warp weighs all splits
 // (lane i has splits i and i + 32) and sums every kJoinWarps-th split's D values;
 // the warps' sums are added in order.  All loads are independent of one another.

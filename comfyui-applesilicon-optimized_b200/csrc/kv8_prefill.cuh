@@ -8,41 +8,42 @@
 // 2^8 (P <= 256 fits fp16 as well as P <= 1 does), so the accumulator in TMEM is
 // rarely rescaled.
 //
-// Per 64-token stage:
-//   warp 8      TMA producer (the ring of kv8.cuh, two stages)
-//   warps 4-7   int8 -> fp16: K and V as 64 x D tiles, rows of 128 bytes with the
-//               128-byte swizzle
-//   warp 9      MMAs, one thread: S[128 x 64] = Q K^T (both K-major), then
-//               O[128 x D] += P V with P from TMEM and V as the N-major operand its
-//               rows are (no transpose)
-//   warps 0-3   softmax, one thread per row: S from TMEM, P back over it
+// A CTA has RT row tiles of 128 (2 when there are more than 128 rows: K and V are
+// then widened once for 256 rows).  Per 64-token stage:
+//   warps 0 .. 4 RT - 1   softmax, one thread per row: S from TMEM, P back over it
+//   the next four         int8 -> fp16: K and V as 64 x D tiles, rows of 128 bytes with
+//                         the 128-byte swizzle
+//   then                  the TMA producer (the ring of kv8.cuh)
+//   and                   the MMAs, one thread: S[128 x 64] = Q K^T (both K-major), then
+//                         O[128 x D] += P V with P from TMEM and V as the N-major
+//                         operand its rows are (no transpose)
 // S has two buffers: stage j + 1's scores are computed while stage j's softmax runs.
-// Two CTAs per SM (256 TMEM columns and about 97 KB of shared memory each) fill each
-// other's gaps.  Bound: the exponentials (64 per row and stage,
-// 16 a cycle and SM) and the conversion's instructions.
+// RT = 2 takes an SM's whole TMEM and double-buffers the fp16 tiles; RT = 1 puts two
+// CTAs on an SM.  Bound: the exponentials (64 per row and stage, 16 a cycle and SM), the
+// softmax's other instructions and the conversion.
 #pragma once
 
 #include "kv8.cuh"
 
 namespace b200q {
 
-constexpr int kPfThreads = 320;
 constexpr int kPfRows = 128;
-constexpr int kPfStages = 2;
-constexpr uint32_t kPfCols = 256;  // TMEM: S 2 x 64 (P over the first half of each), O D (at 128)
+constexpr int pf_threads(int rt) { return 128 * rt + 192; }
+constexpr int pf_stages(int rt) { return rt == 2 ? 4 : 2; }
 
-template <int D>
+template <int D, int RT>
 struct PfSmem {
-  AttnRing<D, kPfStages> ring;
-  alignas(1024) uint8_t q[kPfRows * D * 2];  // D / 64 atoms of 128 rows x 128 bytes
-  alignas(1024) uint8_t k[64 * D * 2];       // D / 64 atoms of 64 rows x 128 bytes
-  alignas(1024) uint8_t v[64 * D * 2];
-  uint64_t k_full, k_empty, v_full, v_empty, s_full, p_full;
+  static constexpr int NB = RT;                   // fp16 tiles of K and of V
+  AttnRing<D, pf_stages(RT)> ring;
+  alignas(1024) uint8_t q[RT][kPfRows * D * 2];   // D / 64 atoms of 128 rows x 128 bytes
+  alignas(1024) uint8_t k[NB][64 * D * 2];        // D / 64 atoms of 64 rows x 128 bytes
+  alignas(1024) uint8_t v[NB][64 * D * 2];
+  uint64_t k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], s_full[RT], p_full[RT], o_done[RT];
   uint32_t tmem;
 };
-template <int D>
+template <int D, int RT>
 constexpr int pf_smem_bytes() {
-  return static_cast<int>(sizeof(PfSmem<D>)) + 1024;
+  return static_cast<int>(sizeof(PfSmem<D, RT>)) + 1024;
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -101,36 +102,45 @@ __device__ __forceinline__ void pf_convert(const uint8_t* src, uint8_t* dst, int
   }
 }
 
-template <int D>
-__global__ void __launch_bounds__(kPfThreads, 2)
+template <int D, int RT>
+__global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const Kv8AttnArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  PfSmem<D>& sm = *reinterpret_cast<PfSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  AttnRing<D, kPfStages>* ring = &sm.ring;
+  using Smem = PfSmem<D, RT>;
+  constexpr int NB = Smem::NB, ST = RT == 2 ? 4 : 2;
+  constexpr int kSoft = 4 * RT;            // softmax warps
+  constexpr uint32_t kCols = 256 * RT;     // TMEM: S at 128 r + 64 (stage & 1), O at 128 (RT + r)
+  Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  AttnRing<D, ST>* ring = &sm.ring;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
-    mbar_init(&sm.k_full, 128);
-    mbar_init(&sm.v_full, 128);
-    mbar_init(&sm.p_full, 128);
-    mbar_init(&sm.k_empty, 1);
-    mbar_init(&sm.v_empty, 1);
-    mbar_init(&sm.s_full, 1);
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(&sm.k_full[i], 128);
+      mbar_init(&sm.v_full[i], 128);
+      mbar_init(&sm.k_empty[i], 1);
+      mbar_init(&sm.v_empty[i], 1);
+    }
+    for (int i = 0; i < RT; ++i) {
+      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.s_full[i], 1);
+      mbar_init(&sm.o_done[i], 1);
+    }
   }
-  if (warp == 9) {
-    tmem_alloc(&sm.tmem, kPfCols);
+  if (warp == kSoft + 5) {
+    tmem_alloc(&sm.tmem, kCols);
     tmem_relinquish();
   }
-  attn_ring_init(ring, &tk, &tv, 8);  // converters and softmax warps; ends with a barrier
+  attn_ring_init(ring, &tk, &tv, kSoft + 4);  // softmax warps and converters; ends with a barrier
   griddep_wait();
   griddep_launch_dependents();
 
   const Kv8Cache& c = a.c;
   const int split = blockIdx.x, b = blockIdx.z, rows = a.G * a.Tq;
-  const int row_tiles = (rows + kPfRows - 1) / kPfRows;
-  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * kPfRows;
+  const int row_tiles = (rows + kPfRows * RT - 1) / (kPfRows * RT);
+  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * (kPfRows * RT);
   const int len = min(max(a.lens[b], 0), c.max_blocks << c.log_t);
-  const int last = min(r0 + kPfRows, rows) - 1;
+  const int last = min(r0 + kPfRows * RT, rows) - 1;
   const int lim_max = attn_limit(a, len, last / a.G), lim_min = attn_limit(a, len, r0 / a.G);
   const int tiles = (lim_max + 15) >> 4, chunks = (tiles + 3) >> 2;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
@@ -141,8 +151,9 @@ __global__ void __launch_bounds__(kPfThreads, 2)
   // ---- Q: one row per softmax thread, scaled to fp16, K-major tile
   float sc = 0.0f;
   int lim = 0, ti = 0, hi = 0;
-  if (warp < 4) {
-    const int r = min(r0 + tid, rows - 1);
+  if (warp < kSoft) {
+    const int r = min(r0 + tid, rows - 1), row = tid & 127;
+    uint8_t* qs = sm.q[tid >> 7];
     ti = r / a.G;
     hi = h * a.G + (r - ti * a.G);
     lim = attn_limit(a, len, ti);
@@ -166,7 +177,7 @@ __global__ void __launch_bounds__(kPfThreads, 2)
 #pragma unroll 4
     for (int j = 0; j < D / 8; ++j) {
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
-      *reinterpret_cast<uint4*>(sm.q + (j >> 3) * (kPfRows * 128) + tid * 128 + (((j & 7) ^ (tid & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(qs + (j >> 3) * (kPfRows * 128) + row * 128 + (((j & 7) ^ (row & 7)) << 4)) =
           make_uint4(q_pair(v.x, a.q_f16, inv), q_pair(v.y, a.q_f16, inv), q_pair(v.z, a.q_f16, inv),
                      q_pair(v.w, a.q_f16, inv));
     }
@@ -176,70 +187,84 @@ __global__ void __launch_bounds__(kPfThreads, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sm.tmem;
-  const uint32_t tm_o = tmem + 128;  // S and P of stage j: tmem + 64 (j & 1)
 
   float m = -INFINITY, l = 0.0f;
-  if (warp == 8) {
+  if (warp == kSoft + 4) {
     attn_produce(a, &tk, &tv, ring, b, h, c0, c1, tiles);
-  } else if (warp == 9) {
+  } else if (warp == kSoft + 5) {
     if (lane == 0) {
-      const uint64_t dq = make_sw128_desc(smem_u32(sm.q)), dk = make_sw128_desc(smem_u32(sm.k));
-      const uint64_t dv = pf_nmajor_desc(smem_u32(sm.v), 64 * 128);
       constexpr uint32_t iqk = kind_idesc<MmaKind::F16>(kPfRows, 64);
       constexpr uint32_t ipv = kind_idesc<MmaKind::F16>(kPfRows, D) | (1u << 16);  // B is N-major
       auto scores = [&](int j) {
-        if (!mbar_wait(&sm.k_full, j & 1, abort)) return false;
+        const int kb = j % NB;
+        if (!mbar_wait(&sm.k_full[kb], (j / NB) & 1, abort)) return false;
         tc_fence_after();
+        const uint64_t dk = make_sw128_desc(smem_u32(sm.k[kb]));
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          umma_ss<MmaKind::F16>(tmem + 64 * (j & 1), dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
-                                dk + (s >> 2) * (64 * 128 >> 4) + (s & 3) * 2, iqk, s > 0);
-        umma_commit(&sm.k_empty);
-        umma_commit(&sm.s_full);
+        for (int r = 0; r < RT; ++r) {
+          const uint64_t dq = make_sw128_desc(smem_u32(sm.q[r]));
+#pragma unroll
+          for (int s = 0; s < D / 16; ++s)
+            umma_ss<MmaKind::F16>(tmem + 128 * r + 64 * (j & 1), dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
+                                  dk + (s >> 2) * (64 * 128 >> 4) + (s & 3) * 2, iqk, s > 0);
+          umma_commit(&sm.s_full[r]);
+        }
+        umma_commit(&sm.k_empty[kb]);
         return true;
       };
       bool live = n_tiles > 0 && scores(0);
       for (int j = 0; live && j < n_tiles; ++j) {
-        // (its buffer was last read by stage j - 1's P V, which is ahead in the pipe)
+        // (its buffers were last read by stage j - 1's P V, which is ahead in the pipe)
         if (j + 1 < n_tiles && !scores(j + 1)) break;
-        live = mbar_wait(&sm.p_full, j & 1, abort) && mbar_wait(&sm.v_full, j & 1, abort);
-        if (!live) break;
-        tc_fence_after();
-        const uint32_t tm_p = tmem + 64 * (j & 1);
+        const int vb = j % NB;
+        live = mbar_wait(&sm.v_full[vb], (j / NB) & 1, abort);
+        const uint64_t dv = pf_nmajor_desc(smem_u32(sm.v[vb]), 64 * 128);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) pf_umma_ts(tm_o, tm_p + s * 8, dv + s * (16 * 128 >> 4), ipv, j > 0 || s > 0);
-        umma_commit(&sm.v_empty);
+        for (int r = 0; r < RT; ++r) {
+          live = live && mbar_wait(&sm.p_full[r], j & 1, abort);
+          if (live) {
+            tc_fence_after();
+            const uint32_t tm_p = tmem + 128 * r + 64 * (j & 1);
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+              pf_umma_ts(tmem + 128 * (RT + r), tm_p + s * 8, dv + s * (16 * 128 >> 4), ipv, j > 0 || s > 0);
+            umma_commit(&sm.o_done[r]);
+          }
+        }
+        if (live) umma_commit(&sm.v_empty[vb]);
       }
     }
     __syncwarp();
-  } else if (warp >= 4) {
-    const int x = tid - 128;
+  } else if (warp >= kSoft) {
+    const int x = tid - 128 * RT;
     for (int j = 0; j < n_tiles; ++j) {
-      const int s = j % kPfStages;
-      if (!mbar_wait_warp(&ring->full[s], (j / kPfStages) & 1, abort)) break;
-      if (j > 0 && !mbar_wait_warp(&sm.k_empty, (j - 1) & 1, abort)) break;
-      pf_convert<D>(ring->k[s], sm.k, x);
+      const int s = j % ST, nb = j % NB;
+      if (!mbar_wait_warp(&ring->full[s], (j / ST) & 1, abort)) break;
+      if (j >= NB && !mbar_wait_warp(&sm.k_empty[nb], (j / NB - 1) & 1, abort)) break;
+      pf_convert<D>(ring->k[s], sm.k[nb], x);
       fence_proxy_async_smem();
-      mbar_arrive(&sm.k_full);
-      if (j > 0 && !mbar_wait_warp(&sm.v_empty, (j - 1) & 1, abort)) break;
-      pf_convert<D>(ring->v[s], sm.v, x);
+      mbar_arrive(&sm.k_full[nb]);
+      if (j >= NB && !mbar_wait_warp(&sm.v_empty[nb], (j / NB - 1) & 1, abort)) break;
+      pf_convert<D>(ring->v[s], sm.v[nb], x);
       fence_proxy_async_smem();
-      mbar_arrive(&sm.v_full);
+      mbar_arrive(&sm.v_full[nb]);
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->empty[s]);
     }
   } else {
-    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+    const int rt = warp >> 2;  // this warp's row tile; it may touch lanes 32 (warp % 4) ..
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tm_o = tmem + 128 * (RT + rt) + lane_base;
     for (int j = 0; j < n_tiles; ++j) {
-      const int st = j % kPfStages;
-      if (!mbar_wait_warp(&ring->full[st], (j / kPfStages) & 1, abort)) break;
+      const int st = j % ST;
+      if (!mbar_wait_warp(&ring->full[st], (j / ST) & 1, abort)) break;
       float4 meta[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) meta[i] = ring->meta[st][i];
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->empty[st]);
-      const uint32_t tm_s = tmem + 64 * (j & 1) + lane_base;
-      if (!mbar_wait_warp(&sm.s_full, j & 1, abort)) break;
+      const uint32_t tm_s = tmem + 128 * rt + 64 * (j & 1) + lane_base;
+      if (!mbar_wait_warp(&sm.s_full[rt], j & 1, abort)) break;
       tc_fence_after();
       uint32_t s0[32], s1[32];
       tmem_ld32(tm_s, s0);
@@ -292,16 +317,16 @@ __global__ void __launch_bounds__(kPfThreads, 2)
         m = mn;
         l *= corr;
         if (j > 0) {
-          if (!mbar_wait_warp(&sm.v_empty, (j - 1) & 1, abort)) break;  // the last P V
+          if (!mbar_wait_warp(&sm.o_done[rt], (j - 1) & 1, abort)) break;  // the last P V
           tc_fence_after();
 #pragma unroll 1
           for (int q = 0; q < D / 16; ++q) {
             uint32_t o[16];
-            tmem_ld16(tm_o + lane_base + 16 * q, o);
+            tmem_ld16(tm_o + 16 * q, o);
             tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
-            pf_tmem_st16(tm_o + lane_base + 16 * q, o);
+            pf_tmem_st16(tm_o + 16 * q, o);
           }
           pf_tmem_st_wait();
         }
@@ -331,11 +356,11 @@ __global__ void __launch_bounds__(kPfThreads, 2)
       weigh(s1, 1);
       pf_tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&sm.p_full);
+      mbar_arrive(&sm.p_full[rt]);
     }
     // ---- O: the last P V has to complete; every lane stores its own row
     bool good = true;
-    if (n_tiles > 0) good = mbar_wait_warp(&sm.v_empty, (n_tiles - 1) & 1, abort);
+    if (n_tiles > 0) good = mbar_wait_warp(&sm.o_done[rt], (n_tiles - 1) & 1, abort);
     tc_fence_after();
     const bool stored = r0 + tid < rows && good;
     const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
@@ -346,7 +371,7 @@ __global__ void __launch_bounds__(kPfThreads, 2)
     for (int q = 0; q < D / 32; ++q) {
       uint32_t o[32];
       if (n_tiles > 0) {
-        tmem_ld32(tm_o + lane_base + 32 * q, o);
+        tmem_ld32(tm_o + 32 * q, o);
         tmem_ld_wait();
       } else {
 #pragma unroll
@@ -381,7 +406,7 @@ __global__ void __launch_bounds__(kPfThreads, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, kPfCols);
+  if (warp == kSoft + 5) tmem_dealloc(tmem, kCols);
 }
 
 }  // namespace b200q

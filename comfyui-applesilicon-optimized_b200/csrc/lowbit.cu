@@ -252,21 +252,21 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
 
 // How many CTAs share a sequence's length.  Up to 16 rows a head: enough to give every
 // SM two, and at most 4096 tokens each so that ragged batches balance; at least 128
-// tokens each.  More rows (128-row tiles, two CTAs per SM): the split with the fewest
+// tokens each.  More rows (128- or 256-row tiles, two CTAs or one per SM): the split with the fewest
 // rounds of stages.  More than one leave fp32 partials for the join kernel.  (A cluster
 // of up to 16 CTAs joining over distributed shared memory was no faster: 8 heads x 2048
 // tokens 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
-int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : kPfRows; }
+int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= kPfRows ? kPfRows : 2 * kPfRows; }
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t rows = Hq / heads * Tq;
   const int64_t base = B * heads * cdiv(rows, attn_row_tile(rows));
   if (rows > 16) {
-    const int64_t stages = cdiv(max_len, 64);
+    const int64_t stages = cdiv(max_len, 64), slots = int64_t(sms) * (rows <= kPfRows ? 2 : 1);
     int best = 1;
     int64_t least = -1;
     for (int s = 1; s <= kAttnMaxSplits && (s == 1 || 4 * s <= stages); ++s) {
       // a CTA's start and end cost about four stages
-      const int64_t cost = cdiv(base * s, 2 * int64_t(sms)) * (cdiv(stages, s) + 4);
+      const int64_t cost = cdiv(base * s, slots) * (cdiv(stages, s) + 4);
       if (least < 0 || cost < least) {
         least = cost;
         best = s;
@@ -554,9 +554,12 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   int s;
   // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel); more
   // than 16: 128-row tiles on tcgen05
-  if (a.G * Tq > 16) {
-    s = D == 128 ? launch(kv8_prefill_kernel<128>, grid, kPfThreads, pf_smem_bytes<128>(), 1, st, tk, tv, a)
-                 : launch(kv8_prefill_kernel<64>, grid, kPfThreads, pf_smem_bytes<64>(), 1, st, tk, tv, a);
+  if (a.G * Tq > kPfRows) {
+    s = D == 128 ? launch(kv8_prefill_kernel<128, 2>, grid, pf_threads(2), pf_smem_bytes<128, 2>(), 1, st, tk, tv, a)
+                 : launch(kv8_prefill_kernel<64, 2>, grid, pf_threads(2), pf_smem_bytes<64, 2>(), 1, st, tk, tv, a);
+  } else if (a.G * Tq > 16) {
+    s = D == 128 ? launch(kv8_prefill_kernel<128, 1>, grid, pf_threads(1), pf_smem_bytes<128, 1>(), 1, st, tk, tv, a)
+                 : launch(kv8_prefill_kernel<64, 1>, grid, pf_threads(1), pf_smem_bytes<64, 1>(), 1, st, tk, tv, a);
   } else if (a.G * Tq <= 8) {
     s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
                  : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
@@ -565,6 +568,11 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
                  : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
   }
   if (s != B200Q_OK || !need) return s;
+  if (splits <= 8) {
+    const dim3 few(static_cast<unsigned>(cdiv(rows, 8)));
+    return D == 128 ? launch(kv8_attn_join_few_kernel<128>, few, 256, 0, 1, st, a)
+                    : launch(kv8_attn_join_few_kernel<64>, few, 256, 0, 1, st, a);
+  }
   const dim3 jgrid(static_cast<unsigned>(rows));
   return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, kJoinWarps * 32, 0, 1, st, a)
                   : launch(kv8_attn_join_kernel<64>, jgrid, kJoinWarps * 32, 0, 1, st, a);
