@@ -116,13 +116,13 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int i = 0; i < NB; ++i) {
-      mbar_init(&sm.k_full[i], 128);
-      mbar_init(&sm.v_full[i], 128);
+      mbar_init(&sm.k_full[i], 4);  // warps
+      mbar_init(&sm.v_full[i], 4);
       mbar_init(&sm.k_empty[i], 1);
       mbar_init(&sm.v_empty[i], 1);
     }
     for (int i = 0; i < RT; ++i) {
-      mbar_init(&sm.p_full[i], 128);
+      mbar_init(&sm.p_full[i], 4);
       mbar_init(&sm.s_full[i], 1);
       mbar_init(&sm.o_done[i], 1);
     }
@@ -243,13 +243,16 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       if (j >= NB && !mbar_wait_warp(&sm.k_empty[nb], (j / NB - 1) & 1, abort)) break;
       pf_convert<D>(ring->k[s], sm.k[nb], x);
       fence_proxy_async_smem();
-      mbar_arrive(&sm.k_full[nb]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.k_full[nb]);
       if (j >= NB && !mbar_wait_warp(&sm.v_empty[nb], (j / NB - 1) & 1, abort)) break;
       pf_convert<D>(ring->v[s], sm.v[nb], x);
       fence_proxy_async_smem();
-      mbar_arrive(&sm.v_full[nb]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ring->empty[s]);
+      if (lane == 0) {
+        mbar_arrive(&sm.v_full[nb]);
+        mbar_arrive(&ring->empty[s]);
+      }
     }
   } else {
     const int rt = warp >> 2;  // this warp's row tile; it may touch lanes 32 (warp % 4) ..
@@ -356,7 +359,8 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       weigh(s1, 1);
       pf_tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&sm.p_full[rt]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.p_full[rt]);
     }
     // ---- O: the last P V has to complete; every lane stores its own row
     bool good = true;
