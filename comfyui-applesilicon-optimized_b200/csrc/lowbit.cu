@@ -383,27 +383,38 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   }
   if (M <= kW4MaxSmallM) return B200Q_ERR_UNSUPPORTED;  // N * K / group above 2^31
   const W4Work o = w4_work(M, N, K);
+  if (x_dtype == B200Q_F16 && !x_vec) return B200Q_ERR_INVALID;  // fp16 rows must be 16-byte aligned here
   uint8_t* base = static_cast<uint8_t*>(workspace);
-  __half* w16 = reinterpret_cast<__half*>(base);
-  float* col = reinterpret_cast<float*>(base + o.col);
-  int s = launch(w4_decode_rows_kernel, dim3(static_cast<unsigned>(N)), 256, 0, 1, st, w, ldw, scales,
-                 scale_dtype, zeros, int(N), int(K), int(group), w16, col);
-  if (s != B200Q_OK) return s;
-  ep.col_scale = col;
+  W4PrepareArgs a{};
+  a.w = w;
+  a.ldw = ldw;
+  a.scales = scales;
+  a.scale_dtype = scale_dtype;
+  a.zeros = zeros;
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.log_g = group == 32 ? 5 : group == 64 ? 6 : 7;
+  a.w16 = reinterpret_cast<__half*>(base);
+  a.w_pow = reinterpret_cast<float*>(base + o.col);
+  ep.col_scale = a.w_pow;
   ep.col_scale_vec = 1;
-  if (x_dtype == B200Q_BF16 || !x_vec) {
-    if (x_dtype != B200Q_BF16) return B200Q_ERR_INVALID;  // fp16 rows must be 16-byte aligned here
-    __half* x16 = reinterpret_cast<__half*>(base + o.x);
-    float* row = reinterpret_cast<float*>(base + o.row);
-    s = launch(w4_x_f16_kernel, dim3(static_cast<unsigned>(M)), 256, 0, 1, st,
-               static_cast<const __nv_bfloat16*>(x), ldx, int(K), int(x_vec), x16, row);
-    if (s != B200Q_OK) return s;
-    ep.row_scale = row;
+  int64_t blocks = cdiv(N, 8);
+  if (x_dtype == B200Q_BF16) {
+    a.x = static_cast<const __nv_bfloat16*>(x);
+    a.ldx = ldx;
+    a.M = static_cast<int>(M);
+    a.x_vec = x_vec;
+    a.x16 = reinterpret_cast<__half*>(base + o.x);
+    a.x_pow = reinterpret_cast<float*>(base + o.row);
+    ep.row_scale = a.x_pow;
     ep.row_scale_vec = 1;
-    x = x16;
+    blocks += cdiv(M, 8);
+    x = a.x16;
     ldx = K;
   }
-  return host::gemm16_scaled(true, x, ldx, w16, K, M, N, K, ep, st);
+  const int s = launch(w4_prepare_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, st, a);
+  if (s != B200Q_OK) return s;
+  return host::gemm16_scaled(true, x, ldx, a.w16, K, M, N, K, ep, st);
 }
 
 int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype,

@@ -693,102 +693,124 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 }
 
 // ---------------------------------------------------------------- many tokens
-// Decodes the weight to fp16 for the tile GEMM.  A row's values are
-// s * (c - z) * 2^-e with 2^e the power of two of the row's largest |s| (at most
-// 15 * 2 in magnitude, so fp16's range holds whatever the scales are), and 2^e
-// goes to row_pow[n] for the GEMM's column scale.  One rounding to fp16's 11
-// bits; an eighth of a bf16 output's own rounding.
-__global__ void __launch_bounds__(256)
-    w4_decode_rows_kernel(const uint8_t* __restrict__ w, int64_t ldw, const void* scales,
-                          int scale_dtype, const uint8_t* __restrict__ zeros, int N, int K, int G,
-                          __half* __restrict__ out, float* __restrict__ row_pow) {
-  __shared__ float wmax[8];
-  griddep_wait();
-  griddep_launch_dependents();
-  const int n = blockIdx.x, tid = threadIdx.x;
-  const int KG = K / G;
-  float m = 0.0f;
-  for (int i = tid; i < KG; i += 256) m = fmaxf(m, fabsf(load_scale(scales, scale_dtype, int64_t(n) * KG + i)));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((tid & 31) == 0) wmax[tid >> 5] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = fmaxf(m, wmax[i]);
-  // exponent field of the maximum, kept where 2^e and 2^-e are both normal
-  int ex = static_cast<int>(__float_as_uint(m) >> 23);
-  ex = min(max(ex, 1), 253);
-  const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-  if (tid == 0) row_pow[n] = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-  const uint8_t* src = w + int64_t(n) * ldw;
-  for (int i = tid; i < K / 32; i += 256) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + int64_t(i) * 16));
-    const int64_t gi = int64_t(n) * KG + i * 32 / G;
-    const float s = load_scale(scales, scale_dtype, gi) * inv;
-    const int z = zeros ? zeros[gi] & 15 : 8;
-    const uint32_t wv[4] = {v.x, v.y, v.z, v.w};
-    uint4* dst = reinterpret_cast<uint4*>(out + int64_t(n) * K + int64_t(i) * 32);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t o[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int lo = static_cast<int>((wv[q] >> (8 * j)) & 15u) - z;
-        const int hi = static_cast<int>((wv[q] >> (8 * j + 4)) & 15u) - z;
-        o[j] = pack_f16x2(s * static_cast<float>(lo), s * static_cast<float>(hi));
-      }
-      dst[q] = make_uint4(o[0], o[1], o[2], o[3]);
-    }
-  }
-}
+// Operands of the tile GEMM, one warp per row.
+//
+// Weight rows: fp16 values s * (c - z) * 2^-e with 2^e the power of two of the row's
+// largest |s| (at most 15 * 2 in magnitude, so fp16's range holds whatever the scales
+// are); 2^e goes to w_pow[n] for the GEMM's column scale.  c - z is exact, its product
+// with s is rounded once, to fp16's 11 bits: an eighth of a bf16 output's own rounding.
+//
+// bf16 token rows: x * 2^-e, 2^e the power of two of the row's largest |x|, to
+// x_pow[m] for the GEMM's row scale.  Exact down to 2^-17 of the row's maximum, within
+// 2^-25 of it below.
+//
+// Bound: memory (half a byte read and two written per weight).
+struct W4PrepareArgs {
+  const uint8_t* w;
+  int64_t ldw;
+  const void* scales;
+  int scale_dtype;
+  const uint8_t* zeros;
+  int N, K, log_g;
+  __half* w16;
+  float* w_pow;
+  const __nv_bfloat16* x;  // null: x is used as it is
+  int64_t ldx;
+  int M, x_vec;
+  __half* x16;
+  float* x_pow;
+};
 
-// A token row of bf16 as fp16: x * 2^-e, 2^e the power of two of the row's
-// largest |x|, to row_pow[m] for the GEMM's row scale.  Exact down to 2^-17 of
-// the row's maximum, within 2^-25 of it below.
-__global__ void __launch_bounds__(256)
-    w4_x_f16_kernel(const __nv_bfloat16* __restrict__ x, int64_t ldx, int K, int x_vec,
-                    __half* __restrict__ out, float* __restrict__ row_pow) {
-  __shared__ uint32_t wmax[8];
+__global__ void __launch_bounds__(256) w4_prepare_kernel(const W4PrepareArgs a) {
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t m = blockIdx.x;
-  const int tid = threadIdx.x;
-  const uint16_t* src = reinterpret_cast<const uint16_t*>(x + m * ldx);
-  auto piece = [&](int i, uint16_t (&e)[8]) {
-    if (x_vec) {
-      *reinterpret_cast<uint4*>(e) = __ldg(reinterpret_cast<const uint4*>(src + i * 8));
-    } else {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (item < a.N) {
+    const int KG = a.K >> a.log_g;
+    const int64_t s0 = item * KG;
+    float m = 0.0f;
+    for (int i = lane; i < KG; i += 32) m = fmaxf(m, fabsf(load_scale(a.scales, a.scale_dtype, s0 + i)));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = __ldg(src + i * 8 + j);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // exponent field of the maximum, kept where 2^e and 2^-e are both normal
+    const int ex = min(max(static_cast<int>(__float_as_uint(m) >> 23), 1), 253);
+    const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+    if (lane == 0) a.w_pow[item] = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(a.w + item * a.ldw);
+    uint4* dst = reinterpret_cast<uint4*>(a.w16 + item * a.K);
+    const int words = a.K >> 3;
+    for (int i0 = lane; i0 < words; i0 += 128) {
+      uint32_t word[4];
+      float s[4];
+      uint32_t z[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 32 * u;
+        if (i < words) {
+          word[u] = __ldg(src + i);
+          const int64_t gi = s0 + ((i << 3) >> a.log_g);
+          s[u] = load_scale(a.scales, a.scale_dtype, gi);
+          z[u] = a.zeros ? __ldg(a.zeros + gi) & 15u : 8u;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int i = i0 + 32 * u;
+        if (i < words) {
+          const uint32_t zz = w4_zero(z[u]);
+          uint32_t p[4];
+          w4_decode(word[u], __byte_perm(zz, 0, 0x1010), __byte_perm(zz, 0, 0x3232), p);
+          const float f = s[u] * inv;
+          float2 v[4];  // codes (0, 4), (1, 5), (2, 6), (3, 7)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[j] = __half22float2(*reinterpret_cast<const __half2*>(&p[j]));
+            v[j].x *= f;
+            v[j].y *= f;
+          }
+          dst[i] = make_uint4(pack_f16x2(v[0].x, v[1].x), pack_f16x2(v[2].x, v[3].x), pack_f16x2(v[0].y, v[1].y),
+                              pack_f16x2(v[2].y, v[3].y));
+        }
+      }
     }
+    return;
+  }
+  const int64_t m = item - (static_cast<int64_t>(a.N) + 7) / 8 * 8;  // (the weight's blocks end on a block)
+  if (!a.x || m < 0 || m >= a.M) return;
+  const uint16_t* row = reinterpret_cast<const uint16_t*>(a.x + m * a.ldx);
+  const int pieces = a.K >> 3;
+  auto piece = [&](int p) {
+    if (a.x_vec) return __ldg(reinterpret_cast<const uint4*>(row + p * 8));
+    uint32_t e[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e[j] = __ldg(row + p * 8 + 2 * j) | (uint32_t(__ldg(row + p * 8 + 2 * j + 1)) << 16);
+    return make_uint4(e[0], e[1], e[2], e[3]);
   };
   uint32_t top = 0;  // largest |x| as bits; infinities and NaN sort above
-  for (int i = tid; i < K / 8; i += 256) {
-    uint16_t e[8];
-    piece(i, e);
+#pragma unroll 4
+  for (int p = lane; p < pieces; p += 32) {
+    const uint4 v = piece(p);
+    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, uint32_t(e[j] & 0x7FFFu));
+    for (int j = 0; j < 4; ++j) top = max(top, max(e[j] & 0x7FFFu, (e[j] >> 16) & 0x7FFFu));
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((tid & 31) == 0) wmax[tid >> 5] = top;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, wmax[i]);
+  top = __reduce_max_sync(0xffffffffu, top);
   // a row holding inf or NaN keeps its values: they carry through the product
   int ex = static_cast<int>(top >> 7);
   ex = ex == 255 ? 127 : min(max(ex, 1), 253);
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-  if (tid == 0) row_pow[m] = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-  for (int i = tid; i < K / 8; i += 256) {
-    uint16_t e[8];
-    piece(i, e);
+  if (lane == 0) a.x_pow[m] = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+  uint4* dst = reinterpret_cast<uint4*>(a.x16 + m * a.K);
+#pragma unroll 4
+  for (int p = lane; p < pieces; p += 32) {
+    const uint4 v = piece(p);
+    const uint32_t e[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      o[j] = pack_f16x2(__uint_as_float(uint32_t(e[2 * j]) << 16) * inv,
-                        __uint_as_float(uint32_t(e[2 * j + 1]) << 16) * inv);
-    *reinterpret_cast<uint4*>(out + m * K + i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+      o[j] = pack_f16x2(__uint_as_float(e[j] << 16) * inv, __uint_as_float(e[j] & 0xFFFF0000u) * inv);
+    dst[p] = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 
