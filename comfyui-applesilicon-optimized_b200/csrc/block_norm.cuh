@@ -333,7 +333,9 @@ __device__ __forceinline__ void fold_mods(const NormArgs& a, int64_t mod, int c,
 template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
 __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(const NormArgs a) {
   extern __shared__ float4 folded[];
-  __shared__ float bufs[3][2][32];
+  // by row parity: with one barrier per norm a fast warp may already be writing the next
+  // row's sums while a slow one reads this row's
+  __shared__ float bufs[2][3][2][32];
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
     if (AFTER) {
 #pragma unroll
       for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(y0[k], v[k]);
-      row_norm<NPT, FULL>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[0]);
+      row_norm<NPT, FULL>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][0]);
 #pragma unroll
       for (int k = 0; k < NPT; ++k) {
         if (FULL || on[k]) {
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
       for (int k = 0; k < NPT; ++k) unpack8<DTYPE>(x0[k], v[k]);
     }
     if (!QUANT && !a.out) continue;
-    row_norm<NPT, FULL>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[1]);
+    row_norm<NPT, FULL>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][1]);
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
@@ -447,9 +449,9 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
       }
     if (!QUANT) continue;
     top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) bufs[2][row & 1][warp] = __uint_as_float(top);
+    if (lane == 0) bufs[row & 1][2][0][warp] = __uint_as_float(top);
     __syncthreads();
-    top = __reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(bufs[2][row & 1][lane]) : 0u);
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(bufs[row & 1][2][0][lane]) : 0u);
     // a row holding inf or NaN gets a NaN scale
     const float t = __uint_as_float(top);
     const float s = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);

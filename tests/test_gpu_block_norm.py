@@ -171,6 +171,32 @@ def test_many_rows_streams_and_ops(native):
     assert bn.norm_modulate(x[:0]).shape == (0, 1024)
 
 
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("post_kind", ["none", "layer"])
+def test_rows_of_a_persistent_cta_stay_apart(native, quant, post_kind):
+    """Tens of thousands of rows of very different sizes through persistent CTAs: each
+    equals the same row computed alone, every time."""
+    g = torch.Generator().manual_seed(11)
+    rows, D = 30000, 1024
+    size = torch.logspace(-2, 2, 97)[torch.randint(0, 97, (rows,), generator=g)][:, None]
+    x = (torch.randn(rows, D, generator=g) * size).to(torch.bfloat16).to(DEV)
+    y = (torch.randn(rows, D, generator=g) * size.flip(0)).to(torch.bfloat16).to(DEV)
+    f = bn.gated_residual_norm_quant_i8 if quant else bn.gated_residual_norm
+    args = (None, None, post_kind, 1.0, None, None, None, "layer")
+    got = f(x, y, *args)
+    # a few rows at a time: the form of one row per CTA
+    pick = torch.arange(0, rows, 101)
+    alone = [torch.cat(t) for t in zip(*(f(x[p], y[p], *args) for p in pick.split(200)))]
+    for a, b in zip(got, alone):
+        if a.dtype == torch.int8:
+            assert int((a[pick].int() - b.int()).abs().max()) <= 1
+        else:  # the sums' order differs between the forms
+            assert bool(((a[pick].double() - b.double()).abs()
+                         <= 2.0 ** -7 * b.double().abs() + 2.0 ** -13 * size.to(DEV)[pick]).all())
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(got, f(x, y, *args)))
+
+
 def test_refusals(native):
     a = make(6, 64, torch.bfloat16, 2)
     x, y, g, w = d(a["x"]), d(a["y"]), d(a["gate"]), d(a["weight"])
