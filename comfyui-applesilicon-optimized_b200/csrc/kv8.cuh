@@ -54,10 +54,10 @@ constexpr int kKvThreads = 256;
 
 // One CTA per (block, head, sequence, K or V).  NV: 8-value vectors a thread
 // holds (T * D <= 2048 * NV).  Bound: HBM; the quotient x / scale is a product with
-// the scale's reciprocal (within 2^-23 of it, so a code differs from the quotient's
-// nearest integer only where that is a tie to seven digits), and the nearest integer
-// is the low byte of its sum with 1.5 * 2^23: division and clamping cost twice the
-// memory's time.
+// the scale's reciprocal and one correction by its remainder, which gives the rounded
+// quotient (16-bit values are often exact ties, half of the block's largest among them),
+// and the nearest integer is the low byte of its sum with 1.5 * 2^23: the divide's
+// branches and the clamping cost twice the memory's time.
 template <typename T, int NV>
 __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendArgs a) {
   __shared__ uint32_t wmax[kKvThreads / 32];
@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const uint16_t e = static_cast<uint16_t>(u[j >> 1] >> (16 * (j & 1)));
-        o[j] = __float_as_uint(fmaf(to_float<T>(*reinterpret_cast<const T*>(&e)), inv, 12582912.0f));
+        const float x = to_float<T>(*reinterpret_cast<const T*>(&e)), y = x * inv;
+        o[j] = __float_as_uint(fmaf(fmaf(-y, s, x), inv, y) + 12582912.0f);
       }
       *reinterpret_cast<uint2*>(codes + i * 8) =
           make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));

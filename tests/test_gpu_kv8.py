@@ -198,6 +198,24 @@ def test_attention_nonfinite(native):
     assert bool(out[:, 2:].isnan().all()) and torch.equal(out[:, :2], clean[0][:, :2])
 
 
+def test_append_ties(native):
+    """x = half of the block's largest value is code 63.5, an exact tie: it rounds as
+    the quotient does, to 64."""
+    kc, vc, ks, vs, table = dev(*pool(1, 1, 16, 64, 1))
+    x = torch.zeros(1, 1, 16, 64, dtype=torch.float16)
+    for i in range(16):
+        x[0, 0, i, 0] = 1.0 + i / 16
+    top = x.amax()
+    x[0, 0, :, 1] = top / 2
+    x[0, 0, :, 2] = -top / 2
+    d = x.to(DEV)
+    kv8.kv8_append(d, d, kc, vc, ks, vs, table, i32(0).to(DEV))
+    codes = kc[int(table[0, 0]), 0].cpu()
+    s = (top.float() / torch.tensor(127.0))
+    want = (x[0, 0].float() / s).round().clamp(-127, 127).to(torch.int8)
+    assert torch.equal(codes, want)
+
+
 def test_bad_pages_are_flagged_and_skipped(native):
     """Out-of-range page numbers inside the length: checked in the kernels, no access."""
     kc, vc, ks, vs, table = pool(1, 1, 16, 64, 4, seed=8)
