@@ -38,7 +38,13 @@ struct PfSmem {
   alignas(1024) uint8_t q[RT][kPfRows * D * 2];   // D / 64 atoms of 128 rows x 128 bytes
   alignas(1024) uint8_t k[NB][64 * D * 2];        // D / 64 atoms of 64 rows x 128 bytes
   alignas(1024) uint8_t v[NB][64 * D * 2];
-  uint64_t k_full[NB], k_empty[NB], v_full[NB], v_empty[NB], s_full[RT], p_full[RT], o_done[RT];
+  uint64_t k_full[NB], k_empty[NB], v_full[NB], v_empty[NB];
+  // the last P V has its own: the last scores only say that the last but one's is issued,
+  // and one parity cannot tell "two to go" from "done"
+  uint64_t o_done[RT], o_last[RT];
+  // by S buffer: one side may be a whole stage ahead of the other, and a wait tells only
+  // the last phase from the one before
+  uint64_t s_full[RT][2], p_full[RT][2];
   uint32_t tmem;
 };
 template <int D, int RT>
@@ -122,9 +128,12 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       mbar_init(&sm.v_empty[i], 1);
     }
     for (int i = 0; i < RT; ++i) {
-      mbar_init(&sm.p_full[i], 4);
-      mbar_init(&sm.s_full[i], 1);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&sm.p_full[i][j], 4);
+        mbar_init(&sm.s_full[i][j], 1);
+      }
       mbar_init(&sm.o_done[i], 1);
+      mbar_init(&sm.o_last[i], 1);
     }
   }
   if (warp == kSoft + 5) {
@@ -202,33 +211,35 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
         const uint64_t dk = make_sw128_desc(smem_u32(sm.k[kb]));
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
+          // stage j - 2's P V still reads P from this buffer until it has completed: only
+          // MMAs on one accumulator are ordered by themselves
+          if (j >= 2 && !mbar_wait(&sm.o_done[r], j & 1, abort)) return false;
           const uint64_t dq = make_sw128_desc(smem_u32(sm.q[r]));
 #pragma unroll
           for (int s = 0; s < D / 16; ++s)
             umma_ss<MmaKind::F16>(tmem + 128 * r + 64 * (j & 1), dq + (s >> 2) * (kPfRows * 128 >> 4) + (s & 3) * 2,
                                   dk + (s >> 2) * (64 * 128 >> 4) + (s & 3) * 2, iqk, s > 0);
-          umma_commit(&sm.s_full[r]);
+          umma_commit(&sm.s_full[r][j & 1]);
         }
         umma_commit(&sm.k_empty[kb]);
         return true;
       };
       bool live = n_tiles > 0 && scores(0);
       for (int j = 0; live && j < n_tiles; ++j) {
-        // (its buffers were last read by stage j - 1's P V, which is ahead in the pipe)
         if (j + 1 < n_tiles && !scores(j + 1)) break;
         const int vb = j % NB;
         live = mbar_wait(&sm.v_full[vb], (j / NB) & 1, abort);
         const uint64_t dv = pf_nmajor_desc(smem_u32(sm.v[vb]), 64 * 128);
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          live = live && mbar_wait(&sm.p_full[r], j & 1, abort);
+          live = live && mbar_wait(&sm.p_full[r][j & 1], (j >> 1) & 1, abort);
           if (live) {
             tc_fence_after();
             const uint32_t tm_p = tmem + 128 * r + 64 * (j & 1);
 #pragma unroll
             for (int s = 0; s < 4; ++s)
               pf_umma_ts(tmem + 128 * (RT + r), tm_p + s * 8, dv + s * (16 * 128 >> 4), ipv, j > 0 || s > 0);
-            umma_commit(&sm.o_done[r]);
+            umma_commit(j + 1 < n_tiles ? &sm.o_done[r] : &sm.o_last[r]);
           }
         }
         if (live) umma_commit(&sm.v_empty[vb]);
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&ring->empty[st]);
       const uint32_t tm_s = tmem + 128 * rt + 64 * (j & 1) + lane_base;
-      if (!mbar_wait_warp(&sm.s_full[rt], j & 1, abort)) break;
+      if (!mbar_wait_warp(&sm.s_full[rt][j & 1], (j >> 1) & 1, abort)) break;
       tc_fence_after();
       uint32_t s0[32], s1[32];
       tmem_ld32(tm_s, s0);
@@ -360,11 +371,10 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       pf_tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full[rt]);
+      if (lane == 0) mbar_arrive(&sm.p_full[rt][j & 1]);
     }
     // ---- O: the last P V has to complete; every lane stores its own row
-    bool good = true;
-    if (n_tiles > 0) good = mbar_wait_warp(&sm.o_done[rt], (n_tiles - 1) & 1, abort);
+    const bool good = n_tiles == 0 || mbar_wait_warp(&sm.o_last[rt], 0, abort);
     tc_fence_after();
     const bool stored = r0 + tid < rows && good;
     const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;

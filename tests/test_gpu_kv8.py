@@ -198,6 +198,26 @@ def test_attention_nonfinite(native):
     assert bool(out[:, 2:].isnan().all()) and torch.equal(out[:, :2], clean[0][:, :2])
 
 
+@pytest.mark.parametrize("H,G,Tq", [(2, 5, 129), (2, 8, 9), (2, 8, 1)])
+def test_attention_repeats_bit_for_bit(native, H, G, Tq):
+    """Many launches of a pipelined kernel, other work in between: the same bits each
+    time, and no wait ever ran out."""
+    c = dev(*pool(3, H, 64, 128, 30, seed=12))
+    q = torch.randn(3, H * G, Tq, 128).to(torch.float16).to(DEV)
+    lens = i32(1900, 1333, 700).to(DEV)
+    native.device_status(reset=True)
+    first = kv8.kv8_attention(q, *c, lens)
+    noise = torch.randn(1 << 20, device=DEV)
+    for i in range(300):
+        if i % 3 == 0:
+            noise.mul_(1.0001)
+        again = kv8.kv8_attention(q, *c, lens)
+        if i % 20 == 0:
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    assert torch.equal(first[0], again[0])
+    assert native.device_status() == 0
+
+
 def test_append_ties(native):
     """x = half of the block's largest value is code 63.5, an exact tie: it rounds as
     the quotient does, to 64."""
