@@ -223,12 +223,12 @@ __global__ void __launch_bounds__(kKvThreads) kv8_gather_kernel(const Kv8GatherA
 // of it below).
 //
 // Softmax, online, base 2.  With sigma = q.k_code * ks * scale * log2 e and vs the
-// block's V scale, the weights kept are P = 2^(sigma + log2 vs - m) <= 1, m the
-// running maximum of that exponent; then
+// block's V scale, the weights kept are P = 2^(sigma + log2 vs - m) <= 2^15, m the
+// running maximum of that exponent less 15; then
 //   out = sum P * v_code / sum P / vs,
 // so V's scales cost one add per score instead of a pass over the accumulators,
 // and P fits fp16 whatever the scales are: P's fp16 rounding (2^-11 relative,
-// 2^-25 of the row's largest weight at least) is the only one before the
+// 2^-40 of the row's largest weight at least) is the only one before the
 // output's.  A block with vs = 0 adds its P to the sum only.
 //
 // Layout, D = 128: lane (g, t) loads 32 consecutive bytes (quarter t) of K token
@@ -338,6 +338,11 @@ __device__ __forceinline__ uint32_t q_pair(uint32_t raw, int f16, float inv) {
   return pack_f16x2(a * inv, b * inv);
 }
 
+// A row's m is its largest exponent less this: P <= 2^15 uses fp16's whole range, so
+// weights down to 2^-29 of the largest keep all their bits (P <= 1 loses bits below
+// 2^-14, which shows where blocks' V scales lie far apart).
+constexpr float kAttnHead = 15.0f;
+
 // log-sum-exp pieces of two halves of a row: (m, l) and the factors of each side.
 __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
   return m == -INFINITY ? 0.0f : ex2f(m - top);
@@ -380,8 +385,9 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     if (n == 0)
       for (int i = 0; i < min(many, ST); ++i) copy(i, i);
     float4 meta = make_float4(ks, 0.0f, 1.0f, 2.0f);
-    if (vs != 0.0f) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
-    if (page < 0) meta.w = 0.0f;
+    // below 2^-80 (values under 2^-73) a block counts as one of zeros: P / vs must not overflow
+    if (!(fabsf(vs) < 8.2718061e-25f)) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
+    if (page < 0) meta = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
     for (int i = 0; i < many; ++i, ++n) {
       const int s = n % ST;
       if (n >= ST) {
@@ -609,7 +615,7 @@ __global__ void __launch_bounds__(kAttnThreads)
     for (int r = 0; r < 2; ++r) {
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
       top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      const float mn = fmaxf(m[r], top[r]);
+      const float mn = fmaxf(m[r], top[r] - kAttnHead);
       corr[r] = safe_ex2_diff(m[r], mn);
       m[r] = mn;
       l[r] *= corr[r];
@@ -826,6 +832,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
     float top = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top -= kAttnHead;
     if (__any_sync(0xffffffffu, top > m)) {
       const float mn = fmaxf(m, top);
       const float corr = safe_ex2_diff(m, mn);

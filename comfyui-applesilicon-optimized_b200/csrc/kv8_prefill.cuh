@@ -4,8 +4,8 @@
 //
 // The mathematics is that of kv8.cuh: codes are exact in fp16, q's rows are scaled by
 // a power of two, the weights are P = 2^(sigma + log2 vs - m) and the sum of P / vs
-// divides at the end.  m is only raised when a row's maximum has grown by more than
-// 2^8 (P <= 256 fits fp16 as well as P <= 1 does), so the accumulator in TMEM is
+// divides at the end.  m starts 7 below a row's largest exponent and is only raised when
+// that has grown by more than 8 (P <= 2^15 fits fp16), so the accumulator in TMEM is
 // rarely rescaled.
 //
 // A CTA has RT row tiles of 128 (2 when there are more than 128 rows: K and V are
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
           add[i] = 0.0f;
         }
       }
-      if (__any_sync(0xffffffffu, top > m + 8.0f)) {
-        const float mn = fmaxf(m, top);
+      if (__any_sync(0xffffffffu, top > m + kAttnHead)) {
+        const float mn = fmaxf(m, top - (kAttnHead - 8.0f));
         const float corr = safe_ex2_diff(m, mn);
         m = mn;
         l *= corr;

@@ -198,6 +198,19 @@ def test_attention_nonfinite(native):
     assert bool(out[:, 2:].isnan().all()) and torch.equal(out[:, :2], clean[0][:, :2])
 
 
+@pytest.mark.parametrize("G,Tq", [(2, 3), (3, 5), (5, 8), (6, 40)])
+def test_attention_small_weights_keep_their_bits(native, G, Tq):
+    """Block scales over six decades: where the largest weight's code is near zero the
+    small ones make the value.  And a block of vanishing values (scale 1e-30)."""
+    kc, vc, ks, vs, table = pool(1, 2, 16, 64, 16, seed=4)
+    for seed in range(12):
+        g = torch.Generator().manual_seed(seed)
+        vs = torch.logspace(-6, 0, vs.numel())[torch.randperm(vs.numel(), generator=g)].reshape(vs.shape)
+        vs[int(table[0, 3])] = 1e-30
+        q = torch.randn(1, 2 * G, Tq, 64, generator=g).to(torch.bfloat16) * 2
+        run_attention(q, (kc, vc, ks * 3, vs, table), i32(250), True)
+
+
 @pytest.mark.parametrize("H,G,Tq", [(2, 5, 129), (2, 8, 9), (2, 8, 1)])
 def test_attention_repeats_bit_for_bit(native, H, G, Tq):
     """Many launches of a pipelined kernel, other work in between: the same bits each
