@@ -21,6 +21,8 @@
 // while one is reduced.
 #pragma once
 
+#include <type_traits>
+
 #include "digits.cuh"
 #include "numerics.cuh"
 #include "ptx.cuh"
@@ -116,7 +118,7 @@ __device__ __forceinline__ void store_vals16(void* p, int dtype, int64_t i, cons
 }
 
 // One CTA per row; thread i holds values i, i + threads, ...  The form for any D,
-// stride and alignment.
+// stride and alignment, used where a row is too long for the other two.
 template <int DTYPE, int VEC, int NPT>
 __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
   __shared__ float bufs[2][32];
@@ -236,8 +238,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
 // Rows of 8-value vectors, NPT per thread (16-byte aligned operands): thread i holds
 // vectors i, i + threads, ...; absent ones are zeros.  inv_n_w: 1 / this warp's values, n_l:
 // those of warp `lane`; buf: one pair of 32 words per norm in flight.
-template <int NPT, bool FULL>
-__device__ __forceinline__ void row_norm(float (&v)[NPT][8], int kind, const bool (&on)[NPT], float inv_n_w, float n_l,
+template <int NPT, bool FULL, int VEC = 8>
+__device__ __forceinline__ void row_norm(float (&v)[NPT][VEC], int kind, const bool (&on)[NPT], float inv_n_w, float n_l,
                                          float inv_n_l, float inv_d, float eps, float (*buf)[32]) {
   if (kind == kNormNone) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
@@ -247,7 +249,7 @@ __device__ __forceinline__ void row_norm(float (&v)[NPT][8], int kind, const boo
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += v[k][j];
+      for (int j = 0; j < VEC; ++j) s += v[k][j];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     mean_w = s * inv_n_w;
@@ -257,7 +259,7 @@ __device__ __forceinline__ void row_norm(float (&v)[NPT][8], int kind, const boo
   for (int k = 0; k < NPT; ++k)
     if (FULL || on[k]) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) q = fmaf(v[k][j] - mean_w, v[k][j] - mean_w, q);
+      for (int j = 0; j < VEC; ++j) q = fmaf(v[k][j] - mean_w, v[k][j] - mean_w, q);
     }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
@@ -283,7 +285,7 @@ __device__ __forceinline__ void row_norm(float (&v)[NPT][8], int kind, const boo
 #pragma unroll
   for (int k = 0; k < NPT; ++k)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[k][j] = (v[k][j] - mean) * r;
+    for (int j = 0; j < VEC; ++j) v[k][j] = (v[k][j] - mean) * r;
 }
 
 template <int DTYPE>
@@ -467,6 +469,170 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
         for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(fmaf(v[k][j], inv, 12582912.0f));
         *reinterpret_cast<uint2*>(a.q + row * a.ldq + col[k]) =
             make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));
+      }
+  }
+}
+
+// ---------------------------------------------------------------- other rows
+// The same for rows that 16-byte vectors do not fit (odd D, strides, views): VW = 2 values
+// per access when every row starts on a pair, else one.  Step s of thread i holds columns
+// (s * threads + i) * VW ..., so a warp's accesses are contiguous; persistent CTAs, the
+// folded vectors in shared memory, the next row's loads in flight, as above.
+constexpr int kLooseValues = 16;  // per thread
+template <int DTYPE, int VW, bool QUANT, bool AFTER>
+__global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a) {
+  constexpr int S = kLooseValues / VW;
+  using Raw = typename std::conditional<VW == 2, uint32_t, uint16_t>::type;
+  extern __shared__ float4 folded[];
+  float* const fold = reinterpret_cast<float*>(folded);  // w * (1 + scale), shift, gate * post_w
+  __shared__ float bufs[2][3][2][32];                    // by row parity, as above
+  griddep_wait();
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const float inv_d = 1.0f / static_cast<float>(a.D);
+  bool on[S];
+  int nw = 0, nl = 0;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    on[s] = static_cast<int>(s * blockDim.x + threadIdx.x) * VW < a.D;
+    nw += min(max(a.D - static_cast<int>(s * blockDim.x + warp * 32) * VW, 0), 32 * VW);
+    nl += min(max(a.D - static_cast<int>(s * blockDim.x + lane * 32) * VW, 0), 32 * VW);
+  }
+  auto col = [&](int s) { return static_cast<int>(s * blockDim.x + threadIdx.x) * VW; };
+  const float n_l = static_cast<float>(max(nl, 1)), inv_n_l = 1.0f / n_l, inv_n_w = 1.0f / static_cast<float>(max(nw, 1));
+  const int64_t r0 = static_cast<int64_t>(a.rows) * blockIdx.x / gridDim.x;
+  const int64_t r1 = static_cast<int64_t>(a.rows) * (blockIdx.x + 1) / gridDim.x;
+  Raw xn[S], yn[S];  // the row after this one
+  const uint16_t* xp = static_cast<const uint16_t*>(a.x) + r0 * a.ldx;
+  const uint16_t* yp = static_cast<const uint16_t*>(a.y) + r0 * a.ldy;
+  auto fetch = [&]() {
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      xn[s] = yn[s] = 0;
+      if (on[s]) {
+        xn[s] = __ldg(reinterpret_cast<const Raw*>(xp + col(s)));
+        if (AFTER) yn[s] = __ldg(reinterpret_cast<const Raw*>(yp + col(s)));
+      }
+    }
+    xp += a.ldx;
+    yp += a.ldy;
+  };
+  auto unpack = [](Raw u, float (&v)[VW]) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+      const uint16_t e = static_cast<uint16_t>(u >> (16 * j));
+      v[j] = DTYPE == kBiasBF16 ? __uint_as_float(static_cast<uint32_t>(e) << 16) : __half2float(__ushort_as_half(e));
+    }
+  };
+  auto store = [&](uint16_t* p, const float (&v)[VW]) {
+    if constexpr (VW == 2)
+      *reinterpret_cast<uint32_t*>(p) = DTYPE == kBiasBF16 ? pack_bf16x2(v[0], v[1]) : pack_f16x2(v[0], v[1]);
+    else
+      store_vals16<1>(p, DTYPE, 0, v);
+  };
+  if (r0 < r1) fetch();
+  int64_t mod_end = r0;  // the first row that needs other vectors
+  for (int64_t row = r0; row < r1; ++row) {
+    Raw x0[S], y0[S];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      x0[s] = xn[s];
+      y0[s] = yn[s];
+    }
+    if (row + 1 < r1) fetch();
+    if (row >= mod_end) {  // a thread writes and reads its own columns
+      const int64_t mod = row / a.rows_per_mod;
+      mod_end = (mod + 1) * a.rows_per_mod;
+      float u[S][VW], t[S][VW];
+      auto read = [&](const void* p, int dtype, int64_t at, float none, float (&to)[S][VW]) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) {
+            float one[1] = {none};
+            if (p && on[s]) load_vals<1>(p, dtype, at + col(s) + j, one);
+            to[s][j] = one[0];
+          }
+      };
+      auto keep = [&](int which) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int j = 0; j < VW; ++j)
+            if (on[s]) fold[which * a.D + col(s) + j] = u[s][j];
+      };
+      auto times = [&](float plus) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int j = 0; j < VW; ++j) u[s][j] *= plus + t[s][j];
+      };
+      read(a.w, a.w_dtype, 0, 1.0f, u);
+      read(a.scale, a.mod_dtype, mod * a.ld_scale, 0.0f, t);
+      times(1.0f);
+      keep(0);
+      read(a.shift, a.mod_dtype, mod * a.ld_shift, 0.0f, u);
+      keep(1);
+      if (AFTER) {
+        read(a.post_w, a.post_w_dtype, 0, 1.0f, u);
+        read(a.gate, a.mod_dtype, mod * a.ld_gate, 1.0f, t);
+        times(0.0f);
+        keep(2);
+      }
+    }
+    float v[S][VW];
+    if (AFTER) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) unpack(y0[s], v[s]);
+      row_norm<S, false, VW>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][0]);
+      uint16_t* hp = static_cast<uint16_t*>(a.h) + row * a.ldh;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        float u[VW];
+        unpack(x0[s], u);
+#pragma unroll
+        for (int j = 0; j < VW; ++j)
+          v[s][j] = on[s] ? fmaf(a.res_scale, u[j], v[s][j] * fold[2 * a.D + col(s) + j]) : 0.0f;
+        if (a.h && on[s]) store(hp + col(s), v[s]);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < S; ++s) unpack(x0[s], v[s]);
+    }
+    if (!QUANT && !a.out) continue;
+    row_norm<S, false, VW>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][1]);
+    uint16_t* op = static_cast<uint16_t*>(a.out) + row * a.ldo;
+    uint32_t top = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (on[s]) {
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+          v[s][j] = fmaf(v[s][j], fold[col(s) + j], fold[a.D + col(s) + j]);
+          if (QUANT) top = max(top, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);  // as bits: NaN sorts above
+        }
+        if (!QUANT) store(op + col(s), v[s]);
+      }
+    if (!QUANT) continue;
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) bufs[row & 1][2][0][warp] = __uint_as_float(top);
+    __syncthreads();
+    top = __reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(bufs[row & 1][2][0][lane]) : 0u);
+    const float t = __uint_as_float(top);
+    const float sc = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);
+    if (threadIdx.x == 0) a.q_scale[row] = sc;
+    const float inv = sc > 0.0f ? fminf(__fdiv_rn(1.0f, sc), 3.402823466e38f) : 0.0f;  // as above
+    int8_t* qp = a.q + row * a.ldq;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (on[s]) {
+        uint32_t o[VW];
+#pragma unroll
+        for (int j = 0; j < VW; ++j) o[j] = __float_as_uint(fmaf(v[s][j], inv, 12582912.0f));
+        if constexpr (VW == 2)
+          *reinterpret_cast<uint16_t*>(qp + col(s)) = static_cast<uint16_t>(__byte_perm(o[0], o[1], 0x0040));
+        else
+          qp[col(s)] = static_cast<int8_t>(o[0]);
       }
   }
 }

@@ -165,11 +165,8 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
 }
 
 // PERSIST: as many CTAs as are resident at once (at most one per row).
-template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
-int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
-  auto kern = block_norm_rows_kernel<DTYPE, PERSIST, NPT, FULL, QUANT, AFTER>;
-  if (!PERSIST) return launch(kern, dim3(static_cast<unsigned>(a.rows)), threads, 0, 1, st, a);
-  const int smem = (AFTER ? 3 : 2) * a.D * 4;
+template <typename K>
+int launch_persistent(K kern, const NormArgs& a, int threads, int smem, int sms, cudaStream_t st) {
   int per_sm = 0;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
       cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, threads, smem) != cudaSuccess || per_sm < 1) {
@@ -178,6 +175,20 @@ int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
   }
   const int64_t ctas = int64_t(sms) * per_sm;
   return launch(kern, dim3(static_cast<unsigned>(a.rows < ctas ? a.rows : ctas)), threads, smem, 1, st, a);
+}
+template <int DTYPE, int VW>
+int launch_norm_loose(const NormArgs& a, int sms, cudaStream_t st) {
+  const int threads = static_cast<int>(cdiv(cdiv(a.D, kLooseValues), 32) * 32), smem = (a.y ? 3 : 2) * a.D * 4;
+  if (a.y) return a.q ? launch_persistent(block_norm_loose_kernel<DTYPE, VW, true, true>, a, threads, smem, sms, st)
+                      : launch_persistent(block_norm_loose_kernel<DTYPE, VW, false, true>, a, threads, smem, sms, st);
+  return a.q ? launch_persistent(block_norm_loose_kernel<DTYPE, VW, true, false>, a, threads, smem, sms, st)
+             : launch_persistent(block_norm_loose_kernel<DTYPE, VW, false, false>, a, threads, smem, sms, st);
+}
+template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
+int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
+  auto kern = block_norm_rows_kernel<DTYPE, PERSIST, NPT, FULL, QUANT, AFTER>;
+  if (PERSIST) return launch_persistent(kern, a, threads, (AFTER ? 3 : 2) * a.D * 4, sms, st);
+  return launch(kern, dim3(static_cast<unsigned>(a.rows)), threads, 0, 1, st, a);
 }
 template <int DTYPE, bool PERSIST, int NPT, bool FULL>
 int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
@@ -193,11 +204,11 @@ int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
 }
 // Aligned rows of up to 8192 values: one row per CTA and one 8-value vector per thread
 // while all rows find a place at once, else persistent CTAs with four vectors per
-// thread (two for short rows: fewer reductions per value, more CTAs per SM).  Anything
-// else takes the form that holds 8 or 32 single values per thread.
+// thread (two for short rows: fewer reductions per value, more CTAs per SM).  Other rows
+// of up to 8192 values: persistent CTAs, by pairs or single values.  Longer ones take the
+// form of 32 single values per thread.
 template <int DTYPE>
-int launch_norm(const NormArgs& a, bool vec, int sms, cudaStream_t st) {
-  const dim3 rows(static_cast<unsigned>(a.rows));
+int launch_norm(const NormArgs& a, bool vec, bool pairs, int sms, cudaStream_t st) {
   if (vec && a.D <= 8192) {
     const int vecs = a.D / 8;
     if (a.rows <= 2 * int64_t(sms))
@@ -208,9 +219,9 @@ int launch_norm(const NormArgs& a, bool vec, int sms, cudaStream_t st) {
     return npt == 4 ? launch_norm_rows<DTYPE, true, 4>(a, threads, sms, st)
                     : launch_norm_rows<DTYPE, true, 2>(a, threads, sms, st);
   }
-  auto threads = [&](int npt) { return static_cast<int>(cdiv(cdiv(a.D, npt), 32) * 32); };
-  if (a.D <= 8 * 512) return launch(block_norm_kernel<DTYPE, 1, 8>, rows, threads(8), 0, 1, st, a);
-  return launch(block_norm_kernel<DTYPE, 1, 32>, rows, threads(32), 0, 1, st, a);
+  if (a.D <= 8192) return pairs ? launch_norm_loose<DTYPE, 2>(a, sms, st) : launch_norm_loose<DTYPE, 1>(a, sms, st);
+  return launch(block_norm_kernel<DTYPE, 1, 32>, dim3(static_cast<unsigned>(a.rows)),
+                static_cast<int>(cdiv(cdiv(a.D, 32), 32) * 32), 0, 1, st, a);
 }
 
 // ------------------------------------------------------------ 8-bit cache
@@ -457,7 +468,11 @@ int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int
                    ok(gate, ld_gate) && ok(scale, ld_scale) && ok(shift, ld_shift) &&
                    ok(post_w, 0) && ok(w, 0) && (!q || (aligned(q, 8) && ldq % 8 == 0));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return dtype == B200Q_F16 ? launch_norm<kBiasF16>(a, vec, sms, st) : launch_norm<kBiasBF16>(a, vec, sms, st);
+  auto even = [](const void* p, int64_t ld, size_t bytes) { return !p || (aligned(p, bytes) && ld % 2 == 0); };
+  const bool pairs = D % 2 == 0 && even(x, ldx, 4) && even(y, ldy, 4) && even(h, ldh, 4) && even(out, ldo, 4) &&
+                     even(q, ldq, 2);
+  return dtype == B200Q_F16 ? launch_norm<kBiasF16>(a, vec, pairs, sms, st)
+                            : launch_norm<kBiasBF16>(a, vec, pairs, sms, st);
 }
 
 int b200q_kv8_append(const void* k, const void* v, int dtype, int64_t B, int64_t S,
