@@ -269,6 +269,7 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
     const int rt = warp >> 2;  // this warp's row tile; it may touch lanes 32 (warp % 4) ..
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tm_o = tmem + 128 * (RT + rt) + lane_base;
+    const bool idle = r0 + 32 * warp >= rows;
     for (int j = 0; j < n_tiles; ++j) {
       const int st = j % ST;
       if (!mbar_wait_warp(&ring->full[st], (j / ST) & 1, abort)) break;
@@ -279,6 +280,11 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
       if (lane == 0) mbar_arrive(&ring->empty[st]);
       const uint32_t tm_s = tmem + 128 * rt + 64 * (j & 1) + lane_base;
       if (!mbar_wait_warp(&sm.s_full[rt][j & 1], (j >> 1) & 1, abort)) break;
+      if (idle) {  // no row of this warp is stored: its lanes of P may hold anything
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[rt][j & 1]);
+        continue;
+      }
       tc_fence_after();
       uint32_t s0[32], s1[32];
       tmem_ld32(tm_s, s0);
