@@ -959,12 +959,11 @@ bool tmap_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, u
   return make_tmap(map, base, CU_TENSOR_MAP_DATA_TYPE_UINT8, cols, rows, ld_bytes, box_cols, box_rows, swizzle);
 }
 
-int gemm16_scaled(bool f16, const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M,
-                  int64_t N, int64_t K, const EpiArgs& ep, cudaStream_t st) {
+int gemm_f16_scaled(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M, int64_t N,
+                    int64_t K, const EpiArgs& ep, cudaStream_t st) {
   const DeviceInfo* d = current_device();
   if (!d) return B200Q_ERR_UNSUPPORTED;
-  if (f16) return gemm16<MmaKind::F16, kEpiScaled>(d, a, lda, w, ldw, M, N, K, ep, st);
-  return gemm16<MmaKind::BF16, kEpiScaled>(d, a, lda, w, ldw, M, N, K, ep, st);
+  return gemm16<MmaKind::F16, kEpiScaled>(d, a, lda, w, ldw, M, N, K, ep, st);
 }
 
 }  // namespace host

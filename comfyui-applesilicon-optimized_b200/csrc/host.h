@@ -25,11 +25,11 @@ bool tmap_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, u
 // The status word of lowbit.cu's kernels on the current device (read, and
 // cleared when `reset`); b200q_get_device_status merges it with capi.cu's.
 int lowbit_device_status(unsigned int* status, bool reset);
-// out = epilogue(a . w^T) with a [M, K] and w [N, K] both bf16 (f16 = false) or
-// fp16, on the CTA-pair / single-CTA kind::f16 tile kernels.  16-byte aligned
-// operands and row strides, K % 8 == 0; `ep` as for the FP8 scaled epilogue.
-int gemm16_scaled(bool f16, const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M,
-                  int64_t N, int64_t K, const EpiArgs& ep, cudaStream_t st);
+// out = epilogue(a . w^T) with a [M, K] and w [N, K] fp16, on the CTA-pair / single-CTA
+// kind::f16 tile kernels.  16-byte aligned operands and row strides, K % 8 == 0; `ep` as
+// for the FP8 scaled epilogue.
+int gemm_f16_scaled(const void* a, int64_t lda, const void* w, int64_t ldw, int64_t M, int64_t N,
+                    int64_t K, const EpiArgs& ep, cudaStream_t st);
 
 }  // namespace host
 }  // namespace b200q

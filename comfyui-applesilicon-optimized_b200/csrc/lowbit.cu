@@ -4,10 +4,13 @@
 // the host before any launch, nothing is allocated, nothing synchronises, and
 // kernels go to the caller's stream as programmatic dependents.
 #include "../../include/b200q.h"
+#include <algorithm>
+
 #include "block_norm.cuh"
 #include "host.h"
 #include "kv8.cuh"
 #include "kv8_prefill.cuh"
+#include "w4_tile.cuh"
 #include "w4a16.cuh"
 
 using namespace b200q;
@@ -66,9 +69,8 @@ int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, 
 }
 
 // ------------------------------------------------------------ 4-bit linear
-// Largest M of the warp-MMA kernels, which run 32 tokens at a time; above it the
-// weight is decoded once per call for the tile GEMM.
-constexpr int64_t kW4MaxSmallM = 64;
+// Largest M of the warp-MMA kernels, whose products are exact.
+constexpr int64_t kW4MaxSmallM = 32;
 
 // K slices and row parts of the slice kernel: the split whose busiest warp has the
 // fewest groups to go through, x's slice beside the rings.
@@ -95,8 +97,14 @@ bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, int max_slices, Ws
   }
   return best >= 0;
 }
-// The slices' sums for one launch of at most 32 tokens.
-size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(kWsMaxSlices) * (M < 32 ? M : 32) * N * 4; }
+size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(kWsMaxSlices) * M * N * 4; }
+
+int launch_join(const float* part, int slices, int64_t ld, const EpiArgs& ep, cudaStream_t st) {
+  const int64_t chunks = cdiv(ep.N, 256);
+  if (ep.M * chunks > kIntMax) return B200Q_ERR_UNSUPPORTED;
+  return launch(w4_join_kernel, dim3(static_cast<unsigned>(ep.M * chunks)), 256, 0, 1, st, part, slices, ld,
+                static_cast<int>(chunks), ep);
+}
 
 template <int LW>
 int launch_slice_cols(const W4SliceArgs& a, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
@@ -110,8 +118,7 @@ int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p
           : G == 64 ? launch_slice_cols<2>(a, ep, p, st)
                     : launch_slice_cols<4>(a, ep, p, st);
   if (s != B200Q_OK || !a.part) return s;
-  const dim3 grid(static_cast<unsigned>(cdiv(int64_t(a.M) * a.N, 256)));
-  return launch(w4_join_kernel, grid, 256, 0, 1, st, static_cast<const float*>(a.part), a.slices, ep);
+  return launch_join(a.part, a.slices, a.N, ep, st);
 }
 
 // The integer kernel for few tokens, when x's digits fit beside the rings: at most
@@ -151,8 +158,13 @@ int launch_digits(const W4DigitArgs& a, int G, const EpiArgs& ep, const WdPlan& 
   return launch_digits_cols<T, 4>(a, ep, p, st);
 }
 
+// Rows of N % 8 != 0 outputs start off the tile GEMM's vector stores (its element stores, a
+// row per lane, took 35 us for 144 x 4135): fp32 rows of a padded stride go to the
+// workspace instead, and the join kernel runs the epilogue from there.
+bool w4_joins(int64_t N) { return N % 8 != 0; }
+int64_t w4_join_ld(int64_t N) { return cdiv(N, 32) * 32; }
 struct W4Work {
-  size_t w, x, row, col, total;  // byte offsets
+  size_t w, x, row, col, out, total;  // byte offsets
 };
 W4Work w4_work(int64_t M, int64_t N, int64_t K) {
   auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
@@ -160,8 +172,110 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
   o.x = up(size_t(N) * K * 2);
   o.row = o.x + up(size_t(M) * K * 2);
   o.col = o.row + up(size_t(M) * 4);
-  o.total = o.col + up(size_t(N) * 4);
+  o.out = o.col + up(size_t(N) * 4);
+  o.total = o.out + (w4_joins(N) ? up(size_t(M) * w4_join_ld(N) * 4) : 0);
   return o;
+}
+
+// 33 to 256 tokens: one token tile of the tile kernel.  (Measured at K 5120, N 13824: 64 tokens
+// 52 us, 64 on the slice kernel in two passes; 256 tokens 69 us, 80 decoded; K 13824, N 5120:
+// 200 tokens 58 us, 129 decoded.  With more token tiles the weight is decoded again for each,
+// and the decoded copy with the pair GEMM is ahead: 300 tokens 101 us, 164 by tiles.)
+constexpr int64_t kW4MaxTileM = 256;
+bool w4_tiles(int64_t M, int64_t N, int64_t K) {
+  return M > kW4MaxSmallM && M <= kW4MaxTileM && N <= (int64_t(1) << 30) && K <= (int64_t(1) << 24);
+}
+// K slices of the tile kernel: the split with the lowest estimate, in cycles.  A slot takes four
+// times the longest of a stage's MMAs, its bytes from L2 and its decode; a tile its start and
+// store besides, and slices the sums' round trip and the join's launch.
+struct W4TilePlan {
+  int tn, slices;
+};
+constexpr int kW4TileMaxSlices = 16;
+W4TilePlan w4_tile_plan(int sms, int64_t M, int64_t N, int64_t K) {
+  const int64_t slots = cdiv(K, 256), tiles = cdiv(N, 128);
+  const int tn = M <= 64 ? 64 : M <= 128 ? 128 : 256;
+  const int64_t slot = 4 * std::max<int64_t>({2 * tn, (tn * 128 + 5120) / 64, 300});
+  W4TilePlan best{tn, 1};
+  int64_t least = -1;
+  for (int s = 1; s <= kW4TileMaxSlices && s <= slots; ++s) {
+    const int64_t cost = cdiv(tiles * s, sms ? sms : 148) * (cdiv(slots, s) * slot + 2000 + 16 * tn) +
+                         (s > 1 ? 4000 + s * M * N * 8 / 3000 : 0);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best.slices = s;
+    }
+  }
+  return best;
+}
+struct W4TileWork {
+  size_t x, x_pow, w_pow, sz, part, total;  // byte offsets
+};
+W4TileWork w4_tile_work(const W4TilePlan& p, int64_t M, int64_t N, int64_t K, int64_t G) {
+  auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
+  W4TileWork o{};
+  o.x_pow = up(size_t(M) * K * 2);
+  o.w_pow = o.x_pow + up(size_t(M) * 4);
+  o.sz = o.w_pow + up(size_t(N) * 4);
+  o.part = o.sz + up(size_t(cdiv(K, 256) * (256 / G)) * cdiv(N, 128) * 128 * 8);
+  o.total = o.part + (p.slices > 1 ? up(size_t(p.slices) * M * N * 4) : 0);
+  return o;
+}
+template <int TN, bool LO>
+int launch_tile(const CUtensorMap& tx, const CUtensorMap& tw, const W4TileArgs& a, const EpiArgs& ep, int64_t ctas,
+                cudaStream_t st) {
+  return launch(w4_tile_kernel<TN, LO>, dim3(static_cast<unsigned>(ctas)), kW4TileThreads, w4_tile_smem_bytes<TN>(), 1,
+                st, tx, tw, a, ep);
+}
+int launch_w4_tile(const W4TilePlan& p, const void* x, int x_dtype, int64_t ldx, bool x_vec, const uint8_t* w,
+                   int64_t ldw, const void* scales, int scale_dtype, const uint8_t* zeros, int64_t G, int64_t M,
+                   int64_t N, int64_t K, const EpiArgs& ep, uint8_t* base, cudaStream_t st) {
+  const W4TileWork o = w4_tile_work(p, M, N, K, G);
+  const int64_t slots = cdiv(K, 256), ctas = cdiv(N, 128) * p.slices;
+  W4TilePrepareArgs r{};
+  r.x = x;
+  r.ldx = ldx;
+  r.x_f16 = x_dtype == B200Q_F16;
+  r.x_vec = x_vec;
+  r.M = static_cast<int>(M);
+  r.K = static_cast<int>(K);
+  r.x16 = reinterpret_cast<__half*>(base + o.x);
+  r.x_pow = reinterpret_cast<float*>(base + o.x_pow);
+  r.scales = scales;
+  r.scale_dtype = scale_dtype;
+  r.zeros = zeros;
+  r.N = static_cast<int>(N);
+  r.KG = static_cast<int>(K / G);
+  r.groups = static_cast<int>(slots * (256 / G));
+  r.ldn = static_cast<int>(cdiv(N, 128) * 128);
+  r.sz = reinterpret_cast<uint2*>(base + o.sz);
+  r.w_pow = reinterpret_cast<float*>(base + o.w_pow);
+  r.group_blocks = static_cast<int>(cdiv(r.groups, kW4PrepGroups));
+  r.scale_blocks = r.ldn / kW4PrepRows * r.group_blocks;
+  int s = launch(w4_tile_prepare_kernel, dim3(static_cast<unsigned>(r.scale_blocks + M)), 256, 0, 1, st, r);
+  if (s != B200Q_OK) return s;
+  CUtensorMap tx, tw;
+  if (!host::tmap_u8(&tx, r.x16, uint64_t(2 * K), uint64_t(M), uint64_t(2 * K), 128, static_cast<uint32_t>(p.tn),
+                     CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !host::tmap_u8(&tw, w, uint64_t(K / 2), uint64_t(N), uint64_t(ldw), 128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+    return B200Q_ERR_CUDA;
+  W4TileArgs a{};
+  a.sz = r.sz;
+  a.ldn = r.ldn;
+  a.w_pow = r.w_pow;
+  a.x_pow = r.x_pow;
+  a.part = p.slices > 1 ? reinterpret_cast<float*>(base + o.part) : nullptr;
+  a.M = r.M;
+  a.N = r.N;
+  a.slots = static_cast<int>(slots);
+  a.log_g = G == 32 ? 5 : G == 64 ? 6 : 7;
+  a.slices = p.slices;
+  const bool lo = scale_dtype == kBiasF32;
+  if (p.tn == 64) s = lo ? launch_tile<64, true>(tx, tw, a, ep, ctas, st) : launch_tile<64, false>(tx, tw, a, ep, ctas, st);
+  else if (p.tn == 128) s = lo ? launch_tile<128, true>(tx, tw, a, ep, ctas, st) : launch_tile<128, false>(tx, tw, a, ep, ctas, st);
+  else s = lo ? launch_tile<256, true>(tx, tw, a, ep, ctas, st) : launch_tile<256, false>(tx, tw, a, ep, ctas, st);
+  if (s != B200Q_OK || p.slices == 1) return s;
+  return launch_join(a.part, p.slices, N, ep, st);
 }
 
 // PERSIST: as many CTAs as are resident at once (at most one per row).
@@ -306,6 +420,7 @@ extern "C" {
 
 size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (w4_tiles(M, N, K)) return w4_tile_work(w4_tile_plan(host::device_sms(), M, N, K), M, N, K, 32).total;
   if (M > kW4MaxSmallM) return w4_work(M, N, K).total;
   // the integer kernel for few tokens needs none
   const int sms = host::device_sms();
@@ -363,34 +478,28 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     return x_dtype == B200Q_F16 ? launch_digits<__half>(a, int(group), ep, wd, st)
                                 : launch_digits<__nv_bfloat16>(a, int(group), ep, wd, st);
   }
+  if (w4_tiles(M, N, K))
+    return launch_w4_tile(w4_tile_plan(sms, M, N, K), x, x_dtype, ldx, x_vec, w, ldw, scales, scale_dtype, zeros, group,
+                          M, N, K, ep, static_cast<uint8_t*>(workspace), st);
   WsPlan ws;
-  const int64_t step = M < 32 ? M : 32;
-  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, step, N, K, int(group), need ? kWsMaxSlices : 1, &ws)) {
-    for (int64_t m0 = 0; m0 < M; m0 += step) {
-      const int64_t rows = M - m0 < step ? M - m0 : step;
-      W4SliceArgs a{};
-      a.x = static_cast<const uint16_t*>(x) + m0 * ldx;
-      a.x_f16 = x_dtype == B200Q_F16;
-      a.ldx = ldx;
-      a.w = w;
-      a.ldw = ldw;
-      a.scales = scales;
-      a.scale_dtype = scale_dtype;
-      a.zeros = zeros;
-      a.part = ws.slices > 1 ? static_cast<float*>(workspace) : nullptr;
-      a.M = static_cast<int>(rows);
-      a.N = static_cast<int>(N);
-      a.K = static_cast<int>(K);
-      a.x_vec = x_vec;
-      a.slices = ws.slices;
-      a.parts = ws.parts;
-      EpiArgs e = ep;
-      e.M = static_cast<int>(rows);
-      e.out = static_cast<char*>(out) + m0 * ldo * (out_dtype == B200Q_F32 ? 4 : 2);
-      const int s = launch_slice(a, int(group), e, ws, st);
-      if (s != B200Q_OK) return s;
-    }
-    return B200Q_OK;
+  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, M, N, K, int(group), need ? kWsMaxSlices : 1, &ws)) {
+    W4SliceArgs a{};
+    a.x = x;
+    a.x_f16 = x_dtype == B200Q_F16;
+    a.ldx = ldx;
+    a.w = w;
+    a.ldw = ldw;
+    a.scales = scales;
+    a.scale_dtype = scale_dtype;
+    a.zeros = zeros;
+    a.part = ws.slices > 1 ? static_cast<float*>(workspace) : nullptr;
+    a.M = static_cast<int>(M);
+    a.N = static_cast<int>(N);
+    a.K = static_cast<int>(K);
+    a.x_vec = x_vec;
+    a.slices = ws.slices;
+    a.parts = ws.parts;
+    return launch_slice(a, int(group), ep, ws, st);
   }
   if (M <= kW4MaxSmallM) return B200Q_ERR_UNSUPPORTED;  // N * K / group above 2^31
   const W4Work o = w4_work(M, N, K);
@@ -423,9 +532,20 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     x = a.x16;
     ldx = K;
   }
-  const int s = launch(w4_prepare_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, st, a);
+  int s = launch(w4_prepare_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, st, a);
   if (s != B200Q_OK) return s;
-  return host::gemm16_scaled(true, x, ldx, a.w16, K, M, N, K, ep, st);
+  if (!w4_joins(N)) return host::gemm_f16_scaled(x, ldx, a.w16, K, M, N, K, ep, st);
+  EpiArgs sums = ep;
+  sums.out = base + o.out;
+  sums.ldo = w4_join_ld(N);
+  sums.out_dtype = kOutF32;
+  sums.bias = nullptr;
+  sums.bias_dtype = kBiasNone;
+  sums.act = kActNone;
+  s = host::gemm_f16_scaled(x, ldx, a.w16, K, M, N, K, sums, st);
+  if (s != B200Q_OK) return s;
+  ep.col_scale = ep.row_scale = nullptr;
+  return launch_join(static_cast<const float*>(sums.out), 1, sums.ldo, ep, st);
 }
 
 int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_t ldy, int dtype,

@@ -366,17 +366,18 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
   }
 }
 
-// Adds the slices of each output in order and runs the epilogue.
-__global__ void __launch_bounds__(256) w4_join_kernel(const float* __restrict__ part, int slices, const EpiArgs ep) {
+// Adds the slices of each output (fp32 [slices][M][ld]) in order and runs the epilogue;
+// grid M * chunks of 256 columns.
+__global__ void __launch_bounds__(256)
+    w4_join_kernel(const float* __restrict__ part, int slices, int64_t ld, int chunks, const EpiArgs ep) {
   griddep_wait();
   griddep_launch_dependents();
-  const int64_t total = static_cast<int64_t>(ep.M) * ep.N;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
+  const int m = blockIdx.x / chunks, n = (blockIdx.x - m * chunks) * 256 + threadIdx.x;
+  if (n >= ep.N) return;
+  const int64_t total = ep.M * ld, i = m * ld + n;
   float v = 0.0f;
 #pragma unroll 8
   for (int s = 0; s < slices; ++s) v += part[s * total + i];
-  const int m = static_cast<int>(i / ep.N), n = static_cast<int>(i - static_cast<int64_t>(m) * ep.N);
   store_out(ep, m, n, epi_scaled(v, 1.0f, 1.0f, 1.0f, ep, n));
 }
 

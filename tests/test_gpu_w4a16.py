@@ -57,6 +57,31 @@ def test_shapes(native, M, N, K, G, dtype):
     check(w4.w4a16_linear(*dev(x, w, s, z)), x, w, s, z, b)
 
 
+@pytest.mark.parametrize("M,N,K,G", [(33, 131, 32, 32), (64, 128, 256, 128), (65, 1001, 544, 32), (128, 5120, 5120, 64),
+                                     (129, 257, 5120, 128), (256, 1046, 1312, 32), (200, 515, 13824, 64),
+                                     (700, 1131, 1536, 128)])
+@pytest.mark.parametrize("scale_dtype", [torch.bfloat16, torch.float32])
+def test_tiles_of_tokens(native, M, N, K, G, scale_dtype):
+    """Tile edges in every direction; fp32 scales keep their bits; the same bits each time."""
+    x, w, s, z, b = make(M, N, K, G, torch.bfloat16, True, bias=True, scale_dtype=scale_dtype, seed=M)
+    d = dev(x, w, s, z, b)
+    native.device_status(reset=True)
+    out = w4.w4a16_linear(*d, "gelu_tanh")
+    check(out, x, w, s, z, b, "gelu_tanh")
+    for _ in range(20):
+        assert torch.equal(w4.w4a16_linear(*d, "gelu_tanh"), out)
+    assert native.device_status() == 0
+
+
+@pytest.mark.parametrize("M", [50, 150])
+def test_scales_far_apart_in_a_row(native, M):
+    """Each group's weights keep their own bits next to groups 2^12 larger."""
+    x, w, s, z, b = make(M, 48, 512, 64, torch.bfloat16, True, scale_dtype=torch.float32)
+    s = s * torch.logspace(-12, 0, 8, base=2)
+    x[:, 64:] = 0  # only the smallest group counts
+    check(w4.w4a16_linear(*dev(x, w, s, z)), x, w, s, z, b)
+
+
 @pytest.mark.parametrize("M", [4, 64])
 @pytest.mark.parametrize("act", ["gelu_tanh", "gelu"])
 @pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
