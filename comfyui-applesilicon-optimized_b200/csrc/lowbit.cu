@@ -121,13 +121,15 @@ int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p
   return launch_join(a.part, a.slices, a.N, ep, st);
 }
 
-// The integer kernel for few tokens, when x's digits fit beside the rings: at most
-// 24 digit columns, M * K up to about 20,000.
+// The integer kernel for few tokens, when x's digits fit beside the rings.  (Against the slice
+// kernel, N 5120, us: 1 token K 1536 4.4 / 7.8, K 5120 7.5 / 11.3; 2 tokens K 5120 10.3 / 11.8;
+// 3 tokens K 1536 7.3 / 7.9, K 2560 9.5 / 9.7, K 5120 14.4 / 11.7; 5 tokens K 1536 8.0 / 8.0;
+// 8 tokens K 1536 9.2 / 8.4: more than two tokens while M * K is small.)
 struct WdPlan {
   int smem, grid, threads;
 };
 bool wd_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WdPlan* p) {
-  if (M > 8 || M * K > 24 * 1024) return false;
+  if (M > 8 || M * K > (M <= 2 ? 24 : 8) * 1024) return false;
   const int nc = M <= 2 ? 1 : M <= 5 ? 2 : 3;
   int teams = wd_teams(nc);
   for (; teams > 0; --teams) {
@@ -317,7 +319,7 @@ int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
                                   : launch_norm_rows<DTYPE, PERSIST, NPT, false>(a, threads, sms, st);
 }
 // Aligned rows of up to 8192 values: one row per CTA and one 8-value vector per thread
-// while all rows find a place at once, else persistent CTAs with four vectors per
+// while all rows find a place at once (296 rows of 5120: 8.0 us, 297 persistent 8.3), else persistent CTAs with four vectors per
 // thread (two for short rows: fewer reductions per value, more CTAs per SM).  Other rows
 // of up to 8192 values: persistent CTAs, by pairs or single values.  Longer ones take the
 // form of 32 single values per thread.
@@ -381,6 +383,9 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
 // rounds of stages.  More than one leave fp32 partials for the join kernel.  (A cluster
 // of up to 16 CTAs joining over distributed shared memory was no faster: 8 heads x 2048
 // tokens 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
+// Row tiles: 8 rows of 32 x 4096 tokens take 71 us on their kernel, 9 rows 80 on the 16-row one and
+// 16 rows 84; a second 16-row tile would read the cache again, and 17 rows take 134 us on the
+// 128-row tiles.  129 rows: 238 us with 256-row tiles, 128 rows 159 us.
 int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= kPfRows ? kPfRows : 2 * kPfRows; }
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t rows = Hq / heads * Tq;
