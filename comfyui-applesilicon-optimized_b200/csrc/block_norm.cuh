@@ -14,8 +14,8 @@
 //   D var = sum_w [ M2_w + n_w (mean_w - mean)^2 ],
 // so one barrier per norm is enough.
 //
-// Bound: HBM.  Wan-shaped rows (65,520 x 5,120 bf16, 2.68 GB with h and out written)
-// run persistent CTAs: a CTA's rows share their modulation, which is folded once into
+// Bound: HBM.  Wan-shaped rows (65,520 x 5,120 bf16, 2.68 GB with h and out written: 460
+// us, 5.8 TB/s, 0.89 of the measured copy) run persistent CTAs: a CTA's rows share their modulation, which is folded once into
 // three fp32 vectors in shared memory (gate * post_w, w * (1 + scale), shift) instead
 // of being read again from L2 for every row, and the next row's loads are in flight
 // while one is reduced.
@@ -477,7 +477,9 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
 // The same for rows that 16-byte vectors do not fit (odd D, strides, views): VW = 2 values
 // per access when every row starts on a pair, else one.  Step s of thread i holds columns
 // (s * threads + i) * VW ..., so a warp's accesses are contiguous; persistent CTAs, the
-// folded vectors in shared memory, the next row's loads in flight, as above.
+// folded vectors in shared memory, the next row's loads in flight, as above.  Bound: the
+// instructions per value.  13824 x 1486 with fp32 modulation: 75 us, 0.34 of the copy rate
+// (190 us with one CTA per row); 6558 x 2020: 48 us (135); one of 159 rows of 783: 6 us (7).
 constexpr int kLooseValues = 16;  // per thread
 template <int DTYPE, int VW, bool QUANT, bool AFTER>
 __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a) {

@@ -21,8 +21,8 @@ HEADER = os.path.join(ROOT, "include", "b200q.h")
 UNITS = {
     "capi.cu": ["host.h", "gemm8.cuh", "prologue.cuh", "qkv_rope.cuh", "quant.cuh", "w8a16.cuh",
                 "w8a16_planes.cuh", "numerics.cuh", "ptx.cuh"],
-    "lowbit.cu": ["host.h", "digits.cuh", "w4a16.cuh", "w4_tile.cuh", "block_norm.cuh", "kv8.cuh", "kv8_prefill.cuh",
-                  "numerics.cuh", "ptx.cuh"],
+    "lowbit.cu": ["host.h", "digits.cuh", "w4a16.cuh", "w4_tile.cuh", "block_norm.cuh", "kv8.cuh",
+                  "kv8_prefill.cuh", "numerics.cuh", "ptx.cuh"],
 }
 SOURCES = sorted({f for unit, deps in UNITS.items() for f in (unit, *deps)})
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

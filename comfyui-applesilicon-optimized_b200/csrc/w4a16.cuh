@@ -1,4 +1,5 @@
-// 4-bit weight-only linear with group scales, few tokens:
+// 4-bit weight-only linear with group scales: up to 32 tokens, and the operands of the
+// decoded form for more than 256 (w4_tile.cuh has what lies between):
 //   out[m,n] = act( sum_k x[m,k] * s[n,k/G] * (c[n,k] - z[n,k/G]) + b[n] )
 // c: unsigned 4-bit codes, two per byte along K (even k in the low nibble);
 // s: one scale per row and group of G codes; z: one zero point (0..15) per row
@@ -121,6 +122,10 @@ __device__ __forceinline__ void w4_decode(uint32_t w, uint32_t z0, uint32_t z1, 
 // slice the fp32 sums go to the workspace, [slice][token][row], and w4_join_kernel
 // adds them in slice order.  Rings as in the integer kernel below: 128 bytes per row
 // and stage, scales travelling along.
+//
+// Bound: the instructions per weight word (unpacking, 2 MMAs per 8 tokens) and the ring's
+// latency.  16 tokens, K 13824, N 5120: 20.9 us, 1.7 TB/s of codes; 32 tokens, K 5120, N
+// 13824: 32.5 us.  TMA boxes instead of cp.async were slower (one issuer per CTA).
 constexpr int kWsWarps = 16;
 constexpr int kWsStages = 3;  // issue() relies on three
 
@@ -405,6 +410,10 @@ __global__ void __launch_bounds__(256)
 // (waiting for them at the start of each tile cost more than the tile).  A tile's sums
 // are double-buffered: one barrier per tile, and a different warp each time adds and
 // stores them while the others go on.
+//
+// Bound: x's digits and the first loads for small weights, issue for large ones.  1 token,
+// K = N = 5120, G 128: 6.3 us (2.1 TB/s of codes, 0.33 of the floor); K 5120, N 13824, G 64
+// with zero points and GELU: 13.8 us (2.6 TB/s, 0.43).  fp16 MMAs took 23 us for the latter.
 constexpr int kWdStages = 3;  // issue() relies on three
 // Most teams per CTA, by the digit columns' register need.
 constexpr int wd_teams(int nc) { return nc == 3 ? 2 : 3; }
@@ -705,7 +714,8 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 // x_pow[m] for the GEMM's row scale.  Exact down to 2^-17 of the row's maximum, within
 // 2^-25 of it below.
 //
-// Bound: memory (half a byte read and two written per weight).
+// Bound: memory (half a byte read and two written per weight): 46 us for 13824 x 5120 and
+// 2047 tokens, 4.4 TB/s; the product then takes 190 us, 0.93 of the measured GEMM rate.
 struct W4PrepareArgs {
   const uint8_t* w;
   int64_t ldw;

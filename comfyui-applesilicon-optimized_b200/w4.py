@@ -60,9 +60,10 @@ def w4_dequantize(w, scales, zeros=None):
 def w4a16_linear(x, w, scales, zeros=None, bias=None, act=None, out_dtype=None):
     """x [..., K] bf16/f16 -> act(x . W^T + bias) [..., N] in ``out_dtype`` (x's type).
 
-    act: None / "none", "gelu_tanh" or "gelu".  Up to 32 tokens run on a kernel
-    that reads the 4-bit weight as stored; more decode it once per call for the
-    16-bit tile GEMM."""
+    act: None / "none", "gelu_tanh" or "gelu".  Up to 256 tokens run on kernels that
+    read the 4-bit weight as stored (up to 32 with exact products, above that with each
+    weight rounded to fp16's 11 bits); more decode it once per call, rounded alike, for
+    the 16-bit tile GEMM."""
     f = _w4a16 or _load()
     return f(x, w, scales, zeros, bias, act, out_dtype)
 

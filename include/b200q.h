@@ -377,10 +377,10 @@ B200Q_API int b200q_fp8_decode(const uint8_t* src, int64_t n, int fp8_kind, void
  * [N, K/group] contiguous, scale_dtype a B200Q_BIAS_* code; zeros [N, K/group]
  * bytes 0..15 or NULL (8).  group 32, 64 or 128, K % group == 0.  X [M, K]
  * bf16/f16, bias bf16/f16/f32 or NULL, out bf16/f16/f32.  fp32 accumulation.
- * M <= 32 rounds once, at the output; larger M decodes W to fp16 in the
- * workspace (one rounding to 11 bits per weight) for the tile GEMM, and needs
- * b200q_w4a16_workspace_size bytes, 256-byte aligned (and, for f16 X, rows on
- * 16-byte boundaries). */
+ * M <= 32 rounds once, at the output; larger M rounds each weight once to fp16's
+ * 11 bits: up to 256 as it is multiplied, above that in a decoded copy in the
+ * workspace (f16 X then needs rows on 16-byte boundaries).  The workspace holds
+ * at least b200q_w4a16_workspace_size bytes (0: none needed), 256-byte aligned. */
 B200Q_API size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K);
 B200Q_API int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w,
                                  int64_t ldw, const void* scales, int scale_dtype,
