@@ -250,6 +250,7 @@ struct Kv8AttnArgs {
   float* part_ml; // [splits][B*Hq*Tq][2]: m (base 2), l
   const int32_t* lens;
   int B, Hq, G, Tq, causal, splits;
+  int longest_first;  // (row tiles) start CTAs in the order of their sequences' lengths
   float scale_log2;  // softmax scale * log2 e
 };
 

@@ -19,11 +19,11 @@
 //                         operand its rows are (no transpose)
 // S has two buffers: stage j + 1's scores are computed while stage j's softmax runs.
 // RT = 2 takes an SM's whole TMEM and double-buffers the fp16 tiles; RT = 1 puts two
-// CTAs on an SM.  Four chunks of 129 tokens (5 rows each) over 4001 to 12001: 201 us, 0.26
-// of the measured GEMM rate (one 128-row tile per CTA 253 us).  Bound: the chain scores ->
-// softmax -> P V of a stage, above all the scores, whose MMAs of 64 columns read q's tile
-// from shared memory for each stage: with an eighth of them 152 us; without conversion 188,
-// exponentials 195, rescaling 190.
+// CTAs on an SM.  Four chunks of 129 tokens (5 rows each) over 4001 to 12001: 185 us, 0.28
+// of the measured GEMM rate (one 128-row tile per CTA 253 us; sequences in any order 201).
+// Bound: the chain scores -> softmax -> P V of a stage, above all the scores, whose MMAs of
+// 64 columns read q's tile from shared memory for each stage: with an eighth of them 201
+// became 152 us; without conversion 188, exponentials 195, rescaling 190.
 #pragma once
 
 #include "kv8.cuh"
@@ -111,6 +111,20 @@ __device__ __forceinline__ void pf_convert(const uint8_t* src, uint8_t* dst, int
   }
 }
 
+// The sequence of this CTA.  CTAs start in grid order, and long ones that start last leave SMs
+// idle: longest first (the four chunks above: 201 -> 185 us).  Called by whole warps.
+__device__ __forceinline__ int attn_sequence(const Kv8AttnArgs& a) {
+  const int z = blockIdx.z, lane = threadIdx.x & 31;
+  if (!a.longest_first) return z;
+  const int len = lane < a.B ? a.lens[lane] : 0;
+  int rank = 0;
+  for (int i = 0; i < a.B; ++i) {
+    const int other = __shfl_sync(0xffffffffu, len, i);
+    rank += other > len || (other == len && i < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < a.B && rank == z)) - 1;
+}
+
 template <int D, int RT>
 __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
     kv8_prefill_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -148,7 +162,7 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
   griddep_launch_dependents();
 
   const Kv8Cache& c = a.c;
-  const int split = blockIdx.x, b = blockIdx.z, rows = a.G * a.Tq;
+  const int split = blockIdx.x, b = attn_sequence(a), rows = a.G * a.Tq;
   const int row_tiles = (rows + kPfRows * RT - 1) / (kPfRows * RT);
   const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * (kPfRows * RT);
   const int len = min(max(a.lens[b], 0), c.max_blocks << c.log_t);

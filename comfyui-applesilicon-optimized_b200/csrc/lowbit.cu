@@ -690,6 +690,8 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   a.B = static_cast<int>(B); a.Hq = static_cast<int>(Hq); a.G = static_cast<int>(Hq / heads);
   a.Tq = static_cast<int>(Tq); a.causal = causal != 0;
   a.splits = splits;
+  // ranked by one warp's lanes; where all CTAs start at once the order is nothing
+  a.longest_first = B > 1 && B <= 32 && B * heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq)) * splits > sms;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq))),
