@@ -475,11 +475,13 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
 
 // ---------------------------------------------------------------- other rows
 // The same for rows that 16-byte vectors do not fit (odd D, strides, views): VW = 2 values
-// per access when every row starts on a pair, else one.  Step s of thread i holds columns
-// (s * threads + i) * VW ..., so a warp's accesses are contiguous; persistent CTAs, the
-// folded vectors in shared memory, the next row's loads in flight, as above.  Bound: the
-// instructions per value.  13824 x 1486 with fp32 modulation: 75 us, 0.34 of the copy rate
-// (190 us with one CTA per row); 6558 x 2020: 48 us (135); one of 159 rows of 783: 6 us (7).
+// per access when every row starts on a pair, else one.  A warp has 512 columns, lane i those
+// at (32 s + i) * VW in step s: its accesses are contiguous and their offsets from the row's
+// pointers constants (with steps of the CTA's width the addresses were half of the
+// instructions: 75 us for the first size below).  Persistent CTAs, the folded vectors in shared
+// memory and the next row's loads in flight, as above.  Bound: the instructions per value.
+// 13824 x 1486 with fp32 modulation: 52 us, 0.48 of the copy rate (190 us with one CTA per
+// row); 6558 x 2020: 38 us (135); 159 rows of 783: 6 us (7).
 constexpr int kLooseValues = 16;  // per thread
 template <int DTYPE, int VW, bool QUANT, bool AFTER>
 __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a) {
@@ -492,28 +494,26 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const float inv_d = 1.0f / static_cast<float>(a.D);
+  const int c0 = warp * (32 * kLooseValues) + lane * VW;  // the thread's first column
+  constexpr int kStep = 32 * VW;
   bool on[S];
-  int nw = 0, nl = 0;
 #pragma unroll
-  for (int s = 0; s < S; ++s) {
-    on[s] = static_cast<int>(s * blockDim.x + threadIdx.x) * VW < a.D;
-    nw += min(max(a.D - static_cast<int>(s * blockDim.x + warp * 32) * VW, 0), 32 * VW);
-    nl += min(max(a.D - static_cast<int>(s * blockDim.x + lane * 32) * VW, 0), 32 * VW);
-  }
-  auto col = [&](int s) { return static_cast<int>(s * blockDim.x + threadIdx.x) * VW; };
+  for (int s = 0; s < S; ++s) on[s] = c0 + s * kStep < a.D;
+  const int nw = min(max(a.D - warp * (32 * kLooseValues), 0), 32 * kLooseValues);
+  const int nl = min(max(a.D - lane * (32 * kLooseValues), 0), 32 * kLooseValues);
   const float n_l = static_cast<float>(max(nl, 1)), inv_n_l = 1.0f / n_l, inv_n_w = 1.0f / static_cast<float>(max(nw, 1));
   const int64_t r0 = static_cast<int64_t>(a.rows) * blockIdx.x / gridDim.x;
   const int64_t r1 = static_cast<int64_t>(a.rows) * (blockIdx.x + 1) / gridDim.x;
   Raw xn[S], yn[S];  // the row after this one
-  const uint16_t* xp = static_cast<const uint16_t*>(a.x) + r0 * a.ldx;
-  const uint16_t* yp = static_cast<const uint16_t*>(a.y) + r0 * a.ldy;
+  const uint16_t* xp = static_cast<const uint16_t*>(a.x) + r0 * a.ldx + c0;
+  const uint16_t* yp = static_cast<const uint16_t*>(a.y) + r0 * a.ldy + c0;
   auto fetch = [&]() {
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       xn[s] = yn[s] = 0;
       if (on[s]) {
-        xn[s] = __ldg(reinterpret_cast<const Raw*>(xp + col(s)));
-        if (AFTER) yn[s] = __ldg(reinterpret_cast<const Raw*>(yp + col(s)));
+        xn[s] = __ldg(reinterpret_cast<const Raw*>(xp + s * kStep));
+        if (AFTER) yn[s] = __ldg(reinterpret_cast<const Raw*>(yp + s * kStep));
       }
     }
     xp += a.ldx;
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
 #pragma unroll
           for (int j = 0; j < VW; ++j) {
             float one[1] = {none};
-            if (p && on[s]) load_vals<1>(p, dtype, at + col(s) + j, one);
+            if (p && on[s]) load_vals<1>(p, dtype, at + c0 + s * kStep + j, one);
             to[s][j] = one[0];
           }
       };
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
         for (int s = 0; s < S; ++s)
 #pragma unroll
           for (int j = 0; j < VW; ++j)
-            if (on[s]) fold[which * a.D + col(s) + j] = u[s][j];
+            if (on[s]) fold[which * a.D + c0 + s * kStep + j] = u[s][j];
       };
       auto times = [&](float plus) {
 #pragma unroll
@@ -582,20 +582,30 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
         keep(2);
       }
     }
+    auto folded_at = [&](int which, int s, float (&to)[VW]) {
+      const float* f = fold + which * a.D + c0 + s * kStep;
+      if constexpr (VW == 2) {
+        const float2 e = *reinterpret_cast<const float2*>(f);
+        to[0] = e.x;
+        to[1] = e.y;
+      } else {
+        to[0] = *f;
+      }
+    };
     float v[S][VW];
     if (AFTER) {
 #pragma unroll
       for (int s = 0; s < S; ++s) unpack(y0[s], v[s]);
       row_norm<S, false, VW>(v, a.post_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][0]);
-      uint16_t* hp = static_cast<uint16_t*>(a.h) + row * a.ldh;
+      uint16_t* hp = static_cast<uint16_t*>(a.h) + row * a.ldh + c0;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
-        float u[VW];
+        float u[VW], g[VW];
         unpack(x0[s], u);
+        if (on[s]) folded_at(2, s, g);
 #pragma unroll
-        for (int j = 0; j < VW; ++j)
-          v[s][j] = on[s] ? fmaf(a.res_scale, u[j], v[s][j] * fold[2 * a.D + col(s) + j]) : 0.0f;
-        if (a.h && on[s]) store(hp + col(s), v[s]);
+        for (int j = 0; j < VW; ++j) v[s][j] = on[s] ? fmaf(a.res_scale, u[j], v[s][j] * g[j]) : 0.0f;
+        if (a.h && on[s]) store(hp + s * kStep, v[s]);
       }
     } else {
 #pragma unroll
@@ -603,17 +613,20 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
     }
     if (!QUANT && !a.out) continue;
     row_norm<S, false, VW>(v, a.pre_kind, on, inv_n_w, n_l, inv_n_l, inv_d, a.eps, bufs[row & 1][1]);
-    uint16_t* op = static_cast<uint16_t*>(a.out) + row * a.ldo;
+    uint16_t* op = static_cast<uint16_t*>(a.out) + row * a.ldo + c0;
     uint32_t top = 0;
 #pragma unroll
     for (int s = 0; s < S; ++s)
       if (on[s]) {
+        float w[VW], b[VW];
+        folded_at(0, s, w);
+        folded_at(1, s, b);
 #pragma unroll
         for (int j = 0; j < VW; ++j) {
-          v[s][j] = fmaf(v[s][j], fold[col(s) + j], fold[a.D + col(s) + j]);
+          v[s][j] = fmaf(v[s][j], w[j], b[j]);
           if (QUANT) top = max(top, __float_as_uint(v[s][j]) & 0x7FFFFFFFu);  // as bits: NaN sorts above
         }
-        if (!QUANT) store(op + col(s), v[s]);
+        if (!QUANT) store(op + s * kStep, v[s]);
       }
     if (!QUANT) continue;
     top = __reduce_max_sync(0xffffffffu, top);
@@ -624,7 +637,7 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
     const float sc = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);
     if (threadIdx.x == 0) a.q_scale[row] = sc;
     const float inv = sc > 0.0f ? fminf(__fdiv_rn(1.0f, sc), 3.402823466e38f) : 0.0f;  // as above
-    int8_t* qp = a.q + row * a.ldq;
+    int8_t* qp = a.q + row * a.ldq + c0;
 #pragma unroll
     for (int s = 0; s < S; ++s)
       if (on[s]) {
@@ -632,9 +645,9 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
 #pragma unroll
         for (int j = 0; j < VW; ++j) o[j] = __float_as_uint(fmaf(v[s][j], inv, 12582912.0f));
         if constexpr (VW == 2)
-          *reinterpret_cast<uint16_t*>(qp + col(s)) = static_cast<uint16_t>(__byte_perm(o[0], o[1], 0x0040));
+          *reinterpret_cast<uint16_t*>(qp + s * kStep) = static_cast<uint16_t>(__byte_perm(o[0], o[1], 0x0040));
         else
-          qp[col(s)] = static_cast<int8_t>(o[0]);
+          qp[s * kStep] = static_cast<int8_t>(o[0]);
       }
   }
 }
