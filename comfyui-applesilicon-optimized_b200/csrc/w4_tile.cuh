@@ -344,15 +344,17 @@ __global__ void __launch_bounds__(kW4TileThreads)
         const float xp = __ldg(a.x_pow + min(c + (lane & 15), a.M - 1));
 #pragma unroll
         for (int i = 0; i < 16; ++i) buf[i * 32] = __uint_as_float(r[i]) * __shfl_sync(0xffffffffu, xp, i) * wp;
-        if (n >= a.N) continue;
-        if (a.part) {
-          float* to = a.part + (static_cast<int64_t>(slice) * a.M + c) * a.N + n;
+        if (n < a.N) {
+          if (a.part) {
+            float* to = a.part + (static_cast<int64_t>(slice) * a.M + c) * a.N + n;
 #pragma unroll 8
-          for (int i = 0; i < many; ++i) to[static_cast<int64_t>(i) * a.N] = buf[i * 32];
-        } else {
+            for (int i = 0; i < many; ++i) to[static_cast<int64_t>(i) * a.N] = buf[i * 32];
+          } else {
 #pragma unroll 4
-          for (int i = 0; i < many; ++i) store_out(ep, c + i, n, epi_scaled(buf[i * 32], 1.0f, 1.0f, 1.0f, ep, n));
+            for (int i = 0; i < many; ++i) store_out(ep, c + i, n, epi_scaled(buf[i * 32], 1.0f, 1.0f, 1.0f, ep, n));
+          }
         }
+        __syncwarp();  // the next load wants the whole warp
       }
     }
   }
