@@ -667,12 +667,14 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
           const float4 tb = table[(g0 + gl) * 4 * NC + 4 * j + t];  // columns 2t, 2t + 1
           const int za = __float_as_int(sa.y), zb = __float_as_int(sb.y);
           const int s0 = __float_as_int(tb.y), s1 = __float_as_int(tb.w);
-          // (i + 1.5 * 2^23) f - 1.5 * 2^23 f: both products are exact, f a power of two
-          const float m0 = -12582912.0f * tb.x, m1 = -12582912.0f * tb.z;
-          acc[j][0] = fmaf(fmaf(__int_as_float(d[j][0] + za * s0), tb.x, m0), sa.x, acc[j][0]);
-          acc[j][1] = fmaf(fmaf(__int_as_float(d[j][1] + za * s1), tb.z, m1), sa.x, acc[j][1]);
-          acc[j][2] = fmaf(fmaf(__int_as_float(d[j][2] + zb * s0), tb.x, m0), sb.x, acc[j][2]);
-          acc[j][3] = fmaf(fmaf(__int_as_float(d[j][3] + zb * s1), tb.z, m1), sb.x, acc[j][3]);
+          // f, a power of two, meets the scale first: f times the sum leaves fp32's range for
+          // |x| from 2^110 on, f s only where the output does.  Sum and f s are exact
+          const float i0 = __int_as_float(d[j][0] + za * s0) - 12582912.0f, i1 = __int_as_float(d[j][1] + za * s1) - 12582912.0f;
+          const float i2 = __int_as_float(d[j][2] + zb * s0) - 12582912.0f, i3 = __int_as_float(d[j][3] + zb * s1) - 12582912.0f;
+          acc[j][0] = fmaf(i0, tb.x * sa.x, acc[j][0]);
+          acc[j][1] = fmaf(i1, tb.z * sa.x, acc[j][1]);
+          acc[j][2] = fmaf(i2, tb.x * sb.x, acc[j][2]);
+          acc[j][3] = fmaf(i3, tb.z * sb.x, acc[j][3]);
         }
       }
     }

@@ -21,3 +21,26 @@ def test_last_rows_of_a_tile_over_several_columns(native, M, N):
         out = w4.w4a16_linear(*dev(x, w, s, z, b), "gelu_tanh")
         check(out, x, w, s, z, b, "gelu_tanh")
         assert native.device_status() == 0
+
+
+def bound(out, ref, size, exact):
+    u = ref64.UNIT[out.dtype]
+    return u * ref.abs() + size * (2.0 ** -17 + (0 if exact else 2.0 ** -11))
+
+
+def large(M, power):
+    """bf16 values up to 2^power and some with weights that keep the output in range, exactly
+    representable ones (whose lower digits are zero) and others."""
+    x, w, s, z, b = make(M, 48, 256, 64, torch.bfloat16, True)
+    s = (s.float() * 2.0 ** -20).to(torch.bfloat16)
+    x[0] = torch.sign(x[0].float()).to(torch.bfloat16)
+    return (x.float() * 2.0 ** power).to(torch.bfloat16), w, s, z
+
+
+@pytest.mark.parametrize("M", [1, 2, 3, 8, 9])
+@pytest.mark.parametrize("power", [100, 110, 117, 124])
+def test_large_activations_of_few_tokens(native, M, power):
+    x, w, s, z = large(M, power)
+    out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
+    ref, size = ref64.w4_linear(x, w, s, z)
+    assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, True)).all())
