@@ -166,14 +166,15 @@ int launch_digits(const W4DigitArgs& a, int G, const EpiArgs& ep, const WdPlan& 
 bool w4_joins(int64_t N) { return N % 8 != 0; }
 int64_t w4_join_ld(int64_t N) { return cdiv(N, 32) * 32; }
 struct W4Work {
-  size_t w, x, row, col, out, total;  // byte offsets
+  size_t w, x, row, last, col, out, total;  // byte offsets
 };
 W4Work w4_work(int64_t M, int64_t N, int64_t K) {
   auto up = [](size_t b) { return (b + 255) & ~size_t(255); };
   W4Work o{};
   o.x = up(size_t(N) * K * 2);
   o.row = o.x + up(size_t(M) * K * 2);
-  o.col = o.row + up(size_t(M) * 4);
+  o.last = o.row + up(size_t(M) * 4);
+  o.col = o.last + up(4);
   o.out = o.col + up(size_t(N) * 4);
   o.total = o.out + (w4_joins(N) ? up(size_t(M) * w4_join_ld(N) * 4) : 0);
   return o;
@@ -533,6 +534,8 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     a.x_pow = reinterpret_cast<float*>(base + o.row);
     ep.row_scale = a.x_pow;
     ep.row_scale_vec = 1;
+    a.last = reinterpret_cast<float*>(base + o.last);
+    ep.extra_scale = a.last;
     blocks += cdiv(M, 8);
     x = a.x16;
     ldx = K;
@@ -549,7 +552,7 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   sums.act = kActNone;
   s = host::gemm_f16_scaled(x, ldx, a.w16, K, M, N, K, sums, st);
   if (s != B200Q_OK) return s;
-  ep.col_scale = ep.row_scale = nullptr;
+  ep.col_scale = ep.row_scale = ep.extra_scale = nullptr;
   return launch_join(static_cast<const float*>(sums.out), 1, sums.ldo, ep, st);
 }
 

@@ -147,6 +147,11 @@ __global__ void __launch_bounds__(256) w4_tile_prepare_kernel(const W4TilePrepar
   }
 }
 
+// v * a * b for powers of two a and b, the smaller first: x's row at 2^110 and then a scale of
+// 2^-10 would leave fp32's range on the way to a value inside it.  (What the smaller one, at
+// least 2^-126, takes off a subnormal product is below 2^-24 of the row's terms.)
+__device__ __forceinline__ float times_powers(float v, float a, float b) { return v * fminf(a, b) * fmaxf(a, b); }
+
 // ---------------------------------------------------------------- the product
 struct W4TileArgs {
   const uint2* sz;
@@ -331,7 +336,7 @@ __global__ void __launch_bounds__(kW4TileThreads)
     tc_fence_after();
     if (live) {
       const int n = n0 + row;
-      const float wp = n < a.N ? __ldg(a.w_pow + n) : 0.0f;
+      const float wp = n < a.N ? __ldg(a.w_pow + n) : 1.0f;
       // through shared memory (the ring is free), so that the epilogue's code is there once
       float* buf = reinterpret_cast<float*>(sm.x) + warp * (16 * 32) + lane;
 #pragma unroll 1
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kW4TileThreads)
         tmem_ld_wait();
         const float xp = __ldg(a.x_pow + min(c + (lane & 15), a.M - 1));
 #pragma unroll
-        for (int i = 0; i < 16; ++i) buf[i * 32] = __uint_as_float(r[i]) * __shfl_sync(0xffffffffu, xp, i) * wp;
+        for (int i = 0; i < 16; ++i) buf[i * 32] = times_powers(__uint_as_float(r[i]), __shfl_sync(0xffffffffu, xp, i), wp);
         if (n < a.N) {
           if (a.part) {
             float* to = a.part + (static_cast<int64_t>(slice) * a.M + c) * a.N + n;

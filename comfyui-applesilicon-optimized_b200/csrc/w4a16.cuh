@@ -714,7 +714,9 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 //
 // bf16 token rows: x * 2^-e, 2^e the power of two of the row's largest |x|, to
 // x_pow[m] for the GEMM's row scale.  Exact down to 2^-17 of the row's maximum, within
-// 2^-25 of it below.
+// 2^-25 of it below.  The GEMM multiplies by the row's power before the column's: 2^-22 of
+// the former is kept for the scalar that comes last, so that sums of up to 2^17 times rows
+// near fp32's largest value pass through finite numbers.
 //
 // Bound: memory (half a byte read and two written per weight): 46 us for 13824 x 5120 and
 // 2047 tokens, 4.4 TB/s; the product then takes 190 us, 0.93 of the measured GEMM rate.
@@ -732,6 +734,7 @@ struct W4PrepareArgs {
   int M, x_vec;
   __half* x16;
   float* x_pow;
+  float* last;  // 2^22
 };
 
 __global__ void __launch_bounds__(256) w4_prepare_kernel(const W4PrepareArgs a) {
@@ -813,7 +816,8 @@ __global__ void __launch_bounds__(256) w4_prepare_kernel(const W4PrepareArgs a) 
   int ex = static_cast<int>(top >> 7);
   ex = ex == 255 ? 127 : min(max(ex, 1), 253);
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-  if (lane == 0) a.x_pow[m] = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+  if (lane == 0) a.x_pow[m] = __uint_as_float(static_cast<uint32_t>(ex) << 23) * 0x1p-22f;  // 2^-148 and up
+  if (lane == 0 && m == 0) *a.last = 0x1p22f;
   uint4* dst = reinterpret_cast<uint4*>(a.x16 + m * a.K);
 #pragma unroll 4
   for (int p = lane; p < pieces; p += 32) {

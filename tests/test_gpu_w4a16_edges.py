@@ -44,3 +44,23 @@ def test_large_activations_of_few_tokens(native, M, power):
     out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
     ref, size = ref64.w4_linear(x, w, s, z)
     assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, True)).all())
+
+
+@pytest.mark.parametrize("M,N", [(40, 48), (130, 48), (300, 48), (300, 45)])
+@pytest.mark.parametrize("power", [100, 110, 117, 124])
+def test_large_activations_of_many_tokens(native, M, N, power):
+    x, w, s, z = large(M, power)
+    w, s, z = w[:N].contiguous(), s[:N].contiguous(), z[:N].contiguous()
+    out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
+    ref, size = ref64.w4_linear(x, w, s, z)
+    assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, False)).all())
+
+
+@pytest.mark.parametrize("M", [40, 300])
+def test_small_activations_and_large_scales(native, M):
+    """The other way round: rows near the smallest normal number, scales far above 1."""
+    x, w, s, z = large(M, -110)
+    s = (s.float() * 2.0 ** 60).to(torch.bfloat16)
+    out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
+    ref, size = ref64.w4_linear(x, w, s, z)
+    assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, False)).all())
