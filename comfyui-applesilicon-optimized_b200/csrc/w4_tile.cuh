@@ -126,8 +126,7 @@ __global__ void __launch_bounds__(256) w4_tile_prepare_kernel(const W4TilePrepar
     if (lane == 0) tops[warp] = top;
     __syncthreads();
     top = __reduce_max_sync(0xffffffffu, tops[lane & 7]);
-    int ex = static_cast<int>(top >> 7);
-    ex = ex == 255 ? 127 : min(max(ex, 1), 253);
+    const int ex = min(max(static_cast<int>(top >> 7), 1), 253);
     inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
     pow = __uint_as_float(static_cast<uint32_t>(ex) << 23);
   }

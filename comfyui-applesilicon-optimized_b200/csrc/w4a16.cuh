@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(kWsWarps * 32) w4_slice_kernel(const W4SliceAr
         if (pieces > 256) load(0);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        int ex = static_cast<int>(top >> 7);
-        ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+        // (an infinity or NaN stays one at any power: its row takes the largest, at which
+        // the finite values beside it stay finite)
+        const int ex = min(max(static_cast<int>(top >> 7), 1), 253);
         inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
         pow = __uint_as_float(static_cast<uint32_t>(ex) << 23);
       }
@@ -812,9 +813,8 @@ __global__ void __launch_bounds__(256) w4_prepare_kernel(const W4PrepareArgs a) 
     for (int j = 0; j < 4; ++j) top = max(top, max(e[j] & 0x7FFFu, (e[j] >> 16) & 0x7FFFu));
   }
   top = __reduce_max_sync(0xffffffffu, top);
-  // a row holding inf or NaN keeps its values: they carry through the product
-  int ex = static_cast<int>(top >> 7);
-  ex = ex == 255 ? 127 : min(max(ex, 1), 253);
+  // infinities and NaN carry through the product; finite values beside them stay finite
+  const int ex = min(max(static_cast<int>(top >> 7), 1), 253);
   const float inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
   if (lane == 0) a.x_pow[m] = __uint_as_float(static_cast<uint32_t>(ex) << 23) * 0x1p-22f;  // 2^-148 and up
   if (lane == 0 && m == 0) *a.last = 0x1p22f;

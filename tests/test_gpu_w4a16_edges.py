@@ -64,3 +64,18 @@ def test_small_activations_and_large_scales(native, M):
     out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
     ref, size = ref64.w4_linear(x, w, s, z)
     assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, False)).all())
+
+
+@pytest.mark.parametrize("M", [12, 100, 300])
+def test_infinity_beside_large_values(native, M):
+    """A row's infinity decides its outputs' sign; finite values of any size beside it do
+    not make infinities of their own."""
+    x, w, s, z, b = make(M, 64, 256, 64, torch.bfloat16, False)
+    x[3] = x[3].float().mul(1e30).to(torch.bfloat16)
+    x[3, 9] = float("inf")
+    out = w4.w4a16_linear(*dev(x, w, s))
+    W = ref64.w4_weight(w, s)[:, 9]
+    want = torch.where(W == 0, torch.nan, torch.sign(W) * torch.inf)
+    got = out[3].double().cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[~want.isnan()], want[~want.isnan()])
