@@ -111,6 +111,7 @@ _SIGNATURES = {
     "b200q_i8_mlp_bridge_prequant": ([_vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i64, _i64, _i64,
                                       _int, _i64, _vp, _vp, _i64, _vp, _vp], _int),
     "b200q_w4a16_workspace_size": ([_i64, _i64, _i64], _sz),
+    "b200q_w4a16_workspace_bytes": ([_i64, _i64, _i64, _i64, _int, _int], _sz),
     "b200q_w4a16_linear": ([_vp, _int, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp, _int, _int, _vp,
                             _int, _i64, _i64, _i64, _i64, _vp, _sz, _vp], _int),
 }

@@ -160,7 +160,7 @@ Tensor w4a16(const Tensor& x, const Tensor& w, const Tensor& scales, const Tenso
   int64_t ldx;
   Tensor x2 = as_rows(x, K, &ldx);
   const int64_t M = x.numel() / K;
-  const size_t bytes = b200q_w4a16_workspace_size(M, N, K);
+  const size_t bytes = b200q_w4a16_workspace_bytes(M, N, K, G, xdt, sdt);
   if (bytes && xdt == B200Q_F16 && (!aligned(x2.data_ptr(), 16) || ldx % 8)) {
     x2 = x2.clone(at::MemoryFormat::Contiguous);
     ldx = K;

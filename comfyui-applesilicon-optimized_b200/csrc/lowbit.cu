@@ -78,10 +78,10 @@ constexpr int kWsMaxSlices = 32;
 struct WsPlan {
   int slices, parts, smem;
 };
-bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, int max_slices, WsPlan* p) {
+bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
   const int64_t KG = K / G, tiles = cdiv(N, 16);
   int64_t best = -1;
-  for (int s = 1; s <= max_slices && s <= KG && s <= sms; ++s) {
+  for (int s = 1; s <= kWsMaxSlices && s <= KG && s <= sms; ++s) {
     const int64_t gs = cdiv(KG, s);
     const int smem = ws_smem_bytes(int(M), int(gs) * G, G);
     if (smem > 227 * 1024) continue;
@@ -97,8 +97,6 @@ bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, int max_slices, Ws
   }
   return best >= 0;
 }
-size_t ws_work_bytes(int64_t M, int64_t N) { return size_t(kWsMaxSlices) * M * N * 4; }
-
 int launch_join(const float* part, int slices, int64_t ld, const EpiArgs& ep, cudaStream_t st) {
   const int64_t chunks = cdiv(ep.N, 256);
   if (ep.M * chunks > kIntMax) return B200Q_ERR_UNSUPPORTED;
@@ -281,6 +279,35 @@ int launch_w4_tile(const W4TilePlan& p, const void* x, int x_dtype, int64_t ldx,
   return launch_join(a.part, p.slices, N, ep, st);
 }
 
+// The kernels of a call and the workspace they take.  The integer kernel for few tokens wants
+// scales of x's type and indexes them with 31 bits, as the slice kernel does.
+enum W4Kind { kW4None, kW4Digits, kW4Slices, kW4Tiles, kW4Decoded };
+struct W4Route {
+  W4Kind kind;
+  WdPlan wd;
+  WsPlan ws;
+  W4TilePlan tile;
+  size_t need;
+};
+W4Route w4_route(int sms, int64_t M, int64_t N, int64_t K, int64_t G, bool same_type) {
+  W4Route r{};
+  const bool small = N * (K / G) <= kIntMax;
+  if (same_type && small && wd_plan(sms, M, N, K, int(G), &r.wd)) {
+    r.kind = kW4Digits;
+  } else if (w4_tiles(M, N, K)) {
+    r.kind = kW4Tiles;
+    r.tile = w4_tile_plan(sms, M, N, K);
+    r.need = w4_tile_work(r.tile, M, N, K, G).total;
+  } else if (M > kW4MaxSmallM) {
+    r.kind = kW4Decoded;
+    r.need = w4_work(M, N, K).total;
+  } else if (small && ws_plan(sms, M, N, K, int(G), &r.ws)) {
+    r.kind = kW4Slices;
+    r.need = r.ws.slices > 1 ? size_t(r.ws.slices) * M * N * 4 : 0;
+  }
+  return r;
+}
+
 // PERSIST: as many CTAs as are resident at once (at most one per row).
 template <typename K>
 int launch_persistent(K kern, const NormArgs& a, int threads, int smem, int sms, cudaStream_t st) {
@@ -424,16 +451,17 @@ bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
 
 extern "C" {
 
-size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (w4_tiles(M, N, K)) return w4_tile_work(w4_tile_plan(host::device_sms(), M, N, K), M, N, K, 32).total;
-  if (M > kW4MaxSmallM) return w4_work(M, N, K).total;
-  // the integer kernel for few tokens needs none
+size_t b200q_w4a16_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group, int x_dtype, int scale_dtype) {
+  if (M <= 0 || N <= 0 || K <= 0 || (group != 32 && group != 64 && group != 128) || K % group != 0) return 0;
   const int sms = host::device_sms();
-  WdPlan wd;
-  if (sms && wd_plan(sms, M, N, K, 32, &wd) && wd_plan(sms, M, N, K, 64, &wd) && wd_plan(sms, M, N, K, 128, &wd))
-    return 0;
-  return ws_work_bytes(M, N);
+  return w4_route(sms ? sms : 148, M, N, K, group, scale_dtype == x_dtype + 1).need;
+}
+size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K) {
+  size_t most = 0;
+  for (int64_t group : {32, 64, 128})
+    for (int scale_dtype : {B200Q_BIAS_BF16, B200Q_BIAS_F32})
+      most = std::max(most, b200q_w4a16_workspace_bytes(M, N, K, group, B200Q_BF16, scale_dtype));
+  return most;
 }
 
 int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w, int64_t ldw,
@@ -463,12 +491,12 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   ep.act = act;
   ep.M = static_cast<int>(M);
   ep.N = static_cast<int>(N);
-  const size_t need = b200q_w4a16_workspace_size(M, N, K);
+  const W4Route route = w4_route(sms, M, N, K, group, scale_dtype == x_dtype + 1);
+  if (route.kind == kW4None) return B200Q_ERR_UNSUPPORTED;
+  const size_t need = route.need;
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return B200Q_ERR_WORKSPACE;
   const bool x_vec = aligned(x, 16) && ldx % 8 == 0;
-  WdPlan wd;
-  // (scales of x's type; N * K / G below 2^31)
-  if (scale_dtype == x_dtype + 1 && N * (K / group) <= kIntMax && wd_plan(sms, M, N, K, int(group), &wd)) {
+  if (route.kind == kW4Digits) {
     W4DigitArgs a{};
     a.x = x;
     a.ldx = ldx;
@@ -481,14 +509,13 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     a.K = static_cast<int>(K);
     a.x_vec = x_vec;
     a.tiles = static_cast<int>(cdiv(N, 16));
-    return x_dtype == B200Q_F16 ? launch_digits<__half>(a, int(group), ep, wd, st)
-                                : launch_digits<__nv_bfloat16>(a, int(group), ep, wd, st);
+    return x_dtype == B200Q_F16 ? launch_digits<__half>(a, int(group), ep, route.wd, st)
+                                : launch_digits<__nv_bfloat16>(a, int(group), ep, route.wd, st);
   }
-  if (w4_tiles(M, N, K))
-    return launch_w4_tile(w4_tile_plan(sms, M, N, K), x, x_dtype, ldx, x_vec, w, ldw, scales, scale_dtype, zeros, group,
-                          M, N, K, ep, static_cast<uint8_t*>(workspace), st);
-  WsPlan ws;
-  if (M <= kW4MaxSmallM && N * (K / group) <= kIntMax && ws_plan(sms, M, N, K, int(group), need ? kWsMaxSlices : 1, &ws)) {
+  if (route.kind == kW4Tiles)
+    return launch_w4_tile(route.tile, x, x_dtype, ldx, x_vec, w, ldw, scales, scale_dtype, zeros, group, M, N, K, ep,
+                          static_cast<uint8_t*>(workspace), st);
+  if (route.kind == kW4Slices) {
     W4SliceArgs a{};
     a.x = x;
     a.x_f16 = x_dtype == B200Q_F16;
@@ -498,16 +525,15 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     a.scales = scales;
     a.scale_dtype = scale_dtype;
     a.zeros = zeros;
-    a.part = ws.slices > 1 ? static_cast<float*>(workspace) : nullptr;
+    a.part = need ? static_cast<float*>(workspace) : nullptr;
     a.M = static_cast<int>(M);
     a.N = static_cast<int>(N);
     a.K = static_cast<int>(K);
     a.x_vec = x_vec;
-    a.slices = ws.slices;
-    a.parts = ws.parts;
-    return launch_slice(a, int(group), ep, ws, st);
+    a.slices = route.ws.slices;
+    a.parts = route.ws.parts;
+    return launch_slice(a, int(group), ep, route.ws, st);
   }
-  if (M <= kW4MaxSmallM) return B200Q_ERR_UNSUPPORTED;  // N * K / group above 2^31
   const W4Work o = w4_work(M, N, K);
   if (x_dtype == B200Q_F16 && !x_vec) return B200Q_ERR_INVALID;  // fp16 rows must be 16-byte aligned here
   uint8_t* base = static_cast<uint8_t*>(workspace);

@@ -380,7 +380,11 @@ B200Q_API int b200q_fp8_decode(const uint8_t* src, int64_t n, int fp8_kind, void
  * M <= 32 rounds once, at the output; larger M rounds each weight once to fp16's
  * 11 bits: up to 256 as it is multiplied, above that in a decoded copy in the
  * workspace (f16 X then needs rows on 16-byte boundaries).  The workspace holds
- * at least b200q_w4a16_workspace_size bytes (0: none needed), 256-byte aligned. */
+ * at least b200q_w4a16_workspace_bytes of the call (0: none needed), 256-byte
+ * aligned; b200q_w4a16_workspace_size is the largest of these over group sizes
+ * and types. */
+B200Q_API size_t b200q_w4a16_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t group,
+                                             int x_dtype, int scale_dtype);
 B200Q_API size_t b200q_w4a16_workspace_size(int64_t M, int64_t N, int64_t K);
 B200Q_API int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w,
                                  int64_t ldw, const void* scales, int scale_dtype,

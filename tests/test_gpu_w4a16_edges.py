@@ -66,6 +66,20 @@ def test_small_activations_and_large_scales(native, M):
     assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, False)).all())
 
 
+@pytest.mark.parametrize("dtype,scale_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16),
+                                               (torch.bfloat16, torch.float16), (torch.float16, torch.float32)])
+@pytest.mark.parametrize("M", [1, 2, 3])
+def test_scales_of_another_type_split_k_too(native, dtype, scale_dtype, M):
+    """Scales that are not of x's type take the slice kernel, whose few tiles at one token
+    need K split over CTAs to fill the GPU: the product and the join are two launches."""
+    x, w, s, z, b = make(M, 1024, 2048, 64, dtype, True, scale_dtype=scale_dtype)
+    d = dev(x, w, s, z)
+    before = native.launch_count()
+    out = w4.w4a16_linear(*d)
+    assert native.launch_count() - before == 2
+    check(out, x, w, s, z, b)
+
+
 @pytest.mark.parametrize("M", [12, 100, 300])
 def test_infinity_beside_large_values(native, M):
     """A row's infinity decides its outputs' sign; finite values of any size beside it do

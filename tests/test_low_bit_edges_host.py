@@ -1,0 +1,20 @@
+"""CPU tests of what the low-bit operators tell a tracer and a caller."""
+import pytest
+import torch
+
+import b200q  # noqa: F401  (registers the operators)
+
+
+def test_w4a16_workspaces():
+    """The workspace of a call without shape-only guesses: the size function covers every group
+    size and type, and calls whose scales are not of x's type get one for their K slices."""
+    from b200q._patches import _native
+    L = _native.lib()
+    for M, N, K in ((1, 5120, 5120), (2, 1024, 2048), (16, 5120, 13824), (40, 515, 1024), (300, 129, 256)):
+        every = [L.b200q_w4a16_workspace_bytes(M, N, K, g, x, s)
+                 for g in (32, 64, 128) for x in (0, 1) for s in (1, 2, 3)]
+        assert max(every) == L.b200q_w4a16_workspace_size(M, N, K)
+    assert L.b200q_w4a16_workspace_bytes(1, 5120, 5120, 128, 0, 1) == 0  # the integer kernel
+    assert L.b200q_w4a16_workspace_bytes(1, 5120, 5120, 128, 0, 3) > 0
+    for bad in ((0, 8, 64, 64), (2, 8, 64, 48), (2, 8, 96, 64)):
+        assert L.b200q_w4a16_workspace_bytes(*bad, 0, 1) == 0
