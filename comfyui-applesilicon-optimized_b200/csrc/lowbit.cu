@@ -73,7 +73,8 @@ int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, 
 constexpr int64_t kW4MaxSmallM = 32;
 
 // K slices and row parts of the slice kernel: the split whose busiest warp has the
-// fewest groups to go through, x's slice beside the rings.
+// fewest groups to go through, x's slice beside the rings.  More than kWsMaxSlices only where
+// x's slice fits no otherwise (32 tokens: K above 42,000 to 57,000 by the group size).
 constexpr int kWsMaxSlices = 32;
 struct WsPlan {
   int slices, parts, smem;
@@ -81,10 +82,10 @@ struct WsPlan {
 bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
   const int64_t KG = K / G, tiles = cdiv(N, 16);
   int64_t best = -1;
-  for (int s = 1; s <= kWsMaxSlices && s <= KG && s <= sms; ++s) {
+  for (int s = 1; s <= KG && s <= sms && (s <= kWsMaxSlices || best < 0); ++s) {
     const int64_t gs = cdiv(KG, s);
-    const int smem = ws_smem_bytes(int(M), int(gs) * G, G);
-    if (smem > 227 * 1024) continue;
+    const int64_t smem = kWsWarps * kWsStages * 2048 + M * 2 * gs * G;  // (without the pitch's padding: 64 bits)
+    if (smem > 227 * 1024 || ws_smem_bytes(int(M), int(gs) * G, G) > 227 * 1024) continue;
     const int64_t parts = sms / s;
     // a slice more costs its partial sums' round trip, about 2 groups of a warp
     const int64_t cost = cdiv(tiles, parts * kWsWarps) * gs * G / 32 + (s > 1 ? 8 + s / 4 : 0);
@@ -92,11 +93,12 @@ bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
       best = cost;
       p->slices = s;
       p->parts = static_cast<int>(parts < cdiv(tiles, kWsWarps) ? parts : cdiv(tiles, kWsWarps));
-      p->smem = smem;
+      p->smem = ws_smem_bytes(int(M), int(gs) * G, G);
     }
   }
   return best >= 0;
 }
+
 int launch_join(const float* part, int slices, int64_t ld, const EpiArgs& ep, cudaStream_t st) {
   const int64_t chunks = cdiv(ep.N, 256);
   if (ep.M * chunks > kIntMax) return B200Q_ERR_UNSUPPORTED;
@@ -184,7 +186,7 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
 // and the decoded copy with the pair GEMM is ahead: 300 tokens 101 us, 164 by tiles.)
 constexpr int64_t kW4MaxTileM = 256;
 bool w4_tiles(int64_t M, int64_t N, int64_t K) {
-  return M > kW4MaxSmallM && M <= kW4MaxTileM && N <= (int64_t(1) << 30) && K <= (int64_t(1) << 24);
+  return M <= kW4MaxTileM && N <= (int64_t(1) << 30) && K <= (int64_t(1) << 24);
 }
 // K slices of the tile kernel: the split with the lowest estimate, in cycles.  A slot takes four
 // times the longest of a stage's MMAs, its bytes from L2 and its decode; a tile its start and
@@ -281,7 +283,9 @@ int launch_w4_tile(const W4TilePlan& p, const void* x, int x_dtype, int64_t ldx,
 
 // The kernels of a call and the workspace they take.  The integer kernel for few tokens wants
 // scales of x's type and indexes them with 31 bits, as the slice kernel does.
-enum W4Kind { kW4None, kW4Digits, kW4Slices, kW4Tiles, kW4Decoded };
+// (Up to 32 tokens whose x fits no slice, K above 194,176 at 32, or with 2^31 scales go on to
+// the kernels for more.)
+enum W4Kind { kW4Digits, kW4Slices, kW4Tiles, kW4Decoded };
 struct W4Route {
   W4Kind kind;
   WdPlan wd;
@@ -294,16 +298,16 @@ W4Route w4_route(int sms, int64_t M, int64_t N, int64_t K, int64_t G, bool same_
   const bool small = N * (K / G) <= kIntMax;
   if (same_type && small && wd_plan(sms, M, N, K, int(G), &r.wd)) {
     r.kind = kW4Digits;
+  } else if (M <= kW4MaxSmallM && small && ws_plan(sms, M, N, K, int(G), &r.ws)) {
+    r.kind = kW4Slices;
+    r.need = r.ws.slices > 1 ? size_t(r.ws.slices) * M * N * 4 : 0;
   } else if (w4_tiles(M, N, K)) {
     r.kind = kW4Tiles;
     r.tile = w4_tile_plan(sms, M, N, K);
     r.need = w4_tile_work(r.tile, M, N, K, G).total;
-  } else if (M > kW4MaxSmallM) {
+  } else {
     r.kind = kW4Decoded;
     r.need = w4_work(M, N, K).total;
-  } else if (small && ws_plan(sms, M, N, K, int(G), &r.ws)) {
-    r.kind = kW4Slices;
-    r.need = r.ws.slices > 1 ? size_t(r.ws.slices) * M * N * 4 : 0;
   }
   return r;
 }
@@ -492,7 +496,6 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
   ep.M = static_cast<int>(M);
   ep.N = static_cast<int>(N);
   const W4Route route = w4_route(sms, M, N, K, group, scale_dtype == x_dtype + 1);
-  if (route.kind == kW4None) return B200Q_ERR_UNSUPPORTED;
   const size_t need = route.need;
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256))) return B200Q_ERR_WORKSPACE;
   const bool x_vec = aligned(x, 16) && ldx % 8 == 0;

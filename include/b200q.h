@@ -377,9 +377,10 @@ B200Q_API int b200q_fp8_decode(const uint8_t* src, int64_t n, int fp8_kind, void
  * [N, K/group] contiguous, scale_dtype a B200Q_BIAS_* code; zeros [N, K/group]
  * bytes 0..15 or NULL (8).  group 32, 64 or 128, K % group == 0.  X [M, K]
  * bf16/f16, bias bf16/f16/f32 or NULL, out bf16/f16/f32.  fp32 accumulation.
- * M <= 32 rounds once, at the output; larger M rounds each weight once to fp16's
- * 11 bits: up to 256 as it is multiplied, above that in a decoded copy in the
- * workspace (f16 X then needs rows on 16-byte boundaries).  The workspace holds
+ * M <= 32 rounds once, at the output (while a 148th of x's rows fits a CTA's shared
+ * memory: K up to 194,176 at M = 32, more with fewer); others round each weight
+ * once to fp16's 11 bits: up to 256 as it is multiplied, above that in a decoded
+ * copy in the workspace (f16 X then needs rows on 16-byte boundaries).  The workspace holds
  * at least b200q_w4a16_workspace_bytes of the call (0: none needed), 256-byte
  * aligned; b200q_w4a16_workspace_size is the largest of these over group sizes
  * and types. */

@@ -66,6 +66,21 @@ def test_small_activations_and_large_scales(native, M):
     assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, False)).all())
 
 
+# (M, K, G) around the longest K whose slice of x fits beside the rings, and past the tile
+# kernel's fallback
+@pytest.mark.parametrize("M,K,G", [(32, 41984, 32), (32, 42016, 32), (17, 53248, 32), (32, 53248, 32),
+                                   (24, 56352, 32), (32, 53312, 64), (32, 57472, 128), (32, 200000, 32),
+                                   (1, 200000, 32), (9, 300032, 128)])
+def test_long_rows_of_few_tokens(native, M, K, G):
+    x, w, s, z, b = make(M, 40, K, G, torch.bfloat16, True, seed=M)
+    out = w4.w4a16_linear(*dev(x, w, s, z), None, None, torch.float32)
+    ref, size = ref64.w4_linear(x, w, s, z)
+    # fp32 sums: 2^-17 covers 5120 additions in any order, a slice and the join at most
+    # K / 32 / G + 64 here
+    exact = K < 190000
+    assert bool(((out.double().cpu() - ref).abs() <= bound(out, ref, size, exact)).all())
+
+
 @pytest.mark.parametrize("dtype,scale_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16),
                                                (torch.bfloat16, torch.float16), (torch.float16, torch.float32)])
 @pytest.mark.parametrize("M", [1, 2, 3])
