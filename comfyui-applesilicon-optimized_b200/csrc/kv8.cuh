@@ -108,12 +108,13 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
   const uint16_t tb = static_cast<uint16_t>(top);
   const float amax = to_float<T>(*reinterpret_cast<const T*>(&tb));
   const float grown = __fdiv_rn(amax, 127.0f);
-  // a NaN on either side must win, so that the block reads back as NaN
-  const float s = before > grown || before != before ? before : grown;
+  // an infinity or NaN on either side makes the scale NaN, so that the block reads back as NaN
+  // (codes times inf would be infinities whose signs say nothing)
+  const float most = before > grown || before != before ? before : grown;
+  const float s = most <= 3.402823466e38f ? most : __uint_as_float(0x7FC00000u);
   if (tid == 0) *scale = s;
-  // a zero scale's block holds zeros, an infinite or NaN one's reads back as NaN anyway;
-  // a scale below 2^-128 would have an infinite reciprocal
-  const float inv = s > 0.0f && s <= 3.402823466e38f ? fminf(__fdiv_rn(1.0f, s), 3.402823466e38f) : 0.0f;
+  // a zero scale's block holds zeros, a NaN one's codes do not matter; a scale below 2^-128 would have an infinite reciprocal
+  const float inv = s > 0.0f ? fminf(__fdiv_rn(1.0f, s), 3.402823466e38f) : 0.0f;
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int i = (old * dv) + tid + k * kKvThreads;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendA
     }
   }
   if (old > 0 && s != before) {
-    const float ratio = s > 0.0f && s <= 3.402823466e38f ? __fdiv_rn(before, s) : 0.0f;
+    const float ratio = s > 0.0f ? __fdiv_rn(before, s) : 0.0f;
     for (int i = tid; i < old * dv; i += kKvThreads) {
       __align__(8) int8_t o[8];
       *reinterpret_cast<uint2*>(o) = *reinterpret_cast<const uint2*>(codes + i * 8);
@@ -371,7 +372,10 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     int page = -1;
     if (tile < tiles && (base + (lane / kAttnWarps)) < c1) page = kv8_page(c, b, pos >> c.log_t);
     const int64_t at = static_cast<int64_t>(page < 0 ? 0 : page) * c.heads + h;
-    const float ks = __ldg(c.ks + at), vs = __ldg(c.vs + at);
+    float ks = __ldg(c.ks + at);
+    const float vs = __ldg(c.vs + at);
+    // scores of an infinite scale are NaN, never the -inf of a masked position
+    if (!(fabsf(ks) <= 3.402823466e38f)) ks = __uint_as_float(0x7FC00000u);
     const bool lead = page >= 0 && (lane & (per_box - 1)) == 0;
     const unsigned leads = __ballot_sync(0xffffffffu, lead);
     const int y = static_cast<int>(at * c.T) + (pos & (c.T - 1));

@@ -7,7 +7,8 @@ fp32 one scale for each page and head: value = code * scale.  ``block_table``
 
 * ``kv8_append`` writes new tokens behind each sequence's length.  A block's scale
   only grows: it becomes max(its scale so far, max|new| / 127), and codes already
-  there are requantized when it does.
+  there are requantized when it does.  An infinity or NaN makes its block's scale
+  NaN: the block reads back as NaN, and so do the rows of attention that see it.
 * ``kv8_gather`` reads tokens back as 16-bit or fp32 values.
 * ``kv8_attention`` is softmax(q K^T) V over the cache, for one query token or
   many, causal or not, with grouped heads.

@@ -1,0 +1,61 @@
+"""The paged 8-bit cache at the edges of its kernels: values that are not finite, scales far
+from 1, prompts of many rows, counts that do not fit (bounds as in test_gpu_kv8.py)."""
+import math
+
+import pytest
+import torch
+
+import ref64
+from b200q import kv8
+from test_gpu_kv8 import dev, i32, pool, run_attention
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+# query heads per cache head and tokens on each attention kernel: up to 8 rows, up to 16, up
+# to 128, more
+ROWS = [(2, 2), (4, 3), (5, 8), (6, 40)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("start", [0, 5])
+def test_an_infinite_value_makes_its_block_nan(native, dtype, sign, start):
+    """Every token of the block, those already there among them; no other block."""
+    g = torch.Generator().manual_seed(start)
+    kc, vc, ks, vs, table = dev(*pool(1, 2, 16, 64, 4))
+    k, v = (torch.randn(1, 2, 40, 64, generator=g).to(dtype) for _ in range(2))
+    k[0, 0, 3, 7], v[0, 1, 20, 1] = sign * math.inf, sign * math.inf
+    kv8.kv8_append(*dev(k, v), kc, vc, ks, vs, table, i32(start).to(DEV))
+    n = start + 40
+    back = kv8.kv8_gather(kc, vc, ks, vs, table, i32(0).to(DEV), i32(n).to(DEV), n, torch.float32)
+    for x, h, at in ((back[0], 0, start + 3), (back[1], 1, start + 20)):
+        bad = torch.zeros(2, n, dtype=torch.bool, device=DEV)
+        bad[h, at // 16 * 16:at // 16 * 16 + 16] = True
+        assert bool(x[0][bad].isnan().all()) and bool(x[0][~bad].isfinite().all())
+
+
+@pytest.mark.parametrize("G,Tq", ROWS)
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_over_an_infinite_key(native, G, Tq, D):
+    """A row that sees the key's block is NaN, whatever the sign of its products; rows that do
+    not see it are what they were."""
+    g = torch.Generator().manual_seed(G)
+    kc, vc, ks, vs, table = dev(*pool(1, 2, 16, D, 8, seed=G))
+    q = torch.randn(1, 2 * G, Tq, D, generator=g).to(torch.float16).to(DEV)
+    k, v = (torch.randn(1, 2, 1, D, generator=g).to(torch.float16).to(DEV) for _ in range(2))
+    n = 81  # the block of the last token holds no other
+    lens = i32(n).to(DEV)
+    kv8.kv8_append(k, v, kc, vc, ks, vs, table, i32(n - 1).to(DEV))
+    clean, clean_lse = kv8.kv8_attention(q, kc, vc, ks, vs, table, lens)
+    for sign in (1, -1):
+        k[0, 1, 0, 3] = sign * math.inf
+        kv8.kv8_append(k, v, kc, vc, ks, vs, table, i32(n - 1).to(DEV))
+        out, lse = kv8.kv8_attention(q, kc, vc, ks, vs, table, lens)
+        hit = torch.zeros(1, 2 * G, Tq, dtype=torch.bool, device=DEV)
+        hit[:, G:, -1] = True  # causal: the last query alone sees position n - 1
+        assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
+        assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+    # a scale that is already infinite in the pool
+    ks[int(table[0, 1]), 0] = math.inf
+    out, lse = kv8.kv8_attention(q, kc, vc, ks, vs, table, lens)
+    assert bool(out[:, :G].isnan().all()) and bool(lse[:, :G].isnan().all())
