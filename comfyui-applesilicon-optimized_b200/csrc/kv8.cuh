@@ -342,6 +342,10 @@ __device__ __forceinline__ uint32_t q_pair(uint32_t raw, int f16, float inv) {
   return pack_f16x2(a * inv, b * inv);
 }
 
+// Whether a row whose largest |q| has these bits is finite.  Every score of one that is not is
+// an infinity or NaN, so its softmax is NaN: its scores are made NaN, as -inf would be masked.
+__device__ __forceinline__ bool q_finite(uint32_t top, int f16) { return top < (f16 ? 0x7C00u : 0x7F80u); }
+
 // A row's m is its largest exponent less this: P <= 2^15 uses fp16's whole range, so
 // weights down to 2^-29 of the largest keep all their bits (P <= 1 loses bits below
 // 2^-14, which shows where blocks' V scales lie far apart).
@@ -557,12 +561,11 @@ __global__ void __launch_bounds__(kAttnThreads)
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
     float inv = 1.0f, up = 1.0f;
     if (!a.q_f16) {
-      int ex = static_cast<int>(top >> 7);
-      ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+      const int ex = min(max(static_cast<int>(top >> 7), 1), 253);
       inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
       up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
     }
-    sc[i] = a.scale_log2 * up;
+    sc[i] = q_finite(top, a.q_f16) ? a.scale_log2 * up : __uint_as_float(0x7FC00000u);
 #pragma unroll
     for (int j = 0; j < KS; ++j) {
       qf[j][i] = q_pair(raw[2 * j], a.q_f16, inv);

@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
     lim = attn_limit(a, len, ti);
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.qb + hi * a.qh + ti * a.qt;
     float inv = 1.0f, up = 1.0f;
+    uint32_t top = 0;
     if (!a.q_f16) {
-      uint32_t top = 0;
 #pragma unroll 4
       for (int j = 0; j < D / 8; ++j) {
         const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
@@ -194,19 +194,23 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7FFFu, (u[i] >> 16) & 0x7FFFu));
       }
-      int ex = static_cast<int>(top >> 7);
-      ex = ex == 255 ? 127 : min(max(ex, 1), 253);  // inf / NaN rows keep their values
+      const int ex = min(max(static_cast<int>(top >> 7), 1), 253);
       inv = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
       up = __uint_as_float(static_cast<uint32_t>(ex) << 23);
     }
-    sc = a.scale_log2 * up;
 #pragma unroll 4
     for (int j = 0; j < D / 8; ++j) {
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + j);
+      if (a.q_f16) {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, max(u[i] & 0x7FFFu, (u[i] >> 16) & 0x7FFFu));
+      }
       *reinterpret_cast<uint4*>(qs + (j >> 3) * (kPfRows * 128) + row * 128 + (((j & 7) ^ (row & 7)) << 4)) =
           make_uint4(q_pair(v.x, a.q_f16, inv), q_pair(v.y, a.q_f16, inv), q_pair(v.z, a.q_f16, inv),
                      q_pair(v.w, a.q_f16, inv));
     }
+    sc = q_finite(top, a.q_f16) ? a.scale_log2 * up : __uint_as_float(0x7FC00000u);
     fence_proxy_async_smem();
   }
   tc_fence_before();

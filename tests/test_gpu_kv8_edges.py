@@ -59,3 +59,22 @@ def test_attention_over_an_infinite_key(native, G, Tq, D):
     ks[int(table[0, 1]), 0] = math.inf
     out, lse = kv8.kv8_attention(q, kc, vc, ks, vs, table, lens)
     assert bool(out[:, :G].isnan().all()) and bool(lse[:, :G].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("G,Tq", ROWS)
+def test_infinite_query(native, dtype, G, Tq):
+    """An infinity in q: its scores are infinite with the keys' signs, or NaN, so its row is NaN,
+    also where every one of them is -inf; a row that sees nothing stays 0 and -inf."""
+    c = pool(2, 1, 16, 64, 6, seed=3)
+    c[0][..., 5] = -c[0][..., 5].abs().clamp(min=1)  # every key is negative there
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(2, G, Tq, 64, generator=g).to(dtype)
+    lens = i32(90, 0)
+    clean, clean_lse = kv8.kv8_attention(q.to(DEV), *dev(*c), lens.to(DEV), False)
+    q[:, 0, 0, 5] = math.inf
+    out, lse = kv8.kv8_attention(q.to(DEV), *dev(*c), lens.to(DEV), False)
+    hit = torch.zeros(2, G, Tq, dtype=torch.bool, device=DEV)
+    hit[0, 0, 0] = True
+    assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
