@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kKvThreads) kv8_gather_kernel(const Kv8GatherA
 // so V's scales cost one add per score instead of a pass over the accumulators,
 // and P fits fp16 whatever the scales are: P's fp16 rounding (2^-11 relative,
 // 2^-40 of the row's largest weight at least) is the only one before the
-// output's.  A block with vs = 0 adds its P to the sum only.
+// output's.  A block with vs = 0 adds its P / 2^-80 to the sum only, as if vs were 2^-80.
 //
 // Layout, D = 128: lane (g, t) loads 32 consecutive bytes (quarter t) of K token
 // g, and 16 bytes (eighth g) of V tokens 2t, 2t+1, 2t+8, 2t+9: every load of the
@@ -264,7 +264,7 @@ constexpr int kAttnThreads = (kAttnWarps + 1) * 32;  // and a producer warp
 
 // The CTA's ring: stages of 64 tokens of K and V, brought by TMA with the row
 // swizzle; 16-token tile w of a stage belongs to consumer warp w.  meta: per tile
-// {ks, log2 vs, 1 / vs, state}, state 0 = skip (bad page), 1 = ok, 2 = vs is 0.
+// {ks, log2 vs, 1 / vs, state}, state 0 = skip (bad page), 1 = ok, 2 = V is 0.
 template <int D, int ST = kAttnStages>
 struct AttnRing {
   uint8_t k[ST][16 * kAttnWarps * D];
@@ -395,9 +395,11 @@ __device__ __forceinline__ void attn_produce(const Kv8AttnArgs& a, const CUtenso
     const int many = min(32 / kAttnWarps, c1 - base);
     if (n == 0)
       for (int i = 0; i < min(many, ST); ++i) copy(i, i);
-    float4 meta = make_float4(ks, 0.0f, 1.0f, 2.0f);
-    // below 2^-80 (values under 2^-73) a block counts as one of zeros: P / vs must not overflow
-    if (!(fabsf(vs) < 8.2718061e-25f)) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
+    // below 2^-80 (values under 2^-73) a block counts as one of zeros at scale 2^-80: P / vs must
+    // not overflow, and its weights, which reach the sum alone, must not raise m and with it
+    // take the bits of weights whose blocks' scales are small but not zero
+    float4 meta = make_float4(ks, -80.0f, 0x1p80f, 2.0f);
+    if (!(fabsf(vs) < 0x1p-80f)) meta = make_float4(ks, log2f(vs), 1.0f / vs, 1.0f);
     if (page < 0) meta = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
     for (int i = 0; i < many; ++i, ++n) {
       const int s = n % ST;

@@ -78,3 +78,22 @@ def test_infinite_query(native, dtype, G, Tq):
     hit[0, 0, 0] = True
     assert bool(out[hit].isnan().all()) and bool(lse[hit].isnan().all())
     assert torch.equal(out[~hit], clean[~hit]) and torch.equal(lse[~hit], clean_lse[~hit])
+
+
+@pytest.mark.parametrize("G,Tq", ROWS)
+@pytest.mark.parametrize("power", [-20, -40, -60])
+def test_a_block_of_zero_values_beside_small_ones(native, G, Tq, power):
+    """A block whose values are all zero counts in the softmax's sum alone: the weights of the
+    other blocks keep their bits however small those blocks' scales are."""
+    kc, vc, ks, vs, table = pool(1, 2, 16, 64, 16, seed=G)
+    vs = vs * 2.0 ** power
+    vs[int(table[0, 2])] = 0.0
+    g = torch.Generator().manual_seed(Tq)
+    q = torch.randn(1, 2 * G, Tq, 64, generator=g).to(torch.bfloat16)
+    d = dev(kc, vc, ks, vs, table)
+    out, lse = kv8.kv8_attention(q.to(DEV), *d, i32(250).to(DEV))
+    ref, lse_ref, size = ref64.attention(q, kc, vc, ks, vs, table, i32(250), True)
+    tol = ref64.UNIT[q.dtype] * ref.abs() + 2.0 ** -10 * size
+    err = (out.double().cpu() - ref).abs()
+    assert bool((err <= tol).all()), f"worst {(err / tol).max().item():.3g} of the bound"
+    assert bool(((lse.double().cpu() - lse_ref).abs() <= 2.0 ** -17 * (1 + lse_ref.abs())).all())
