@@ -97,3 +97,19 @@ def test_a_block_of_zero_values_beside_small_ones(native, G, Tq, power):
     err = (out.double().cpu() - ref).abs()
     assert bool((err <= tol).all()), f"worst {(err / tol).max().item():.3g} of the bound"
     assert bool(((lse.double().cpu() - lse_ref).abs() <= 2.0 ** -17 * (1 + lse_ref.abs())).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16])
+@pytest.mark.parametrize("power", [-100, -120, -130])
+def test_append_of_vanishing_values(native, dtype, power):
+    """Codes are the rounded quotients also where the scale's reciprocal is not finite."""
+    g = torch.Generator().manual_seed(1)
+    x = (torch.rand(1, 1, 16, 64, generator=g) * 2 - 1)
+    x = (x * 2.0 ** power).to(dtype) if power > -126 else (x * 2.0 ** -100).mul(2.0 ** (power + 100)).to(dtype)
+    kc, vc, ks, vs, table = dev(*pool(1, 1, 16, 64, 1))
+    kv8.kv8_append(*dev(x, x), kc, vc, ks, vs, table, i32(0).to(DEV))
+    page = int(table[0, 0])
+    s = ks[page, 0].cpu()
+    assert torch.equal(s, (x.float().abs().max() / torch.tensor(127.0)))
+    want = (x[0, 0].double() / s.double())
+    assert bool(((kc[page, 0].cpu().double() - want).abs() <= 0.5 + 2.0 ** -16).all())
