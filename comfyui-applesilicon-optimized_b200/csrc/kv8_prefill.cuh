@@ -162,9 +162,10 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
   griddep_launch_dependents();
 
   const Kv8Cache& c = a.c;
-  const int split = blockIdx.x, b = attn_sequence(a), rows = a.G * a.Tq;
-  const int row_tiles = (rows + kPfRows * RT - 1) / (kPfRows * RT);
-  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * (kPfRows * RT);
+  // grid (splits * heads * row tiles, 1, B): a prompt's heads x tiles go past what y holds
+  const int split = blockIdx.x % a.splits, b = attn_sequence(a), rows = a.G * a.Tq;
+  const int row_tiles = (rows + kPfRows * RT - 1) / (kPfRows * RT), tile = blockIdx.x / a.splits;
+  const int h = tile / row_tiles, r0 = (tile - h * row_tiles) * (kPfRows * RT);
   const int len = min(max(a.lens[b], 0), c.max_blocks << c.log_t);
   const int last = min(r0 + kPfRows * RT, rows) - 1;
   const int lim_max = attn_limit(a, len, last / a.G), lim_min = attn_limit(a, len, r0 / a.G);

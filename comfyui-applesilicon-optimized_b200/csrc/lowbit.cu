@@ -448,7 +448,7 @@ size_t attn_work_bytes(int splits, int64_t rows, int64_t D) {
 }
 bool attn_dims(int64_t B, int64_t Hq, int64_t heads, int64_t Tq) {
   return B >= 0 && B <= 65535 && heads >= 1 && Hq >= heads && Hq % heads == 0 && Tq >= 0 &&
-         Hq / heads * Tq <= kIntMax && B * Hq * Tq <= kIntMax && heads * cdiv(Hq / heads * Tq, 16) <= 65535;
+         Hq * Tq <= kIntMax && B * Hq * Tq <= kIntMax;
 }
 
 }  // namespace
@@ -726,8 +726,10 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   a.longest_first = B > 1 && B <= 32 && B * heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq)) * splits > sms;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const dim3 grid(static_cast<unsigned>(splits), static_cast<unsigned>(heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq))),
-                  static_cast<unsigned>(B));
+  const int64_t tiles = heads * cdiv(a.G * Tq, attn_row_tile(a.G * Tq));  // heads (<= 65535) up to 16 rows
+  if (tiles * splits > kIntMax) return B200Q_ERR_UNSUPPORTED;
+  const dim3 grid = a.G * Tq > 16 ? dim3(static_cast<unsigned>(tiles * splits), 1, static_cast<unsigned>(B))
+                                  : dim3(static_cast<unsigned>(splits), static_cast<unsigned>(tiles), static_cast<unsigned>(B));
   // the pool as rows of D bytes; a page's rows of one head are contiguous
   const int64_t pool_rows = pages * heads * block;
   const uint32_t box = static_cast<uint32_t>(block < kAttnBox ? block : kAttnBox);

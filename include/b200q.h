@@ -453,7 +453,7 @@ B200Q_API int b200q_kv8_gather(const int8_t* k_codes, const int8_t* v_codes, con
  * causal: query i of Tq sees positions <= lens[b] - Tq + i; otherwise all.  out
  * [B, Hq, Tq, D] like q, lse [B, Hq, Tq] fp32 contiguous (natural log of the
  * softmax's sum); a row that sees nothing gives 0 and -inf.  max_len: an upper
- * bound of lens used for planning only.  workspace:
+ * bound of lens used for planning only.  B <= 65535, B * Hq * Tq < 2^31.  workspace:
  * b200q_kv8_attention_workspace_size bytes (same max_len). */
 B200Q_API size_t b200q_kv8_attention_workspace_size(int64_t B, int64_t Hq, int64_t heads,
                                                     int64_t Tq, int64_t D, int64_t max_len);

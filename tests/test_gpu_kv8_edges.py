@@ -113,3 +113,31 @@ def test_append_of_vanishing_values(native, dtype, power):
     assert torch.equal(s, (x.float().abs().max() / torch.tensor(127.0)))
     want = (x[0, 0].double() / s.double())
     assert bool(((kc[page, 0].cpu().double() - want).abs() <= 0.5 + 2.0 ** -16).all())
+
+
+@pytest.mark.parametrize("Hq,H,Tq", [(64, 8, 16384), (40, 8, 26300), (1, 1, 131)])
+def test_prompts_of_many_rows(native, Hq, H, Tq):
+    """The number of a call's 16-row tiles is no limit: what runs is tiles of 256 rows."""
+    c = pool(1, H, 16, 64, 3, seed=1)
+    g = torch.Generator().manual_seed(Tq)
+    q = torch.randn(1, Hq, Tq, 64, generator=g).to(torch.bfloat16)
+    run_attention(q, c, i32(37), True)
+    run_attention(q[:, :, :500], c, i32(37), False)
+
+
+@pytest.mark.parametrize("H,G,Tq", [(65535, 1, 17), (960, 1, 18000)])
+def test_row_tiles_and_heads_past_65535(native, H, G, Tq):
+    """Heads x row tiles of a call go past what one axis of a grid holds in its y and z."""
+    D, T = 64, 16
+    kc = torch.randint(-127, 128, (1, H, T, D), dtype=torch.int8, device=DEV)
+    vc = torch.randint(-127, 128, (1, H, T, D), dtype=torch.int8, device=DEV)
+    ks, vs = (torch.full((1, H), 0.01, device=DEV) for _ in range(2))
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    q = torch.randn(1, H * G, Tq, D, dtype=torch.float16, device=DEV)
+    out, lse = kv8.kv8_attention(q, kc, vc, ks, vs, table, i32(9).to(DEV), False)
+    for h in (0, H // 2, H - 1):
+        k, v = (t[0, h, :9].double() * 0.01 for t in (kc, vc))
+        p = torch.softmax(q[0, h * G].double() @ k.t() * D ** -0.5, -1)
+        ref, size = p @ v, p @ v.abs()
+        err = (out[0, h * G].double() - ref).abs()
+        assert bool((err <= 2.0 ** -11 * ref.abs() + 2.0 ** -10 * size + 1e-7).all())
