@@ -35,7 +35,7 @@ def _load():
 
 def kv8_append(k, v, k_codes, v_codes, k_scale, v_scale, block_table, start, counts=None):
     """Write k, v [B, heads, S, D] (bf16/f16) into the cache, in place: the first
-    counts[b] (all S without counts) tokens of sequence b go to positions start[b],
+    counts[b] (all S without counts, at most S) tokens of sequence b go to positions start[b],
     start[b] + 1, ...  Sequences must not share a page that is written."""
     (_calls or _load())[0](k, v, k_codes, v_codes, k_scale, v_scale, block_table, start, counts)
 
@@ -85,9 +85,10 @@ class KV8Cache:
         return self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.table
 
     def append(self, k, v, counts=None):
-        """Add k, v [B, heads, S, D] behind what is there and advance the lengths."""
+        """Add k, v [B, heads, S, D] behind what is there (sequence b: its first counts[b],
+        at most S and none below 0) and advance the lengths."""
         kv8_append(k, v, *self.pool, self.lens, counts)
-        self.lens += k.shape[2] if counts is None else counts
+        self.lens += k.shape[2] if counts is None else counts.clamp(0, k.shape[2])
 
     def attention(self, q, causal=True, scale=None, max_len=None):
         """out [B, Hq, Tq, D] over everything appended so far."""

@@ -141,3 +141,15 @@ def test_row_tiles_and_heads_past_65535(native, H, G, Tq):
         ref, size = p @ v, p @ v.abs()
         err = (out[0, h * G].double() - ref).abs()
         assert bool((err <= 2.0 ** -11 * ref.abs() + 2.0 ** -10 * size + 1e-7).all())
+
+
+def test_counts_outside_the_tokens_given(native):
+    """counts above S write S tokens and negative ones none: the lengths say the same."""
+    cache = kv8.KV8Cache(3, 1, 64, 64, block=16, device=DEV)
+    x = torch.randn(3, 1, 5, 64).to(torch.bfloat16).to(DEV)
+    cache.append(x, x, i32(9, -2, 3).to(DEV))
+    assert cache.lens.tolist() == [5, 0, 3]
+    cache.append(x[:, :, :2], x[:, :, :2])
+    assert cache.lens.tolist() == [7, 2, 5]
+    k = cache.values(9, torch.float32)[0]
+    assert bool((k[0, :, 7:] == 0).all()) and bool((k[0, :, :7].abs().amax(-1) > 0).all())
