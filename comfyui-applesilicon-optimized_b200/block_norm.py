@@ -73,21 +73,24 @@ def _register():
     post = ("Tensor residual, Tensor y, Tensor? gate=None, Tensor? post_weight=None, "
             "str post_kind='none', float residual_scale=1.0")
 
+    def like(x):  # contiguous, whatever x's strides
+        return x.new_empty(x.shape)
+
     def codes(x):
         rows = x.numel() // x.shape[-1]
         return (x.new_empty((rows, x.shape[-1]), dtype=torch.int8),
                 x.new_empty((rows, 1), dtype=torch.float32))
 
     for fn, schema, fake in (
-            (norm_modulate, f"(Tensor x, {pre}) -> Tensor", lambda x, *a, **k: torch.empty_like(x)),
+            (norm_modulate, f"(Tensor x, {pre}) -> Tensor", lambda x, *a, **k: like(x)),
             (norm_modulate_quant_i8, f"(Tensor x, {pre}) -> (Tensor, Tensor)",
              lambda x, *a, **k: codes(x)),
             (gated_residual, f"({post}, float eps=1e-06) -> Tensor",
-             lambda x, *a, **k: torch.empty_like(x)),
+             lambda x, *a, **k: like(x)),
             (gated_residual_norm, f"({post}, {pre}) -> (Tensor, Tensor)",
-             lambda x, *a, **k: (torch.empty_like(x), torch.empty_like(x))),
+             lambda x, *a, **k: (like(x), like(x))),
             (gated_residual_norm_quant_i8, f"({post}, {pre}) -> (Tensor, Tensor, Tensor)",
-             lambda x, *a, **k: (torch.empty_like(x), *codes(x)))):
+             lambda x, *a, **k: (like(x), *codes(x)))):
         name = fn.__name__
         _LIB.define(name + schema)
         _LIB.impl(name, fn, "CUDA")

@@ -428,10 +428,10 @@ B200Q_API int b200q_block_norm(const void* x, int64_t ldx, const void* y, int64_
  *
  * append: k, v [B, heads, S, D] bf16/f16 (strides of the first three axes, in
  * elements, multiples of 8; 16-byte aligned): sequence b's first counts[b]
- * tokens (NULL: S) go to positions start[b], start[b] + 1, ...  A block's scale
- * becomes max(its scale if it already holds tokens, max|new| / 127), NaN where
- * that is not finite; codes it holds are requantized when the scale grew.  Sequences must not share a page
- * that is written. */
+ * tokens (NULL: S; at most S) go to positions start[b], start[b] + 1, ...  A
+ * block's scale becomes max(its scale if it already holds tokens, max|new| /
+ * 127), NaN where that is not finite; codes it holds are requantized when the
+ * scale grew.  Sequences must not share a page that is written. */
 B200Q_API int b200q_kv8_append(const void* k, const void* v, int dtype, int64_t B, int64_t S,
                                const int64_t* k_strides, const int64_t* v_strides,
                                int8_t* k_codes, int8_t* v_codes, float* k_scale, float* v_scale,

@@ -5,6 +5,18 @@ import torch
 import b200q  # noqa: F401  (registers the operators)
 
 
+@pytest.mark.parametrize("shape,order", [((5, 3, 256), (1, 0, 2)), ((4, 6), (1, 0)), ((2, 3, 4, 32), (0, 2, 1, 3))])
+def test_fake_norms_are_contiguous(shape, order):
+    """The kernels write contiguous outputs whatever x's strides are."""
+    with torch._subclasses.FakeTensorMode():
+        x = torch.empty(shape, dtype=torch.bfloat16, device="cuda").permute(order)
+        ops = torch.ops.b200q
+        outs = [ops.norm_modulate(x), ops.gated_residual(x, x), *ops.gated_residual_norm(x, x),
+                ops.gated_residual_norm_quant_i8(x, x)[0]]
+        for o in outs:
+            assert o.shape == x.shape and o.dtype == x.dtype and o.is_contiguous()
+
+
 def test_w4a16_workspaces():
     """The workspace of a call without shape-only guesses: the size function covers every group
     size and type, and calls whose scales are not of x's type get one for their K slices."""
