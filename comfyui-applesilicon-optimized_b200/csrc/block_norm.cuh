@@ -327,6 +327,34 @@ __device__ __forceinline__ void fold_mods(const NormArgs& a, int64_t mod, int c,
   if (a.shift) load_vals<8>(a.shift, a.mod_dtype, mod * a.ld_shift + c, b);
 }
 
+// A row's INT8 codes: the nearest integers of the rounded quotients v / s (16-bit rows meet
+// exact ties often, half of the row's largest value among them).  The quotient is the product
+// with 1 / s and one correction by its remainder; the nearest integer is the low byte of its
+// sum with 1.5 * 2^23.  `lift` brings a row whose scale is below 2^-100, where the remainder
+// and the reciprocal leave fp32's range, up by 2^64 (and holds it to 127 of a scale that was
+// rounded to a few bits).
+struct RowCodes {
+  float s, inv;
+  __device__ __forceinline__ explicit RowCodes(float scale) {
+    s = scale < 0x1p-100f ? scale * 0x1p64f : scale;
+    inv = scale > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
+    if (!(scale > 0.0f)) s = 0.0f;  // of zeros, or NaN: codes of 0
+  }
+  template <int NPT, int VEC>
+  __device__ __forceinline__ static void lift(float scale, float (&v)[NPT][VEC]) {
+    if (!(scale > 0.0f && scale < 0x1p-100f)) return;
+    const float most = 127.0f * (scale * 0x1p64f);
+#pragma unroll
+    for (int k = 0; k < NPT; ++k)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[k][j] = fminf(fmaxf(v[k][j] * 0x1p64f, -most), most);
+  }
+  __device__ __forceinline__ uint32_t operator()(float v) const {
+    const float y = v * inv;
+    return __float_as_uint(fmaf(fmaf(-y, s, v), inv, y) + 12582912.0f);
+  }
+};
+
 // PERSIST: CTAs loop over contiguous rows, the folded vectors in shared memory (AFTER 3,
 // else 2; a thread writes and reads its own columns; the first four values of all
 // vectors, then the other four, so that neighbouring threads read neighbouring words).  Otherwise one row per CTA, one
@@ -458,15 +486,14 @@ __global__ void __launch_bounds__(PERSIST ? 512 : 1024) block_norm_rows_kernel(c
     const float t = __uint_as_float(top);
     const float s = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);
     if (threadIdx.x == 0) a.q_scale[row] = s;
-    // out / s as a product with 1 / s, within 2^-23 of the quotient; the nearest integer
-    // is the low byte of the sum with 1.5 * 2^23 (at most 127 in magnitude)
-    const float inv = s > 0.0f ? fminf(__fdiv_rn(1.0f, s), 3.402823466e38f) : 0.0f;
+    const RowCodes code(s);
+    RowCodes::lift(s, v);
 #pragma unroll
     for (int k = 0; k < NPT; ++k)
       if (FULL || on[k]) {
         uint32_t o[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(fmaf(v[k][j], inv, 12582912.0f));
+        for (int j = 0; j < 8; ++j) o[j] = code(v[k][j]);
         *reinterpret_cast<uint2*>(a.q + row * a.ldq + col[k]) =
             make_uint2(low_bytes(o[0], o[1], o[2], o[3]), low_bytes(o[4], o[5], o[6], o[7]));
       }
@@ -636,14 +663,15 @@ __global__ void __launch_bounds__(512) block_norm_loose_kernel(const NormArgs a)
     const float t = __uint_as_float(top);
     const float sc = top >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : __fdiv_rn(t, 127.0f);
     if (threadIdx.x == 0) a.q_scale[row] = sc;
-    const float inv = sc > 0.0f ? fminf(__fdiv_rn(1.0f, sc), 3.402823466e38f) : 0.0f;  // as above
+    const RowCodes code(sc);
+    RowCodes::lift(sc, v);
     int8_t* qp = a.q + row * a.ldq + c0;
 #pragma unroll
     for (int s = 0; s < S; ++s)
       if (on[s]) {
         uint32_t o[VW];
 #pragma unroll
-        for (int j = 0; j < VW; ++j) o[j] = __float_as_uint(fmaf(v[s][j], inv, 12582912.0f));
+        for (int j = 0; j < VW; ++j) o[j] = code(v[s][j]);
         if constexpr (VW == 2)
           *reinterpret_cast<uint16_t*>(qp + s * kStep) = static_cast<uint16_t>(__byte_perm(o[0], o[1], 0x0040));
         else
