@@ -153,3 +153,38 @@ def test_counts_outside_the_tokens_given(native):
     assert cache.lens.tolist() == [7, 2, 5]
     k = cache.values(9, torch.float32)[0]
     assert bool((k[0, :, 7:] == 0).all()) and bool((k[0, :, :7].abs().amax(-1) > 0).all())
+
+
+# ---- the widest forms against 64 bits
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("H,G,Tq", [(2, 5, 129), (1, 4, 33), (1, 3, 43), (1, 17, 1), (2, 1, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_row_tiles_over_split_lengths(native, D, H, G, Tq, causal):
+    """Both tile kernels with their lengths split over CTAs, ragged, one shorter than its
+    queries and one empty."""
+    c = pool(4, H, 64, D, 18, seed=D + G)
+    g = torch.Generator().manual_seed(Tq)
+    q = torch.randn(4, H * G, Tq, D, generator=g).to(torch.float16)
+    run_attention(q, c, i32(1100, 20, 641, 0), causal)
+
+
+@pytest.mark.parametrize("H,G,Tq", [(20, 2, 70), (10, 1, 100)])
+def test_more_tiles_than_places(native, H, G, Tq):
+    """More CTAs than SMs: sequences start by length, equal and empty ones among them."""
+    lens = i32(300, 900, 0, 900, 17, 900, 640, 300)
+    c = pool(8, H, 64, 128, 15, seed=G)
+    g = torch.Generator().manual_seed(Tq)
+    q = torch.randn(8, H * G, Tq, 128, generator=g).to(torch.bfloat16)
+    run_attention(q, c, lens, True)
+
+
+@pytest.mark.parametrize("D,G,Tq", [(128, 5, 700), (64, 1, 513), (128, 1, 1025)])
+def test_prompt_into_an_empty_cache(native, D, G, Tq):
+    """append, then attention of the same tokens: every row sees itself and what is before."""
+    g = torch.Generator().manual_seed(Tq)
+    k, v = (torch.randn(1, 2, Tq, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 2 * G, Tq, D, generator=g).to(torch.bfloat16)
+    cache = kv8.KV8Cache(1, 2, D, Tq, block=32, device=DEV)
+    cache.append(*dev(k, v))
+    pool_ = tuple(t.cpu() for t in cache.pool)
+    run_attention(q, pool_, i32(Tq), True)
