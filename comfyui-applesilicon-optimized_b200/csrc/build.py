@@ -1,6 +1,8 @@
 """Build in-tree: the b200q C-ABI library ``_lib/libb200q.so`` (sm_100a) and, on
 top of it, ``_lib/b200q_bindings.so``, the CPython bindings of the low-bit decode
-operators (``bindings.cpp``, against torch's headers).
+operators (``bindings.cpp``, against torch's headers).  The library needs nvcc alone;
+where a C++ compiler, Python.h or torch's headers are missing the bindings are left
+out with a message, and the low-bit operators raise.
 
 Usage: ``python csrc/build.py [--verbose]``.  Rebuilds only when a source is
 newer than the library.  nvcc cross-compiles, so no GPU is needed.  The
@@ -8,6 +10,7 @@ translation units are compiled without --use_fast_math: the INT8 epilogue and th
 quantizers rely on IEEE round-to-nearest fp32 arithmetic.
 """
 import os
+import shutil
 import subprocess
 import sys
 
@@ -53,6 +56,23 @@ def cxx_runtime():
             if os.path.basename(path).startswith("libstdc++.so.6"):
                 return path
     return "-lstdc++"
+
+
+def bindings_lack():
+    """What the bindings need and this machine has not, or None."""
+    import sysconfig
+    try:
+        import torch
+    except ImportError:
+        return "torch"
+    cxx = os.environ.get("CXX", "g++")
+    if not shutil.which(cxx):
+        return f"a C++ compiler ({cxx})"
+    for header in (os.path.join(sysconfig.get_paths()["include"], "Python.h"),
+                   os.path.join(os.path.dirname(torch.__file__), "include", "ATen", "ATen.h")):
+        if not os.path.exists(header):
+            return header
+    return None
 
 
 def bindings_cmd(out=BINDINGS):
@@ -116,16 +136,24 @@ def build(force=False, verbose=False):
             print(msg)
     if failed:
         raise RuntimeError("\n".join(failed))
-    steps = [link_cmd([object_of(u) for u in UNITS])]
+    run(link_cmd([object_of(u) for u in UNITS]), verbose)
     if force or not newer(BINDINGS, BINDINGS_SOURCES):
-        steps.append(bindings_cmd())
-    for cmd in steps:
-        if verbose:
-            print(" ".join(cmd))
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({r.returncode}):\n{r.stdout}{r.stderr}")
+        lack = bindings_lack()
+        if lack:
+            print(f"[b200q] {BINDINGS} not built: {lack} is missing; the low-bit operators will raise")
+            if os.path.exists(BINDINGS):
+                os.remove(BINDINGS)  # one of another source
+        else:
+            run(bindings_cmd(), verbose)
     return OUT
+
+
+def run(cmd, verbose):
+    if verbose:
+        print(" ".join(cmd))
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({r.returncode}):\n{r.stdout}{r.stderr}")
 
 
 if __name__ == "__main__":

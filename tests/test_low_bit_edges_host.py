@@ -30,3 +30,27 @@ def test_w4a16_workspaces():
     assert L.b200q_w4a16_workspace_bytes(1, 5120, 5120, 128, 0, 3) > 0
     for bad in ((0, 8, 64, 64), (2, 8, 64, 48), (2, 8, 96, 64)):
         assert L.b200q_w4a16_workspace_bytes(*bad, 0, 1) == 0
+
+
+def test_build_without_a_host_compiler(tmp_path, monkeypatch, capsys):
+    """The library is whole without the bindings: a machine that cannot compile them gets it,
+    and a message, in place of an error."""
+    import importlib.util
+    import os
+    from conftest import PACK_DIR
+    spec = importlib.util.spec_from_file_location("b200q_build_test", PACK_DIR / "csrc" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    monkeypatch.setattr(build, "OUT", str(tmp_path / "libb200q.so"))
+    monkeypatch.setattr(build, "BINDINGS", str(tmp_path / "b200q_bindings.so"))
+    monkeypatch.setattr(build, "newer", lambda target, sources: target.endswith(".o"))  # objects are there
+    linked = ["true"]
+    monkeypatch.setattr(build, "link_cmd", lambda objects: linked)
+    monkeypatch.setenv("CXX", "no-such-compiler")
+    assert build.build() == build.OUT
+    assert "no-such-compiler" in capsys.readouterr().out and not os.path.exists(build.BINDINGS)
+    monkeypatch.delenv("CXX")
+    assert build.bindings_lack() is None
+    linked[0] = "false"  # what does not link is still an error
+    with pytest.raises(RuntimeError):
+        build.build()
