@@ -119,7 +119,7 @@ __device__ __forceinline__ void store_vals16(void* p, int dtype, int64_t i, cons
 
 // One CTA per row; thread i holds values i, i + threads, ...  The form for any D,
 // stride and alignment, used where a row is too long for the other two.
-template <int DTYPE, int VEC, int NPT>
+template <int DTYPE, int NPT>
 __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
   __shared__ float bufs[2][32];
   int turn = 0;
@@ -127,15 +127,14 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
   griddep_launch_dependents();
   const int64_t row = blockIdx.x;
   const int mod = static_cast<int>(row / a.rows_per_mod);
-  const int nv = a.D / VEC;
   const float inv_d = 1.0f / static_cast<float>(a.D);
-  float v[NPT][VEC];
+  float v[NPT][1];
 
   auto each = [&](auto f) {
 #pragma unroll
     for (int k = 0; k < NPT; ++k) {
       const int i = threadIdx.x + k * blockDim.x;
-      if (i < nv) f(k, i * VEC);
+      if (i < a.D) f(k, i);
     }
   };
   // norm of the row in v (zeros past its end)
@@ -143,76 +142,56 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
     if (kind == kNormNone) return;
     if (kind == kNormLayer) {
       float s = 0.0f;
-      each([&](int k, int) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += v[k][j];
-      });
+      each([&](int k, int) { s += v[k][0]; });
       const float mean = block_all<false>(s, bufs[turn ^= 1]) * inv_d;
-      each([&](int k, int) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k][j] -= mean;
-      });
+      each([&](int k, int) { v[k][0] -= mean; });
     }
     float s = 0.0f;
-    each([&](int k, int) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) s = fmaf(v[k][j], v[k][j], s);
-    });
+    each([&](int k, int) { s = fmaf(v[k][0], v[k][0], s); });
     const float r = rsqrtf(block_all<false>(s, bufs[turn ^= 1]) * inv_d + a.eps);
-    each([&](int k, int) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] *= r;
-    });
+    each([&](int k, int) { v[k][0] *= r; });
   };
 
   if (a.y) {
-    each([&](int k, int c) { load_vals<VEC>(a.y, DTYPE, row * a.ldy + c, v[k]); });
+    each([&](int k, int c) { load_vals<1>(a.y, DTYPE, row * a.ldy + c, v[k]); });
     normalise(a.post_kind);
     each([&](int k, int c) {
-      float u[VEC];
+      float u[1];
       if (a.post_w) {
-        load_vals<VEC>(a.post_w, a.post_w_dtype, c, u);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k][j] *= u[j];
+        load_vals<1>(a.post_w, a.post_w_dtype, c, u);
+        v[k][0] *= u[0];
       }
       if (a.gate) {
-        load_vals<VEC>(a.gate, a.mod_dtype, mod * a.ld_gate + c, u);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[k][j] *= u[j];
+        load_vals<1>(a.gate, a.mod_dtype, mod * a.ld_gate + c, u);
+        v[k][0] *= u[0];
       }
-      load_vals<VEC>(a.x, DTYPE, row * a.ldx + c, u);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] = fmaf(a.res_scale, u[j], v[k][j]);
-      if (a.h) store_vals16<VEC>(a.h, DTYPE, row * a.ldh + c, v[k]);
+      load_vals<1>(a.x, DTYPE, row * a.ldx + c, u);
+      v[k][0] = fmaf(a.res_scale, u[0], v[k][0]);
+      if (a.h) store_vals16<1>(a.h, DTYPE, row * a.ldh + c, v[k]);
     });
   } else {
-    each([&](int k, int c) { load_vals<VEC>(a.x, DTYPE, row * a.ldx + c, v[k]); });
+    each([&](int k, int c) { load_vals<1>(a.x, DTYPE, row * a.ldx + c, v[k]); });
   }
   if (!a.out && !a.q) return;
   normalise(a.pre_kind);
   float top = 0.0f;
   each([&](int k, int c) {
-    float u[VEC];
+    float u[1];
     if (a.w) {
-      load_vals<VEC>(a.w, a.w_dtype, c, u);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] *= u[j];
+      load_vals<1>(a.w, a.w_dtype, c, u);
+      v[k][0] *= u[0];
     }
     if (a.scale) {
-      load_vals<VEC>(a.scale, a.mod_dtype, mod * a.ld_scale + c, u);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] *= 1.0f + u[j];
+      load_vals<1>(a.scale, a.mod_dtype, mod * a.ld_scale + c, u);
+      v[k][0] *= 1.0f + u[0];
     }
     if (a.shift) {
-      load_vals<VEC>(a.shift, a.mod_dtype, mod * a.ld_shift + c, u);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[k][j] += u[j];
+      load_vals<1>(a.shift, a.mod_dtype, mod * a.ld_shift + c, u);
+      v[k][0] += u[0];
     }
-    if (a.out) store_vals16<VEC>(a.out, DTYPE, row * a.ldo + c, v[k]);
+    if (a.out) store_vals16<1>(a.out, DTYPE, row * a.ldo + c, v[k]);
     // NaN must reach the maximum (fmaxf drops it): compare the bits
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(v[k][j]) & 0x7FFFFFFFu));
+    top = __uint_as_float(max(__float_as_uint(top), __float_as_uint(v[k][0]) & 0x7FFFFFFFu));
   });
   if (!a.q) return;
   // a NaN anywhere in the row makes its scale NaN: block_all's fmaxf would drop it
@@ -221,16 +200,8 @@ __global__ void __launch_bounds__(1024) block_norm_kernel(const NormArgs a) {
   const float s = bad ? __uint_as_float(0x7FC00000u) : __fdiv_rn(top, 127.0f);
   if (threadIdx.x == 0) a.q_scale[row] = s;
   each([&](int k, int c) {
-    __align__(8) int8_t o[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      const float f = s > 0.0f ? rintf(__fdiv_rn(v[k][j], s)) : 0.0f;
-      o[j] = static_cast<int8_t>(fminf(fmaxf(f, -127.0f), 127.0f));
-    }
-    if constexpr (VEC == 8)
-      *reinterpret_cast<uint2*>(a.q + row * a.ldq + c) = *reinterpret_cast<const uint2*>(o);
-    else
-      a.q[row * a.ldq + c] = o[0];
+    const float f = s > 0.0f ? rintf(__fdiv_rn(v[k][0], s)) : 0.0f;
+    a.q[row * a.ldq + c] = static_cast<int8_t>(fminf(fmaxf(f, -127.0f), 127.0f));
   });
 }
 

@@ -332,12 +332,6 @@ __device__ __forceinline__ uint32_t hsub2_1152(uint32_t a) {
 __device__ __forceinline__ uint32_t i8_lo(uint32_t w) { return hsub2_1152(__byte_perm(w, 0x64646464u, 0x4140)); }
 __device__ __forceinline__ uint32_t i8_hi(uint32_t w) { return hsub2_1152(__byte_perm(w, 0x64646464u, 0x4342)); }
 
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // Value of q as fp16 bits after scaling, from bf16 / fp16 bits.
 __device__ __forceinline__ uint32_t q_pair(uint32_t raw, int f16, float inv) {
   float a, b;
@@ -363,7 +357,7 @@ constexpr float kAttnHead = 15.0f;
 
 // log-sum-exp pieces of two halves of a row: (m, l) and the factors of each side.
 __device__ __forceinline__ float safe_ex2_diff(float m, float top) {
-  return m == -INFINITY ? 0.0f : ex2f(m - top);
+  return m == -INFINITY ? 0.0f : ex2_approx(m - top);
 }
 
 // The producer warp: chunks c0 .. c1 - 1 (64 tokens each) of (sequence b, head h).
@@ -469,11 +463,11 @@ struct AttnOut {
 };
 // Joins the warps in order and stores the rows, or hands the CTA's partial to the
 // join kernel.  ml: (m, l) of each warp and row; each warp's o is already scaled to
-// the CTA's maximum.  Called by all threads, for rows r0 .. r0 + live - 1.
+// the CTA's maximum.  Called by all threads, for rows 0 .. rows - 1.
 template <int D, int R>
 __device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, const AttnOut<D, R>* buf,
                                               const float (&ml)[kAttnWarps][R][2], float (&fin)[R][2], int b,
-                                              int h, int split, int r0, int live) {
+                                              int h, int split, int rows) {
   __syncthreads();
   if (threadIdx.x < R) {
     const int r = threadIdx.x;
@@ -486,9 +480,9 @@ __device__ __forceinline__ void attn_epilogue(const Kv8AttnArgs& a, const AttnOu
     fin[r][1] = l;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < live * D; e += kAttnThreads) {
+  for (int e = threadIdx.x; e < rows * D; e += kAttnThreads) {
     const int r = e / D, d = e - r * D, ds = AttnOut<D, R>::at(d);
-    const int row = r0 + r, ti = row / a.G, hi = h * a.G + (row - ti * a.G);
+    const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
     const int64_t flat = (static_cast<int64_t>(b) * a.Hq + hi) * a.Tq + ti;
     const float m = fin[r][0], l = fin[r][1];
     float x = 0.0f;
@@ -529,9 +523,7 @@ __global__ void __launch_bounds__(kAttnThreads)
   const Kv8Cache& c = a.c;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int split = blockIdx.x, b = blockIdx.z;
-  const int rows = a.G * a.Tq;
-  const int row_tiles = (rows + 15) >> 4;
-  const int h = blockIdx.y / row_tiles, r0 = (blockIdx.y - h * row_tiles) * 16;
+  const int rows = a.G * a.Tq, h = blockIdx.y;  // at most 16 rows
   const int cap = c.max_blocks << c.log_t;
   const int len = min(max(a.lens[b], 0), cap);
 
@@ -540,15 +532,13 @@ __global__ void __launch_bounds__(kAttnThreads)
   int64_t q_at[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = min(r0 + g + 8 * i, rows - 1);
+    const int r = min(g + 8 * i, rows - 1);
     const int ti = r / a.G, hi = h * a.G + (r - ti * a.G);
-    lim[i] = a.causal ? min(max(len - a.Tq + ti + 1, 0), len) : len;
+    lim[i] = attn_limit(a, len, ti);
     q_at[i] = b * a.qb + hi * a.qh + ti * a.qt;
   }
   // the tile's last row sees the most, its first the least
-  const int last = min(r0 + 15, rows - 1);
-  const int lim_max = a.causal ? min(max(len - a.Tq + last / a.G + 1, 0), len) : len;
-  const int lim_min = a.causal ? min(max(len - a.Tq + r0 / a.G + 1, 0), len) : len;
+  const int lim_max = attn_limit(a, len, (rows - 1) / a.G), lim_min = attn_limit(a, len, 0);
   const int tiles = (lim_max + 15) >> 4;  // 16-token tiles to visit
   const int chunks = (tiles + kAttnWarps - 1) / kAttnWarps;
   const int c0 = static_cast<int>(static_cast<int64_t>(chunks) * split / a.splits);
@@ -650,7 +640,7 @@ __global__ void __launch_bounds__(kAttnThreads)
       for (int j = 0; j < 4; ++j) {
         const int r = j >> 1;
         // a masked score is exactly -inf; a NaN one (NaN q or scales) stays NaN
-        p[j] = s[i][j] == -INFINITY ? 0.0f : ex2f(s[i][j] - m[r]);
+        p[j] = s[i][j] == -INFINITY ? 0.0f : ex2_approx(s[i][j] - m[r]);
         l[r] = fmaf(p[j], iv, l[r]);
       }
       pf[2 * i] = zero_v ? 0u : pack_f16x2(p[0], p[1]);
@@ -707,7 +697,7 @@ __global__ void __launch_bounds__(kAttnThreads)
           buf->o[warp][g + 8 * r][AttnOut<D, 16>::at((2 * t + j) * (D / 8) + i)] = o[i][2 * r + j] * f;
     }
   }
-  attn_epilogue<D, 16>(a, buf, sm_ml, sm_fin, b, h, split, r0, min(16, rows - r0));
+  attn_epilogue<D, 16>(a, buf, sm_ml, sm_fin, b, h, split, rows);
 }
 
 // ---- up to 8 rows per key/value head (one token of up to 8 grouped heads)
@@ -875,7 +865,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
     float p[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)  // a masked score is exactly -inf; a NaN one stays NaN
-      p[i] = s[i] == -INFINITY ? 0.0f : ex2f(s[i] - m);
+      p[i] = s[i] == -INFINITY ? 0.0f : ex2_approx(s[i] - m);
     l = fmaf((p[0] + p[1]) + (p[2] + p[3]), iv, l);
     const uint32_t pb0 = zero_v ? 0u : pack_f16x2(p[0], p[1]), pb1 = zero_v ? 0u : pack_f16x2(p[2], p[3]);
     attn_read_v<D>(ring->v[s_] + warp * 16 * D, g, t, vw);
@@ -917,7 +907,7 @@ __global__ void __launch_bounds__(kAttnThreads, 3)
           buf->o[warp][2 * t + j][AttnOut<D, 8>::at(g * (D / 8) + 2 * i + r)] = o[i][2 * r + j] * f;
     }
   }
-  attn_epilogue<D, 8>(a, buf, sm_ml, sm_fin, b, h, split, 0, rows);
+  attn_epilogue<D, 8>(a, buf, sm_ml, sm_fin, b, h, split, rows);
 }
 
 // Joins up to 8 splits of each row, one warp per row.

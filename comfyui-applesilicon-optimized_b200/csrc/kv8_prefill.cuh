@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(128 * RT + 192, RT == 2 ? 1 : 2)
           float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float px = ex2f(fmaf(__uint_as_float(r[16 * q + i]), ksc[u], shift));
-            const float py = ex2f(fmaf(__uint_as_float(r[16 * q + i + 1]), ksc[u], shift));
+            const float px = ex2_approx(fmaf(__uint_as_float(r[16 * q + i]), ksc[u], shift));
+            const float py = ex2_approx(fmaf(__uint_as_float(r[16 * q + i + 1]), ksc[u], shift));
             sum += px + py;
             p[8 * q + (i >> 1)] = zero ? 0u : pack_f16x2(px, py);
           }

@@ -35,11 +35,10 @@ constexpr int64_t kIntMax = (int64_t(1) << 31) - 1;
 bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A launch with optional dynamic shared memory and cluster size, as a
-// programmatic dependent of the kernel before it (B200Q_PDL=0: plainly).
+// A launch with optional dynamic shared memory, as a programmatic dependent of the kernel
+// before it (B200Q_PDL=0: plainly).
 template <typename... KArgs, typename... Args>
-int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, cudaStream_t st,
-           Args... args) {
+int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, cudaStream_t st, Args... args) {
   if (smem > 48 * 1024 &&
       cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
@@ -50,20 +49,11 @@ int launch(void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, 
   cfg.blockDim = dim3(static_cast<unsigned>(block));
   cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  int n = 0;
-  if (host::pdl_on()) {
-    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster > 1) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = static_cast<unsigned>(cluster);
-    at[n].val.clusterDim.y = 1;
-    at[n++].val.clusterDim.z = 1;
-  }
-  cfg.attrs = at;
-  cfg.numAttrs = n;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = host::pdl_on() ? 1 : 0;
   cudaLaunchKernelEx(&cfg, kern, args...);  // errors surface in finish_launch
   return host::finish_launch();
 }
@@ -102,16 +92,16 @@ bool ws_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WsPlan* p) {
 int launch_join(const float* part, int slices, int64_t ld, const EpiArgs& ep, cudaStream_t st) {
   const int64_t chunks = cdiv(ep.N, 256);
   if (ep.M * chunks > kIntMax) return B200Q_ERR_UNSUPPORTED;
-  return launch(w4_join_kernel, dim3(static_cast<unsigned>(ep.M * chunks)), 256, 0, 1, st, part, slices, ld,
+  return launch(w4_join_kernel, dim3(static_cast<unsigned>(ep.M * chunks)), 256, 0, st, part, slices, ld,
                 static_cast<int>(chunks), ep);
 }
 
 template <int LW>
 int launch_slice_cols(const W4SliceArgs& a, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.slices * p.parts));
-  if (a.M <= 8) return launch(w4_slice_kernel<LW, 1>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
-  if (a.M <= 16) return launch(w4_slice_kernel<LW, 2>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
-  return launch(w4_slice_kernel<LW, 4>, grid, kWsWarps * 32, p.smem, 1, st, a, ep);
+  if (a.M <= 8) return launch(w4_slice_kernel<LW, 1>, grid, kWsWarps * 32, p.smem, st, a, ep);
+  if (a.M <= 16) return launch(w4_slice_kernel<LW, 2>, grid, kWsWarps * 32, p.smem, st, a, ep);
+  return launch(w4_slice_kernel<LW, 4>, grid, kWsWarps * 32, p.smem, st, a, ep);
 }
 int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p, cudaStream_t st) {
   int s = G == 32   ? launch_slice_cols<1>(a, ep, p, st)
@@ -149,9 +139,9 @@ bool wd_plan(int sms, int64_t M, int64_t N, int64_t K, int G, WdPlan* p) {
 template <typename T, int LW>
 int launch_digits_cols(const W4DigitArgs& a, const EpiArgs& ep, const WdPlan& p, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(p.grid));
-  if (a.M <= 2) return launch(w4_digit_kernel<T, LW, 1>, grid, p.threads, p.smem, 1, st, a, ep);
-  if (a.M <= 5) return launch(w4_digit_kernel<T, LW, 2>, grid, p.threads, p.smem, 1, st, a, ep);
-  return launch(w4_digit_kernel<T, LW, 3>, grid, p.threads, p.smem, 1, st, a, ep);
+  if (a.M <= 2) return launch(w4_digit_kernel<T, LW, 1>, grid, p.threads, p.smem, st, a, ep);
+  if (a.M <= 5) return launch(w4_digit_kernel<T, LW, 2>, grid, p.threads, p.smem, st, a, ep);
+  return launch(w4_digit_kernel<T, LW, 3>, grid, p.threads, p.smem, st, a, ep);
 }
 template <typename T>
 int launch_digits(const W4DigitArgs& a, int G, const EpiArgs& ep, const WdPlan& p, cudaStream_t st) {
@@ -227,7 +217,7 @@ W4TileWork w4_tile_work(const W4TilePlan& p, int64_t M, int64_t N, int64_t K, in
 template <int TN, bool LO>
 int launch_tile(const CUtensorMap& tx, const CUtensorMap& tw, const W4TileArgs& a, const EpiArgs& ep, int64_t ctas,
                 cudaStream_t st) {
-  return launch(w4_tile_kernel<TN, LO>, dim3(static_cast<unsigned>(ctas)), kW4TileThreads, w4_tile_smem_bytes<TN>(), 1,
+  return launch(w4_tile_kernel<TN, LO>, dim3(static_cast<unsigned>(ctas)), kW4TileThreads, w4_tile_smem_bytes<TN>(),
                 st, tx, tw, a, ep);
 }
 int launch_w4_tile(const W4TilePlan& p, const void* x, int x_dtype, int64_t ldx, bool x_vec, const uint8_t* w,
@@ -255,7 +245,7 @@ int launch_w4_tile(const W4TilePlan& p, const void* x, int x_dtype, int64_t ldx,
   r.w_pow = reinterpret_cast<float*>(base + o.w_pow);
   r.group_blocks = static_cast<int>(cdiv(r.groups, kW4PrepGroups));
   r.scale_blocks = r.ldn / kW4PrepRows * r.group_blocks;
-  int s = launch(w4_tile_prepare_kernel, dim3(static_cast<unsigned>(r.scale_blocks + M)), 256, 0, 1, st, r);
+  int s = launch(w4_tile_prepare_kernel, dim3(static_cast<unsigned>(r.scale_blocks + M)), 256, 0, st, r);
   if (s != B200Q_OK) return s;
   CUtensorMap tx, tw;
   if (!host::tmap_u8(&tx, r.x16, uint64_t(2 * K), uint64_t(M), uint64_t(2 * K), 128, static_cast<uint32_t>(p.tn),
@@ -322,7 +312,7 @@ int launch_persistent(K kern, const NormArgs& a, int threads, int smem, int sms,
     return B200Q_ERR_CUDA;
   }
   const int64_t ctas = int64_t(sms) * per_sm;
-  return launch(kern, dim3(static_cast<unsigned>(a.rows < ctas ? a.rows : ctas)), threads, smem, 1, st, a);
+  return launch(kern, dim3(static_cast<unsigned>(a.rows < ctas ? a.rows : ctas)), threads, smem, st, a);
 }
 template <int DTYPE, int VW>
 int launch_norm_loose(const NormArgs& a, int sms, cudaStream_t st) {
@@ -336,7 +326,7 @@ template <int DTYPE, bool PERSIST, int NPT, bool FULL, bool QUANT, bool AFTER>
 int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
   auto kern = block_norm_rows_kernel<DTYPE, PERSIST, NPT, FULL, QUANT, AFTER>;
   if (PERSIST) return launch_persistent(kern, a, threads, (AFTER ? 3 : 2) * a.D * 4, sms, st);
-  return launch(kern, dim3(static_cast<unsigned>(a.rows)), threads, 0, 1, st, a);
+  return launch(kern, dim3(static_cast<unsigned>(a.rows)), threads, 0, st, a);
 }
 template <int DTYPE, bool PERSIST, int NPT, bool FULL>
 int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
@@ -368,8 +358,8 @@ int launch_norm(const NormArgs& a, bool vec, bool pairs, int sms, cudaStream_t s
                     : launch_norm_rows<DTYPE, true, 2>(a, threads, sms, st);
   }
   if (a.D <= 8192) return pairs ? launch_norm_loose<DTYPE, 2>(a, sms, st) : launch_norm_loose<DTYPE, 1>(a, sms, st);
-  return launch(block_norm_kernel<DTYPE, 1, 32>, dim3(static_cast<unsigned>(a.rows)),
-                static_cast<int>(cdiv(cdiv(a.D, 32), 32) * 32), 0, 1, st, a);
+  return launch(block_norm_kernel<DTYPE, 32>, dim3(static_cast<unsigned>(a.rows)),
+                static_cast<int>(cdiv(cdiv(a.D, 32), 32) * 32), 0, st, a);
 }
 
 // ------------------------------------------------------------ 8-bit cache
@@ -403,10 +393,10 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
   const dim3 grid(static_cast<unsigned>(cdiv(a.S + a.c.T - 1, a.c.T)), static_cast<unsigned>(a.c.heads),
                   static_cast<unsigned>(2 * a.B));
   const int vecs = a.c.T * a.c.D / 8;
-  if (vecs <= kKvThreads) return launch(kv8_append_kernel<T, 1>, grid, kKvThreads, 0, 1, st, a);
-  if (vecs <= 2 * kKvThreads) return launch(kv8_append_kernel<T, 2>, grid, kKvThreads, 0, 1, st, a);
-  if (vecs <= 4 * kKvThreads) return launch(kv8_append_kernel<T, 4>, grid, kKvThreads, 0, 1, st, a);
-  return launch(kv8_append_kernel<T, 8>, grid, kKvThreads, 0, 1, st, a);
+  if (vecs <= kKvThreads) return launch(kv8_append_kernel<T, 1>, grid, kKvThreads, 0, st, a);
+  if (vecs <= 2 * kKvThreads) return launch(kv8_append_kernel<T, 2>, grid, kKvThreads, 0, st, a);
+  if (vecs <= 4 * kKvThreads) return launch(kv8_append_kernel<T, 4>, grid, kKvThreads, 0, st, a);
+  return launch(kv8_append_kernel<T, 8>, grid, kKvThreads, 0, st, a);
 }
 
 // How many CTAs share a sequence's length.  Up to 16 rows a head: enough to give every
@@ -569,7 +559,7 @@ int b200q_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* w
     x = a.x16;
     ldx = K;
   }
-  int s = launch(w4_prepare_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, 1, st, a);
+  int s = launch(w4_prepare_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, a);
   if (s != B200Q_OK) return s;
   if (!w4_joins(N)) return host::gemm_f16_scaled(x, ldx, a.w16, K, M, N, K, ep, st);
   EpiArgs sums = ep;
@@ -677,7 +667,7 @@ int b200q_kv8_gather(const int8_t* k_codes, const int8_t* v_codes, const float* 
   a.B = static_cast<int>(B); a.S = static_cast<int>(S);
   const dim3 grid(static_cast<unsigned>(cdiv(S * (D / 8), kKvThreads * kGatherVecs)), static_cast<unsigned>(heads),
                   static_cast<unsigned>(2 * B));
-  return launch(kv8_gather_kernel, grid, kKvThreads, 0, 1, static_cast<cudaStream_t>(stream), a);
+  return launch(kv8_gather_kernel, grid, kKvThreads, 0, static_cast<cudaStream_t>(stream), a);
 }
 
 size_t b200q_kv8_attention_workspace_size(int64_t B, int64_t Hq, int64_t heads, int64_t Tq,
@@ -742,27 +732,27 @@ int b200q_kv8_attention(const void* q, int dtype, int64_t B, int64_t Hq, int64_t
   // up to 8 rows a head: integer q.K and transposed P V (see kv8_attn8_kernel); more
   // than 16: 128-row tiles on tcgen05
   if (a.G * Tq > kPfRows) {
-    s = D == 128 ? launch(kv8_prefill_kernel<128, 2>, grid, pf_threads(2), pf_smem_bytes<128, 2>(), 1, st, tk, tv, a)
-                 : launch(kv8_prefill_kernel<64, 2>, grid, pf_threads(2), pf_smem_bytes<64, 2>(), 1, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_prefill_kernel<128, 2>, grid, pf_threads(2), pf_smem_bytes<128, 2>(), st, tk, tv, a)
+                 : launch(kv8_prefill_kernel<64, 2>, grid, pf_threads(2), pf_smem_bytes<64, 2>(), st, tk, tv, a);
   } else if (a.G * Tq > 16) {
-    s = D == 128 ? launch(kv8_prefill_kernel<128, 1>, grid, pf_threads(1), pf_smem_bytes<128, 1>(), 1, st, tk, tv, a)
-                 : launch(kv8_prefill_kernel<64, 1>, grid, pf_threads(1), pf_smem_bytes<64, 1>(), 1, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_prefill_kernel<128, 1>, grid, pf_threads(1), pf_smem_bytes<128, 1>(), st, tk, tv, a)
+                 : launch(kv8_prefill_kernel<64, 1>, grid, pf_threads(1), pf_smem_bytes<64, 1>(), st, tk, tv, a);
   } else if (a.G * Tq <= 8) {
-    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
-                 : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_attn8_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), st, tk, tv, a)
+                 : launch(kv8_attn8_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), st, tk, tv, a);
   } else {
-    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), 1, st, tk, tv, a)
-                 : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), 1, st, tk, tv, a);
+    s = D == 128 ? launch(kv8_attn_kernel<128>, grid, kAttnThreads, attn_smem_bytes<128>(), st, tk, tv, a)
+                 : launch(kv8_attn_kernel<64>, grid, kAttnThreads, attn_smem_bytes<64>(), st, tk, tv, a);
   }
   if (s != B200Q_OK || !need) return s;
   if (splits <= 8) {
     const dim3 few(static_cast<unsigned>(cdiv(rows, 8)));
-    return D == 128 ? launch(kv8_attn_join_few_kernel<128>, few, 256, 0, 1, st, a)
-                    : launch(kv8_attn_join_few_kernel<64>, few, 256, 0, 1, st, a);
+    return D == 128 ? launch(kv8_attn_join_few_kernel<128>, few, 256, 0, st, a)
+                    : launch(kv8_attn_join_few_kernel<64>, few, 256, 0, st, a);
   }
   const dim3 jgrid(static_cast<unsigned>(rows));
-  return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, kJoinWarps * 32, 0, 1, st, a)
-                  : launch(kv8_attn_join_kernel<64>, jgrid, kJoinWarps * 32, 0, 1, st, a);
+  return D == 128 ? launch(kv8_attn_join_kernel<128>, jgrid, kJoinWarps * 32, 0, st, a)
+                  : launch(kv8_attn_join_kernel<64>, jgrid, kJoinWarps * 32, 0, st, a);
 }
 
 }  // extern "C"
