@@ -57,9 +57,8 @@ constexpr int kKvThreads = 256;
 // the scale's reciprocal and one correction by its remainder, which gives the rounded
 // quotient (16-bit values are often exact ties, half of the block's largest among them),
 // and the nearest integer is the low byte of its sum with 1.5 * 2^23: the divide's
-// branches and the clamping cost twice the memory's time.  With the gather of the touched
-// blocks: one token for each of 64 sequences 8.8 us (two launches' latency), two prompts of
-// up to 8191 tokens 42 us, 0.64 of the copy rate.
+// branches and the clamping cost twice the memory's time.  Two prompts of 8191 tokens, 8
+// heads: 26 us, 0.60 of the copy rate (issue 63%); one token for each of 64 sequences 4 us.
 template <typename T, int NV>
 __global__ void __launch_bounds__(kKvThreads) kv8_append_kernel(const Kv8AppendArgs a) {
   __shared__ uint32_t wmax[kKvThreads / 32];
@@ -167,7 +166,8 @@ struct Kv8GatherArgs {
 };
 
 // Four vectors of 8 codes per thread, their loads in flight together; grid (vectors of
-// a head, heads, 2 B).  Bound: HBM.
+// a head, heads, 2 B).  Bound: HBM (two times 8191 tokens, 8 heads: 16 us, 0.94 of the copy
+// rate).
 constexpr int kGatherVecs = 4;
 __global__ void __launch_bounds__(kKvThreads) kv8_gather_kernel(const Kv8GatherArgs a) {
   griddep_wait();
@@ -714,8 +714,9 @@ __global__ void __launch_bounds__(kAttnThreads)
 // 8 columns: half the MMAs and accumulators of the 16-row form.
 //
 // Bound: HBM for long caches.  32 sequences of 0 to 32767 tokens, 8 heads of 8 rows, D 128:
-// 198 us, 5.4 TB/s, 0.83 of the measured copy; one sequence of 8193 tokens, 5 rows: 9.9 us,
-// of which the splits' join and two launches' latency are half.
+// 198 to 202 us in a captured graph, 0.82 of the measured copy, 214 (0.77) among eager calls;
+// one sequence of 8193 tokens, 5 rows: 9.8 us (11.2), of which the splits' join and two
+// launches' latency are half.
 __device__ __forceinline__ void mma_s8_start(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   const int z = 0x4B400000;
   asm(

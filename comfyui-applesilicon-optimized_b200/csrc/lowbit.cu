@@ -112,9 +112,12 @@ int launch_slice(const W4SliceArgs& a, int G, const EpiArgs& ep, const WsPlan& p
 }
 
 // The integer kernel for few tokens, when x's digits fit beside the rings.  (Against the slice
-// kernel, N 5120, us: 1 token K 1536 4.4 / 7.8, K 5120 7.5 / 11.3; 2 tokens K 5120 10.3 / 11.8;
-// 3 tokens K 1536 7.3 / 7.9, K 2560 9.5 / 9.7, K 5120 14.4 / 11.7; 5 tokens K 1536 8.0 / 8.0;
-// 8 tokens K 1536 9.2 / 8.4: more than two tokens while M * K is small.)
+// kernel, us.  1 token, N 1024 / 5120 / 13824: K 5120 4.5 7.9 11.8 against 7.3 11.5 17.4, K
+// 13824 9.3 15.0 21.2 against 9.9 18.3 33.7, K 24576 13.7 23.7 33.3 against 10.9 27.6 51.9; 2
+// tokens: K 5120 5.4 8.2 12.1 against 7.2 12.1 17.6, K 12288 10.8 15.1 20.1 against 9.4 17.3
+// 28.8: longer rows lose at narrow N only.  N 5120: 3 tokens K 1536 5.4 / 7.5, K 2560 8.0 / 9.5,
+// K 5120 14.4 / 12.2; 5 tokens K 1536 6.8 / 7.6; 8 tokens K 1024 6.9 / 6.9, K 1536 9.2 / 8.0:
+// more than two tokens while M * K is small.)
 struct WdPlan {
   int smem, grid, threads;
 };
@@ -171,9 +174,9 @@ W4Work w4_work(int64_t M, int64_t N, int64_t K) {
 }
 
 // 33 to 256 tokens: one token tile of the tile kernel.  (Measured at K 5120, N 13824: 64 tokens
-// 52 us, 64 on the slice kernel in two passes; 256 tokens 69 us, 80 decoded; K 13824, N 5120:
-// 200 tokens 58 us, 129 decoded.  With more token tiles the weight is decoded again for each,
-// and the decoded copy with the pair GEMM is ahead: 300 tokens 101 us, 164 by tiles.)
+// 50 us, 64 on the slice kernel in two passes; 256 tokens 63 us, 80 decoded; K 13824, N 5120:
+// 200 tokens 56 us, 129 decoded.  With more token tiles the weight is decoded again for each,
+// and the decoded copy with the pair GEMM is ahead: 300 tokens 98 us, 164 by tiles.)
 constexpr int64_t kW4MaxTileM = 256;
 bool w4_tiles(int64_t M, int64_t N, int64_t K) {
   return M <= kW4MaxTileM && N <= (int64_t(1) << 30) && K <= (int64_t(1) << 24);
@@ -341,8 +344,9 @@ int launch_norm_rows(const NormArgs& a, int threads, int sms, cudaStream_t st) {
                                   : launch_norm_rows<DTYPE, PERSIST, NPT, false>(a, threads, sms, st);
 }
 // Aligned rows of up to 8192 values: one row per CTA and one 8-value vector per thread
-// while all rows find a place at once (296 rows of 5120: 8.0 us, 297 persistent 8.3), else persistent CTAs with four vectors per
-// thread (two for short rows: fewer reductions per value, more CTAs per SM).  Other rows
+// while all rows find a place at once (after + before, 296 rows of 5120: 7.7 us, 297 persistent
+// 8.2), else persistent CTAs with four vectors per thread (two for short rows: fewer reductions
+// per value, more CTAs per SM).  Other rows
 // of up to 8192 values: persistent CTAs, by pairs or single values.  Longer ones take the
 // form of 32 single values per thread.
 template <int DTYPE>
@@ -405,9 +409,9 @@ int launch_append(const Kv8AppendArgs& a, cudaStream_t st) {
 // rounds of stages.  More than one leave fp32 partials for the join kernel.  (A cluster
 // of up to 16 CTAs joining over distributed shared memory was no faster: 8 heads x 2048
 // tokens 7.4 us against 7.1, 8193 tokens 12.7 against 10.0.)
-// Row tiles: 8 rows of 32 x 4096 tokens take 71 us on their kernel, 9 rows 80 on the 16-row one and
-// 16 rows 84; a second 16-row tile would read the cache again, and 17 rows take 134 us on the
-// 128-row tiles.  129 rows: 238 us with 256-row tiles, 128 rows 159 us.
+// Row tiles: 8 rows of 32 x 4096 tokens take 71 us on their kernel, 9 rows 79 on the 16-row one and
+// 16 rows 83; a second 16-row tile would read the cache again, and 17 rows take 129 us on the
+// 128-row tiles, 128 rows 144.  129 rows: 239 us with 256-row tiles.
 int attn_row_tile(int64_t rows) { return rows <= 16 ? 16 : rows <= kPfRows ? kPfRows : 2 * kPfRows; }
 int attn_splits(int sms, int64_t B, int64_t Hq, int64_t heads, int64_t Tq, int64_t max_len) {
   const int64_t rows = Hq / heads * Tq;

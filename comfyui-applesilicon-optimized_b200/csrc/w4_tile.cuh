@@ -15,9 +15,9 @@
 // brings x, warp 18 the codes and the scales; warp 17 issues the MMAs.
 //
 // Bound: per stage and SM, x's TN * 128 bytes from L2 (64 bytes a cycle) against the MMAs'
-// 2 * TN cycles and the decode.  K 5120, N 13824, 64 tokens: 52 us, 11 of them the operand
+// 2 * TN cycles and the decode.  K 5120, N 13824, 64 tokens: 50 us, 11 of them the operand
 // kernel, 0.33 us per stage of which half stays with decode and MMAs taken out (x from L2
-// into 108 SMs); 256 tokens: 69 us.  K 13824, N 5120, 200 tokens: 58 us.
+// into 108 SMs); 256 tokens: 63 us.  K 13824, N 5120, 200 tokens: 56 us.
 #pragma once
 
 #include "kv8_prefill.cuh"

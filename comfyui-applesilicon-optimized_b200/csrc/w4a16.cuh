@@ -95,6 +95,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
   return r;
 }
+// Nibbles become fp16 by their place in the mantissa of a constant power of two, a published
+// method (Kim, Henry, Fahim and Awadalla, "Who Says Elephants Can't Run: Bringing Large Scale
+// MoE Models into Cloud Scale Production", 2022).
 // A row's zero point for w4_decode: 1024 + z (low half) and -(64 + z) as fp16.
 __device__ __forceinline__ uint32_t w4_zero(uint32_t z) { return 0xD4006400u | (z << 20) | z; }
 
@@ -124,8 +127,8 @@ __device__ __forceinline__ void w4_decode(uint32_t w, uint32_t z0, uint32_t z1, 
 // and stage, scales travelling along.
 //
 // Bound: the instructions per weight word (unpacking, 2 MMAs per 8 tokens) and the ring's
-// latency.  16 tokens, K 13824, N 5120: 20.9 us, 1.7 TB/s of codes; 32 tokens, K 5120, N
-// 13824: 32.5 us.  TMA boxes instead of cp.async were slower (one issuer per CTA).
+// latency.  16 tokens, K 13824, N 5120: 21 us, 1.7 TB/s of codes; 32 tokens, K 5120, N
+// 13824: 30 us.  TMA boxes instead of cp.async were slower (one issuer per CTA).
 constexpr int kWsWarps = 16;
 constexpr int kWsStages = 3;  // issue() relies on three
 
@@ -413,8 +416,8 @@ __global__ void __launch_bounds__(256)
 // stores them while the others go on.
 //
 // Bound: x's digits and the first loads for small weights, issue for large ones.  1 token,
-// K = N = 5120, G 128: 6.3 us (2.1 TB/s of codes, 0.33 of the floor); K 5120, N 13824, G 64
-// with zero points and GELU: 13.8 us (2.6 TB/s, 0.43).  fp16 MMAs took 23 us for the latter.
+// K = N = 5120, G 128: 6.4 us (2.1 TB/s of codes, 0.32 of the floor); K 5120, N 13824, G 64
+// with zero points and GELU: 14.0 us (2.5 TB/s, 0.42).  fp16 MMAs took 23 us for the latter.
 constexpr int kWdStages = 3;  // issue() relies on three
 // Most teams per CTA, by the digit columns' register need.
 constexpr int wd_teams(int nc) { return nc == 3 ? 2 : 3; }

@@ -2,7 +2,7 @@
 
 ``k_codes``, ``v_codes`` [pages, heads, T, D] int8 hold the tokens' values in pages
 of T tokens (16, 32, 64 or 128; D 64 or 128), ``k_scale``, ``v_scale`` [pages, heads]
-fp32 one scale for each page and head: value = code * scale.  ``block_table``
+fp32 one scale (not negative) for each page and head: value = code * scale.  ``block_table``
 [B, max_blocks] int32 gives the page of each block of T tokens of a sequence.
 
 * ``kv8_append`` writes new tokens behind each sequence's length.  A block's scale

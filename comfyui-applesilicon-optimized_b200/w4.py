@@ -63,7 +63,9 @@ def w4a16_linear(x, w, scales, zeros=None, bias=None, act=None, out_dtype=None):
     act: None / "none", "gelu_tanh" or "gelu".  Up to 256 tokens run on kernels that
     read the 4-bit weight as stored (up to 32 with exact products, above that with each
     weight rounded to fp16's 11 bits); more decode it once per call, rounded alike, for
-    the 16-bit tile GEMM."""
+    the 16-bit tile GEMM.  One and two tokens are fastest with scales of x's type.  A
+    token that holds an infinity or NaN gives infinities or NaN and no other token does
+    (of one or two tokens: NaN in either case)."""
     f = _w4a16 or _load()
     return f(x, w, scales, zeros, bias, act, out_dtype)
 
