@@ -719,8 +719,9 @@ __global__ void __launch_bounds__(NC == 3 ? 512 : 768) w4_digit_kernel(const W4D
 // bf16 token rows: x * 2^-e, 2^e the power of two of the row's largest |x|, to
 // x_pow[m] for the GEMM's row scale.  Exact down to 2^-17 of the row's maximum, within
 // 2^-25 of it below.  The GEMM multiplies by the row's power before the column's: 2^-22 of
-// the former is kept for the scalar that comes last, so that sums of up to 2^17 times rows
-// near fp32's largest value pass through finite numbers.
+// the former is kept for the scalar that comes last, so that sums of up to 2^23 times rows
+// near fp32's largest value pass through finite numbers (and rows below 2^-105 lose bits of
+// outputs near 2^-128).
 //
 // Bound: memory (half a byte read and two written per weight): 46 us for 13824 x 5120 and
 // 2047 tokens, 4.4 TB/s; the product then takes 190 us, 0.93 of the measured GEMM rate.
